@@ -1,0 +1,48 @@
+// Weights of 4 bits with group scales: their layout, and what the kernels that read them share.
+//
+//   W[f, k] = scale[f, k / group] * (code[f, k] - zero[f, k / group]),   code 0 .. 15, zero 0 .. 15 (8 where there is none), group 32, 64 or 128
+//
+// A matrix is cut into strips of 16 rows and steps of 128 along K (skein_b200/ops/int4.py packs it; rows and K are padded). For a pair of
+// matrices (gate and up of a SwiGLU) a strip holds 8 gate rows and the 8 up rows of the same features, so that whoever holds accumulator
+// row r of a strip has its partner at r + 8.
+//   codes  [strip][step][2][lane 32][16 bytes]: a lane (g = lane / 4, t = lane % 4) of half j owns rows g and g + 8 at k = 64 j + 8 t .. + 7 and
+//          64 j + 32 + 8 t .. + 7: words {row g, first; row g, second; row g + 8, first; row g + 8, second}. One 16-byte load of a warp is 16 rows x
+//          64 k in the order in which mma.sync's A operand wants them (any order of k is right as long as B has the same), and the row's eight
+//          codes of a word are neighbours in k, so that the tensor-memory kernel takes its rows from the same bytes.
+//          Inside a word the codes of even k are the low half's nibbles, those of odd k the high half's: (word >> 4 i) & 0x000f000f is the
+//          pair (k = 2 i, 2 i + 1).
+//   scales [strip][step][8][128 / group][2] 16-bit: rows g and g + 8 side by side; zeros the same in bytes.
+#pragma once
+#include "gemm_sched.cuh"
+#include "ptx.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace skein {
+
+constexpr int I4_STEP = 128;                       // elements of K
+constexpr int I4_STEP_BYTES = 16 * I4_STEP / 2;    // of one strip
+
+// code pair -> bf16 pair 128 + code: the codes are the low mantissa bits of a bf16 whose unit in the last place is 1
+__device__ __forceinline__ uint32_t i4_magic(uint32_t word, int i) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(word >> (4 * i)));
+  return r;
+}
+// (128 + code) - (128 + zero): both are whole numbers below 256, so the difference is exact in bf16
+__device__ __forceinline__ uint32_t i4_sub(uint32_t v, uint32_t base) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(base));
+  return r;
+}
+__device__ __forceinline__ void i4_expand(uint32_t word, uint32_t base, uint32_t (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = i4_sub(i4_magic(word, i), base);
+}
+// a zero as the pair that i4_sub takes
+__device__ __forceinline__ uint32_t i4_base(uint32_t zero) { return 0x43004300u | zero | (zero << 16); }
+__device__ __forceinline__ float i4_scale(uint32_t raw, bool half) {
+  return half ? __half2float(__ushort_as_half((unsigned short)raw)) : __uint_as_float(raw << 16);
+}
+
+}  // namespace skein

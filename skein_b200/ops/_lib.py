@@ -228,6 +228,10 @@ def lib():
     _sig(L, "skein_rec_channel", i32, [rec, chunk, i32, i32, vp])
     _sig(L, "skein_rec_channel_scratch_bytes", i64, [rec, i32, i32])
     _sig(L, "skein_rec_tail", i32, [rec, chunk, i32, i32, vp])
+    _sig(L, "skein_route_balanced_scratch", i64, [i32, i32])
+    _sig(L, "skein_route_balanced",
+         i32, [vp, i64, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp])
+    _sig(L, "skein_int4_rows", i32, [vp, i64, vp, vp, vp, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp])
     for name, rt, at in _OPTIONAL:
         if hasattr(L, name):
             _sig(L, name, rt, at)
@@ -252,6 +256,22 @@ def ptr(t) -> int | None:
 
 def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(t):
+    """Context in which the tensor's device is the current one (streams, allocations and launches follow it)."""
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def check(rc: int, what: str) -> None:

@@ -1,0 +1,239 @@
+"""Products with weights of 4 bits and group scales: W[f, k] = scale[f, k / group] (code[f, k] - zero[f, k / group]).
+
+Codes are 0 .. 15, a zero is 0 .. 15 (8 where there is none), a group is 32, 64 or 128 neighbours along K, scales are bf16 or fp16. Activations are
+bf16 and are not quantised; sums, the scales' products included, are fp32, and nothing is rounded before the result. Beside ops/fp8.py this is the other
+form of weights narrower than the activations: half its bytes, scales of finer groups.
+
+A weight is laid out once (`pack_weight` from codes, `quantize_weight` from a matrix) for the kernels: csrc/kernels/int4.cuh has the layout. On CPU the
+same mathematics run through the reference (dequantise, matmul; reference_int4.py).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, functional as F, reference_int4 as ri
+
+GROUPS = (32, 64, 128)
+STRIP, STEP = 16, 128      # rows and elements of K of a packed block
+MAX_EXPERTS = 65535
+
+
+class Int4Weight:
+    """codes uint8 [matrices, strips, steps, 1024], scale 16-bit [matrices, strips, steps, 8, 128 / group, 2], zero uint8 of the same shape or None
+    (csrc/kernels/int4.cuh). `shape` is the logical [rows, K] or [experts, rows, K]; `pair`: gate rows, then up rows, packed side by side for the
+    SwiGLU product."""
+
+    def __init__(self, codes, scale, zero, shape, group, pair):
+        self.codes, self.scale, self.zero = codes, scale, zero
+        self.shape, self.group, self.pair = tuple(shape), group, pair
+        self.device = codes.device
+        self.features = shape[-2] // 2 if pair else shape[-2]
+        self.flags = int(pair) | (2 if scale.dtype == torch.float16 else 0)
+
+    @property
+    def is_cuda(self):
+        return self.codes.is_cuda
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scale.numel() * 2 + (self.zero.numel() if self.zero is not None else 0)
+
+    def parts(self):
+        """(codes [..., rows, K / 2], scale [..., rows, K / group], zero or None) as pack_weight takes them."""
+        *lead, rows, K = self.shape
+        n, S, B = self.codes.shape[:3]
+        w = self.codes.view(torch.int32).view(n, S, B, 2, 8, 4, 2, 2).permute(0, 1, 6, 4, 2, 3, 7, 5)      # [n, S, half, g, B, j, h, t]
+        w = _rows_out(w.reshape(n, S, 2, 8, B * 16), self.pair, rows)[:, :, :K // 8]
+        codes = _interleave(w.contiguous()).view(torch.uint8).reshape(*lead, rows, K // 2)
+
+        def back(t):
+            u = t.permute(0, 1, 5, 3, 2, 4).reshape(n, S, 2, 8, -1)
+            return _rows_out(u, self.pair, rows)[:, :, :K // self.group].reshape(*lead, rows, K // self.group)
+        return codes, back(self.scale), None if self.zero is None else back(self.zero)
+
+    def dequant(self) -> torch.Tensor:
+        """The weight in fp32, in its logical shape."""
+        return ri.dequant(*self.parts(), self.group)
+
+    def copy_(self, src: "Int4Weight"):
+        """In-place update (hot swap keeps the storage that captured CUDA graphs point at)."""
+        if (src.shape, src.group, src.pair, src.scale.dtype, src.zero is None) != (self.shape, self.group, self.pair, self.scale.dtype, self.zero is None):
+            raise ValueError("int4 weight: another shape, group, pairing or type of scales")
+        self.codes.copy_(src.codes)
+        self.scale.copy_(src.scale)
+        if self.zero is not None:
+            self.zero.copy_(src.zero)
+        return self
+
+
+def _deinterleave(w):
+    """Words of eight codes in order -> codes of even k in the low half, of odd k in the high half."""
+    def squeeze(v):
+        v = (v | (v >> 4)) & 0x00FF00FF
+        return (v | (v >> 8)) & 0x0000FFFF
+    return squeeze(w & 0x0F0F0F0F) | (squeeze((w >> 4) & 0x0F0F0F0F) << 16)
+
+
+def _interleave(w):
+    def spread(v):
+        v = (v | (v << 8)) & 0x00FF00FF
+        return (v | (v << 4)) & 0x0F0F0F0F
+    return spread(w & 0xFFFF) | (spread((w >> 16) & 0xFFFF) << 4)
+
+
+def _rows_in(t, pair, strips):
+    """[n, rows, ...] -> [n, strips, 2, 8, ...], rows padded with zeros."""
+    n, rows = t.shape[:2]
+    parts = t.reshape(n, 2, rows // 2, *t.shape[2:]) if pair else t.unsqueeze(1)
+    pad = strips * (8 if pair else 16) - parts.shape[2]
+    if pad:
+        parts = torch.cat((parts, parts.new_zeros(*parts.shape[:2], pad, *parts.shape[3:])), 2)
+    if pair:
+        return parts.reshape(n, 2, strips, 8, *t.shape[2:]).transpose(1, 2)
+    return parts.reshape(n, strips, 2, 8, *t.shape[2:])
+
+
+def _rows_out(t, pair, rows):
+    """[n, strips, 2, 8, m] -> [n, rows, m]."""
+    n, S, _, _, m = t.shape
+    if pair:
+        return t.transpose(1, 2).reshape(n, 2, S * 8, m)[:, :, :rows // 2].reshape(n, rows, m)
+    return t.reshape(n, S * 16, m)[:, :rows]
+
+
+def pack_weight(codes, scale, zero=None, pair=False) -> Int4Weight:
+    """codes uint8 [rows, K / 2] or [experts, rows, K / 2], two to a byte (the even k in the low half); scale bf16 or fp16 [.., rows, K / group]; zero
+    uint8 of scale's shape, 0 .. 15, or None (all 8). pair: the first half of the rows are the gate, the second half the up projection of a SwiGLU."""
+    if codes.dim() not in (2, 3) or codes.dtype != torch.uint8 or codes.numel() == 0:
+        raise ValueError("int4 weight: codes must be uint8 [rows, K / 2] or [experts, rows, K / 2]")
+    *lead, rows, half = codes.shape
+    K = 2 * half
+    if scale.dtype not in (torch.bfloat16, torch.float16) or scale.shape[:-1] != codes.shape[:-1] or scale.shape[-1] == 0 or K % scale.shape[-1]:
+        raise ValueError("int4 weight: scale must be bf16 or fp16 [.., rows, K / group]")
+    group = K // scale.shape[-1]
+    if group not in GROUPS:
+        raise ValueError(f"int4 weight: groups of {group}; they are {GROUPS}")
+    if zero is not None:
+        if zero.dtype != torch.uint8 or zero.shape != scale.shape:
+            raise ValueError("int4 weight: zero must be uint8 of scale's shape")
+        if int(zero.max()) > 15:
+            raise ValueError("int4 weight: zeros are 0 .. 15")
+    if pair and rows % 2:
+        raise ValueError("int4 weight: a pair has as many up rows as gate rows")
+    if any(t is not None and t.device != codes.device for t in (scale, zero)):
+        raise ValueError("int4 weight: codes, scale and zero lie on different devices")
+    n = lead[0] if lead else 1
+    if n > MAX_EXPERTS:
+        raise ValueError(f"int4 weight: at most {MAX_EXPERTS} experts")
+    S = -(-(rows // 2) // 8) if pair else -(-rows // 16)
+    B = -(-K // STEP)
+    w = _rows_in(_deinterleave(codes.reshape(n, rows, half).contiguous().view(torch.int32)), pair, S)        # [n, S, half, g, K / 8]
+    w = torch.nn.functional.pad(w, (0, B * 16 - w.shape[-1])) if w.shape[-1] < B * 16 else w
+    w = w.reshape(n, S, 2, 8, B, 2, 2, 4).permute(0, 1, 4, 5, 3, 7, 2, 6).contiguous()                       # [n, S, B, j, g, t, half, h]
+    per = STEP // group
+
+    def lay(t):
+        t = _rows_in(t.reshape(n, rows, -1), pair, S)
+        if t.shape[-1] < B * per:
+            t = torch.nn.functional.pad(t, (0, B * per - t.shape[-1]))
+        return t.reshape(n, S, 2, 8, B, per).permute(0, 1, 4, 3, 5, 2).contiguous()
+    return Int4Weight(w.view(n, S, B, -1).view(torch.uint8), lay(scale), None if zero is None else lay(zero), (*lead, rows, K), group, bool(pair))
+
+
+def quantize_weight(w: torch.Tensor, group: int = 128, symmetric: bool = True, pair: bool = False) -> Int4Weight:
+    """Nearest codes of a weight [rows, K] or [experts, rows, K]. symmetric: a group's scale maps its largest magnitude to 7 (codes 1 .. 15 around 8);
+    else scale and zero map its range, zero included, onto 0 .. 15. Scales are bf16. K must be a multiple of the group."""
+    if w.dim() not in (2, 3) or group not in GROUPS or w.shape[-1] % group:
+        raise ValueError(f"int4 weight: [.., rows, K] with K a multiple of the group ({GROUPS})")
+    v = w.float().unflatten(-1, (-1, group))
+    if symmetric:
+        s, zero = v.abs().amax(-1) / 7, None
+    else:
+        lo, hi = v.amin(-1).clamp(max=0), v.amax(-1).clamp(min=0)
+        s = (hi - lo) / 15
+    s = torch.where(s > 0, s, torch.ones_like(s)).to(torch.bfloat16)
+    if not symmetric:
+        zero = (-lo / s.float()).round().clamp(0, 15).to(torch.uint8)
+    z = 8.0 if zero is None else zero.float()[..., None]
+    q = ((v / s.float()[..., None]).round() + z).clamp(0, 15).to(torch.uint8).flatten(-2)
+    return pack_weight(q[..., 0::2] | (q[..., 1::2] << 4), s, zero, pair)
+
+
+def _check(what, x, w: Int4Weight, pair, dims):
+    if not isinstance(w, Int4Weight) or len(w.shape) != dims:
+        raise ValueError(f"{what}: the weight must be an Int4Weight of {dims} dimensions")
+    if w.pair != pair:
+        raise ValueError(f"{what}: the weight is {'' if w.pair else 'not '}packed as a gate / up pair")
+    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != w.shape[-1] or x.stride(1) != 1:
+        raise ValueError(f"{what}: x must be bf16 [rows, {w.shape[-1]}] with contiguous rows")
+    if x.device != w.device:
+        raise ValueError(f"{what}: x is on {x.device}, the weight on {w.device}")
+
+
+def _out(what, out, rows, w, dtype, device):
+    if out is None:
+        return torch.empty(rows, w.features, dtype=dtype, device=device)
+    if out.shape != (rows, w.features) or out.dtype != dtype or out.device != device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
+        raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
+    return out
+
+
+def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags):
+    rc = _lib.lib().skein_int4_rows(
+        x.data_ptr(), x.stride(0), _lib.ptr(src_row), w.codes.data_ptr(), w.scale.data_ptr(), _lib.ptr(w.zero), _lib.ptr(residual), out.data_ptr(),
+        out.stride(0), _lib.ptr(counts), _lib.ptr(offsets), rows, x.shape[0], w.codes.shape[0], w.features, w.shape[-1], w.group, hint, flags,
+        F.workspace(x.device).status.data_ptr(), _lib.stream_ptr())
+    _lib.check(rc, what)
+    _lib.count_launch()
+
+
+def linear(x, w: Int4Weight, out=None, residual=None, out_f32=False):
+    """y[t, f] = sum_k x[t, k] W[f, k] (+ residual[t, f]) for bf16 x [T, K] (rows may be strided). out_f32: y and the residual are fp32, else both are
+    bf16. out may be the residual, or a run of columns of a wider matrix."""
+    _check("int4 linear", x, w, False, 2)
+    return _dense("int4 linear", x, w, out, residual, out_f32)
+
+
+def swiglu_linear(x, w: Int4Weight, out=None):
+    """silu(x Wg^T) * (x Wu^T) with both products from one pass over x; w is packed as a pair."""
+    _check("int4 swiglu_linear", x, w, True, 2)
+    return _dense("int4 swiglu_linear", x, w, out, None, False)
+
+
+def _dense(what, x, w, out, residual, out_f32):
+    T = x.shape[0]
+    out = _out(what, out, T, w, torch.float32 if out_f32 else torch.bfloat16, x.device)
+    if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
+                                 or residual.stride() != out.stride()):
+        raise ValueError(f"{what}: the residual must have the result's shape, type and strides")
+    if T == 0:
+        return out
+    if not x.is_cuda:
+        return out.copy_(ri.product(x, w.dequant(), residual, out_f32, w.pair))
+    with _lib.on_device(x):
+        _launch(what, x, w, out, residual, None, None, None, T, T, w.flags | (4 if out_f32 else 0))
+    return out
+
+
+def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None, out=None, rows_hint=None):
+    """Per-expert linear over expert-sorted rows. counts / offsets are int32 device tensors of E (offsets may have E + 1) entries: rows of expert e are
+    offsets[e] : offsets[e] + counts[e] of the result. They read the same rows of x, or with src_row (int32, one entry per row of the result) rows
+    src_row[r]: the tokens themselves, without a sorted copy. Rows not covered by any expert are left untouched (uninitialised in a result that the call
+    makes). rows_hint: rows expected over all experts, of which the choice of kernel depends (default: all of the result's)."""
+    what = "int4 grouped_linear"
+    _check(what, x, w, bool(swiglu), 3)
+    E = w.shape[0]
+    for t, name, least in ((counts, "counts", E), (offsets, "offsets", E)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < least or not t.is_contiguous() or t.device != x.device:
+            raise ValueError(f"{what}: {name} must be int32 [{E}] on x's device")
+    if src_row is not None and (src_row.dtype != torch.int32 or src_row.dim() != 1 or not src_row.is_contiguous() or src_row.device != x.device):
+        raise ValueError(f"{what}: src_row must be int32 [rows] on x's device")
+    rows = x.shape[0] if src_row is None else src_row.shape[0]
+    out = _out(what, out, rows, w, torch.bfloat16, x.device)
+    if rows == 0:
+        return out
+    if not x.is_cuda:
+        return ri.grouped_product(x, w.dequant(), counts[:E], offsets[:E], swiglu, src_row, out)
+    hint = -(-(rows if rows_hint is None else max(1, min(int(rows_hint), rows))) // E)
+    with _lib.on_device(x):
+        _launch(what, x, w, out, None, counts, offsets, src_row, rows, hint, w.flags)
+    return out

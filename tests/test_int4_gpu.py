@@ -1,0 +1,300 @@
+"""4-bit products and the balanced choice of experts on the GPU, against 64 bits."""
+import pytest
+import torch
+
+from skein_b200 import ops
+from skein_b200.ops import experts, int4, reference_int4 as ri
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def weight(lead, rows, K, group, zeros, scales, pair, seed=0):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    codes = torch.randint(0, 256, (*lead, rows, K // 2), generator=gen, device=DEV, dtype=torch.uint8)
+    scale = (torch.rand(*lead, rows, K // group, generator=gen, device=DEV) * 0.02 + 0.005).to(scales)
+    zero = torch.randint(0, 16, (*lead, rows, K // group), generator=gen, device=DEV, dtype=torch.uint8) if zeros else None
+    return int4.pack_weight(codes, scale, zero, pair=pair), ri.dequant(codes, scale, zero, group).double()
+
+
+def acts(rows, K, seed=1):
+    return torch.randn(rows, K, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV).bfloat16()
+
+
+def within(y, x, w, pair=False, residual=None, half_step=2.0 ** -8):
+    """|y - exact| against the bound of the arithmetic: K sums in 32 bits, each off by at most a step (2^-23, the tensor cores cut off) of the sum of
+    magnitudes, and one rounding of the result. A pair adds what its two sums' errors do through silu (slope at most 1.1) and the error of a
+    fast exponential (2^-20)."""
+    x = x.double()
+    K = x.shape[1]
+    exact, size = x @ w.t(), x.abs() @ w.abs().t()
+    d = K * 2.0 ** -23 * size
+    if pair:
+        g, u = exact.chunk(2, 1)
+        dg, du = d.chunk(2, 1)
+        s = g * torch.sigmoid(g)
+        exact = s * u
+        d = 1.1 * dg * (u.abs() + du) + s.abs() * du + 2.0 ** -20 * exact.abs()
+    if residual is not None:
+        exact = exact + residual.double()
+        d = d + 2.0 ** -24 * exact.abs()
+    off = (y.double() - exact).abs() - d - half_step * (exact.abs() + d)
+    assert bool((off <= 0).all()), (float(off.max()), int((off > 0).sum()))
+
+
+SIZES = [  # rows, features, K, group, zeros, scales
+    (1, 16, 128, 128, False, torch.bfloat16), (1, 1, 32, 32, True, torch.float16), (3, 17, 96, 32, True, torch.bfloat16), (8, 130, 384, 64, True, torch.float16),
+    (9, 200, 1408, 128, False, torch.bfloat16), (16, 64, 4096, 128, True, torch.float16), (17, 48, 256, 32, False, torch.bfloat16), (33, 1000, 512, 64, False, torch.bfloat16),
+    (64, 256, 3584, 128, True, torch.bfloat16), (100, 129, 640, 128, False, torch.float16), (257, 384, 1056, 32, True, torch.float16), (130, 513, 2048, 64, True, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("rows, features, K, group, zeros, scales", SIZES)
+def test_linear(rows, features, K, group, zeros, scales):
+    w, full = weight((), features, K, group, zeros, scales, False)
+    assert torch.equal(w.dequant().double(), full)
+    x = acts(rows, K)
+    within(int4.linear(x, w), x, full)
+    within(int4.linear(x, w, out_f32=True), x, full, half_step=2.0 ** -24)
+    r = torch.randn(rows, features, device=DEV)
+    within(int4.linear(x, w, residual=r, out_f32=True), x, full, residual=r, half_step=2.0 ** -24)
+    rb = r.bfloat16()
+    keep = rb.clone()
+    assert int4.linear(x, w, residual=rb, out=rb) is rb
+    within(rb, x, full, residual=keep)
+
+
+@pytest.mark.parametrize("rows, features, K, group, zeros, scales", SIZES)
+def test_swiglu_linear(rows, features, K, group, zeros, scales):
+    w, full = weight((), 2 * features, K, group, zeros, scales, True)
+    x = acts(rows, K)
+    within(int4.swiglu_linear(x, w), x, full, pair=True)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 40, 150])
+def test_strides_and_alignment(rows):
+    w, full = weight((), 96, 256, 64, True, torch.bfloat16, False)
+    wide = acts(rows, 600)
+    for first in (0, 8, 1, 3):             # on and off 16-byte boundaries
+        x = wide[:, first:first + 256]
+        out = torch.full((rows, 200), 5.0, device=DEV, dtype=torch.bfloat16)
+        int4.linear(x, w, out=out[:, 50:146])
+        within(out[:, 50:146], x, full)
+        assert bool((out[:, :50] == 5).all()) and bool((out[:, 146:] == 5).all())
+    odd = acts(rows, 257)[:, :256]         # rows of 514 bytes
+    within(int4.linear(odd, w), odd, full)
+    within(int4.linear(wide[:1, :256].expand(rows, 256), w), wide[:1, :256].expand(rows, 256), full)
+
+
+@pytest.mark.parametrize("rows", [4, 40])
+def test_a_row_that_is_no_number_stays_alone(rows):
+    w, full = weight((), 64, 256, 128, False, torch.bfloat16, False)
+    x = acts(rows, 256)
+    x[1, 5], x[2, 255] = float("nan"), float("inf")
+    y = int4.linear(x, w)
+    assert bool(y[1].isnan().all()) and not bool(y[2].isfinite().any())
+    others = [r for r in range(rows) if r not in (1, 2)]
+    within(y[others], x[others], full)
+
+
+EXPERTS = [  # counts, features, K, group, zeros, scales, pair
+    ([1], 32, 128, 128, False, torch.bfloat16, False), ([0, 1, 0, 1], 64, 256, 64, True, torch.float16, True), ([3, 0, 9, 20, 1, 0], 40, 384, 128, False, torch.bfloat16, False),
+    ([0, 0, 50, 0], 24, 160, 32, True, torch.bfloat16, True), ([130, 1, 0, 77], 136, 512, 128, True, torch.float16, False), ([200, 3, 260], 72, 256, 64, False, torch.bfloat16, True),
+    ([1, 0, 2] * 30, 48, 128, 64, False, torch.float16, False), ([0, 0], 16, 128, 128, False, torch.bfloat16, True)]
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("hint", [None, 1, 10 ** 6])
+@pytest.mark.parametrize("counts, features, K, group, zeros, scales, pair", EXPERTS)
+def test_grouped_linear(counts, features, K, group, zeros, scales, pair, hint, gather):
+    E, spare = len(counts), 3
+    w, full = weight((E,), features * (2 if pair else 1), K, group, zeros, scales, pair)
+    n = sum(counts)
+    cnt = torch.tensor(counts, dtype=torch.int32, device=DEV)
+    off = torch.cat((cnt.new_zeros(1), cnt.cumsum(0))).to(torch.int32)
+    tokens = max(1, n // 2)
+    x = acts(tokens if gather else n + spare, K)
+    src = torch.randint(0, tokens, (n + spare,), device=DEV, dtype=torch.int32) if gather else None
+    out = torch.full((n + spare, features), 3.0, device=DEV, dtype=torch.bfloat16)
+    int4.grouped_linear(x, w, cnt, off, swiglu=pair, src_row=src, out=out, rows_hint=hint)
+    rows = x[src.long()] if gather else x
+    for e in range(E):
+        a, b = int(off[e]), int(off[e + 1])
+        if a < b:
+            within(out[a:b], rows[a:b], full[e], pair)
+    assert bool((out[n:] == 3).all())
+    ops.workspace().check_status()
+
+
+def test_rows_outside_are_reported():
+    w, _ = weight((2,), 32, 128, 128, False, torch.bfloat16, False)
+    x = acts(4, 128)
+    n = torch.tensor([2, 2], dtype=torch.int32, device=DEV)
+    off = torch.tensor([0, 2], dtype=torch.int32, device=DEV)
+    for counts, offsets, src in ((n, off, torch.tensor([0, 4, 1, 2], dtype=torch.int32, device=DEV)), (n, off, torch.tensor([0, -1, 1, 2], dtype=torch.int32, device=DEV)),
+                                 (n + 1, off, None), (n, off - 1, None)):
+        int4.grouped_linear(x, w, counts, offsets, src_row=src)
+        with pytest.raises(RuntimeError, match="out of range"):
+            ops.workspace().check_status()
+    int4.grouped_linear(x, w, n, off)
+    ops.workspace().check_status()
+
+
+@pytest.mark.parametrize("rows", [1, 12, 80])
+def test_captured_products_follow_their_inputs(rows):
+    w, full = weight((4,), 64, 256, 128, False, torch.bfloat16, True)
+    x, cnt, off = acts(rows, 256), torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(5, dtype=torch.int32, device=DEV)
+    cnt[0], off[1:] = rows, rows
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        int4.grouped_linear(x, w, cnt, off, swiglu=True)
+        with torch.cuda.graph(graph, stream=side):
+            y = int4.grouped_linear(x, w, cnt, off, swiglu=True)
+    torch.cuda.current_stream().wait_stream(side)
+    for e in (0, 3, 1):
+        x.copy_(acts(rows, 256, seed=e + 7))
+        cnt.zero_()
+        cnt[e] = rows
+        off.copy_(torch.cat((cnt.new_zeros(1), cnt.cumsum(0))))
+        graph.replay()
+        within(y, x, full[e], True)
+
+
+def test_same_bits_twice_and_on_two_streams():
+    w, full = weight((), 512, 2048, 128, True, torch.bfloat16, False)
+    for rows in (2, 14, 60, 300):
+        x = acts(rows, 2048)
+        y = int4.linear(x, w, out_f32=True)
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append([int4.linear(x, w, out_f32=True) for _ in range(3)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, z) for g in got for z in g)
+
+
+# ---- choice of experts ------------------------------------------------------------------------------------------------
+ROUTES = [  # tokens, experts, top, groups, keep, group_best, score, renorm
+    (1, 1, 1, 1, 1, 2, "softmax", True), (1, 128, 8, 1, 1, 2, "softmax", True), (5, 33, 4, 1, 1, 1, "sigmoid", False), (64, 64, 6, 8, 4, 2, "sigmoid", True),
+    (200, 120, 8, 8, 2, 1, "softmax", True), (256, 256, 8, 8, 4, 2, "sigmoid", True), (257, 40, 3, 5, 2, 2, "sigmoid", True), (300, 512, 16, 64, 8, 2, "softmax", False),
+    (31, 512, 16, 1, 1, 2, "sigmoid", True), (4096, 256, 8, 8, 4, 2, "sigmoid", True), (9000, 8, 2, 1, 1, 2, "softmax", True), (1000, 6, 2, 6, 3, 2, "sigmoid", True)]
+
+
+def plan_of(ids, E, e_first, e_count):
+    flat = ids.reshape(-1).long()
+    mine = (flat >= e_first) & (flat < e_first + e_count)
+    counts = torch.bincount(flat[mine], minlength=E).to(torch.int32)
+    offsets = torch.cat((counts.new_zeros(1), counts.cumsum(0))).to(torch.int32)
+    order = torch.where(mine, flat, torch.full_like(flat, E)).sort(stable=True).indices[:int(mine.sum())]
+    row_of = torch.full_like(flat, -1)
+    row_of[order] = torch.arange(order.numel(), device=flat.device)
+    return counts, offsets, row_of.to(torch.int32), (order // ids.shape[1]).to(torch.int32)
+
+
+def check_route(z, top, bias, groups, keep, best, score, renorm, scale=1.0, e_first=0, e_count=None):
+    E = z.shape[1]
+    got = experts.route_balanced(z, top, bias=bias, groups=groups, keep=keep, score=score, group_best=best, renorm=renorm, scale=scale, e_first=e_first,
+                                 e_count=e_count)
+    ids, w = ri.select_balanced(z, top, bias, groups, keep, score, best, renorm, scale)
+    assert torch.equal(got[0], ids)
+    # one rounding of a 64-bit value on either side
+    assert torch.allclose(got[1].double(), w.double(), rtol=2.0 ** -23, atol=1e-40)
+    want = plan_of(ids, E, e_first, E - e_first if e_count is None else e_count)
+    for a, b in zip(got[2:5], want[:3]):
+        assert torch.equal(a, b)
+    assert torch.equal(got[5][:want[3].numel()], want[3])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T, E, top, groups, keep, best, score, renorm", ROUTES)
+def test_route_balanced(T, E, top, groups, keep, best, score, renorm, dtype):
+    gen = torch.Generator(device=DEV).manual_seed(T + E)
+    z = torch.randn(T, E, generator=gen, device=DEV).to(dtype)
+    bias = torch.randn(E, generator=gen, device=DEV) * 0.1
+    for b in (None, bias):
+        check_route(z, top, b, groups, keep, best, score, renorm, 2.5)
+    if E > 2:
+        check_route(z, top, bias, groups, keep, best, score, renorm, 1.0, E // 3, E // 2)
+    wide = torch.randn(T, E + 5, generator=gen, device=DEV).to(dtype)
+    check_route(wide[:, 3:3 + E], top, bias, groups, keep, best, score, renorm)
+
+
+@pytest.mark.parametrize("T", [16, 600])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_of_masked_and_equal_logits(T, score):
+    z = torch.randn(T, 48, device=DEV)
+    z[0] = 0
+    z[1] = -float("inf")
+    z[2, 5:] = -float("inf")
+    z[3] = float("nan")
+    z[4, ::2] = float("nan")
+    z[5, 7] = float("inf")
+    z[6] = torch.finfo(torch.float32).min
+    z[7] = torch.finfo(torch.float32).max
+    z[8] = z[8].bfloat16().float().round()
+    z[9, 40] = -float("inf")
+    off = torch.zeros(48, device=DEV)
+    off[3], off[11] = -float("inf"), float("inf")
+    for bias in (None, off):
+        for groups, keep in ((1, 1), (6, 2), (48, 7)):
+            check_route(z, 7, bias, groups, keep, 2, score, True)
+
+
+def test_route_of_no_tokens():
+    got = experts.route_balanced(torch.empty(0, 12, device=DEV), 3)
+    assert got[0].shape == (0, 3) and bool((got[2] == 0).all()) and bool((got[3] == 0).all()) and got[4].numel() == 0
+
+
+@pytest.mark.parametrize("T", [40, 700])
+def test_captured_route_follows_its_logits(T):
+    z = torch.randn(T, 64, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        experts.route_balanced(z, 6, groups=8, keep=4)
+        with torch.cuda.graph(graph, stream=side):
+            got = experts.route_balanced(z, 6, groups=8, keep=4)
+    torch.cuda.current_stream().wait_stream(side)
+    for seed in range(3):
+        z.copy_(torch.randn(T, 64, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV))
+        graph.replay()
+        ids, _ = ri.select_balanced(z, 6, None, 8, 4, "sigmoid", 2, True, 1.0)
+        assert torch.equal(got[0], ids)
+        for a, b in zip(got[2:], plan_of(ids, 64, 0, 64)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [1, 50, 400])
+def test_layer_of_experts(T):
+    """Router, gate / up by the router's layout, down, combine with the residual: a layer as it is used."""
+    H, I, E, top = 256, 128, 12, 3
+    gen = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, H, generator=gen, device=DEV).bfloat16()
+    wg = torch.randn(E, H, generator=gen, device=DEV).bfloat16()
+    bias = torch.randn(E, generator=gen, device=DEV) * 0.1
+    up, up_full = weight((E,), 2 * I, H, 64, True, torch.bfloat16, True, seed=2)
+    down, down_full = weight((E,), H, I, 32, False, torch.float16, False, seed=3)
+    logits = ops.linear(x, wg, out_f32=True)
+    ids, w, counts, offsets, row_of, src = experts.route_balanced(logits, top, bias=bias, groups=4, keep=2, scale=2.0)
+    h = int4.grouped_linear(x, up, counts, offsets, swiglu=True, src_row=src)
+    y = int4.grouped_linear(h, down, counts, offsets)
+    out, _ = ops.reduce_residual_rmsnorm(x, y[None], None, 1e-5, row_idx=row_of.view(T, top), row_w=w)
+    ops.workspace().check_status()
+    ids_want, w_want = ri.select_balanced(logits, top, bias, 4, 2, "sigmoid", 2, True, 2.0)
+    assert torch.equal(ids, ids_want)
+    want, size = x.double(), torch.zeros(T, H, dtype=torch.float64, device=DEV)
+    for j in range(top):
+        for t in range(T):
+            e = int(ids[t, j])
+            g, u = (x[t].double() @ up_full[e].t()).chunk(2)
+            a = g * torch.sigmoid(g) * u
+            v = a @ down_full[e].t()
+            want[t] += w_want[t, j].double() * v
+            # h is rounded (2^-8 of each product of the sum), y and the result are
+            size[t] += w_want[t, j].double() * ((a.abs() @ down_full[e].abs().t()) * 2.0 ** -8 * 1.01 + v.abs() * 2.0 ** -8 * 1.01)
+    off = (out.double() - want).abs() - size - 2.0 ** -8 * (want.abs() + size) - 1e-4 * size
+    assert bool((off <= 0).all()), float(off.max())

@@ -5,13 +5,16 @@
 // A matrix is cut into strips of 16 rows and steps of 128 along K (skein_b200/ops/int4.py packs it; rows and K are padded). For a pair of
 // matrices (gate and up of a SwiGLU) a strip holds 8 gate rows and the 8 up rows of the same features, so that whoever holds accumulator
 // row r of a strip has its partner at r + 8.
-//   codes  [strip][step][2][lane 32][16 bytes]: a lane (g = lane / 4, t = lane % 4) of half j owns rows g and g + 8 at k = 64 j + 8 t .. + 7 and
+// A block (strip, step) is one record of memory, codes, then scales, then zeros where there are any, so that it arrives in one copy; the records of
+// a strip follow one another along K.
+//   codes  [2][t 4][g 8][16 bytes]: lane (g = lane / 4, t = lane % 4) of half j owns rows g and g + 8 at k = 64 j + 8 t .. + 7 and
 //          64 j + 32 + 8 t .. + 7: words {row g, first; row g, second; row g + 8, first; row g + 8, second}. One 16-byte load of a warp is 16 rows x
-//          64 k in the order in which mma.sync's A operand wants them (any order of k is right as long as B has the same), and the row's eight
-//          codes of a word are neighbours in k, so that the tensor-memory kernel takes its rows from the same bytes.
+//          64 k in the order in which mma.sync's A operand wants them (any order of k is right as long as B has the same). The row's eight
+//          codes of a word are neighbours in k, so that the tensor-memory kernel takes its rows from the same bytes, eight bytes at a time and
+//          without bank conflicts (that is why g runs fastest).
 //          Inside a word the codes of even k are the low half's nibbles, those of odd k the high half's: (word >> 4 i) & 0x000f000f is the
 //          pair (k = 2 i, 2 i + 1).
-//   scales [strip][step][8][128 / group][2] 16-bit: rows g and g + 8 side by side; zeros the same in bytes.
+//   scales [g 8][128 / group][2] 16-bit: rows g and g + 8 side by side; zeros the same in bytes.
 #pragma once
 #include "gemm_sched.cuh"
 #include "ptx.cuh"
@@ -21,7 +24,8 @@
 namespace skein {
 
 constexpr int I4_STEP = 128;                       // elements of K
-constexpr int I4_STEP_BYTES = 16 * I4_STEP / 2;    // of one strip
+constexpr int I4_CODES = 16 * I4_STEP / 2;         // bytes of a record's codes
+__host__ __device__ constexpr int i4_record(int gp, bool zero) { return I4_CODES + 32 * gp + (zero ? 16 * gp : 0); }     // gp: groups of a step
 
 // code pair -> bf16 pair 128 + code: the codes are the low mantissa bits of a bf16 whose unit in the last place is 1
 __device__ __forceinline__ uint32_t i4_magic(uint32_t word, int i) {

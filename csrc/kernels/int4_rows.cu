@@ -17,9 +17,7 @@ constexpr int IR_DEPTH = 4;      // steps whose codes are in flight
 struct Int4Rows {
   const __nv_bfloat16* x;
   const int* src_row;
-  const uint8_t* codes;
-  const uint16_t* scale;
-  const uint8_t* zero;
+  const uint8_t* w;
   const void* residual;
   void* out;
   const int *counts, *offsets;
@@ -48,16 +46,17 @@ struct Int4Step {       // a lane's part of a step of one strip
   uint4 c[2];
   uint32_t s[GP];       // scales of rows g and g + 8
   uint16_t z[GP];
-  __device__ __forceinline__ void load(const Int4Rows& p, size_t block, int lane) {
-    const uint8_t* at = p.codes + block * I4_STEP_BYTES + lane * 16;
+  __device__ __forceinline__ void load(const uint8_t* rec, int lane) {
+    const int g = lane >> 2;
+    const uint8_t* at = rec + ((lane & 3) * 8 + g) * 16;
     c[0] = __ldcs(reinterpret_cast<const uint4*>(at));
     c[1] = __ldcs(reinterpret_cast<const uint4*>(at + 512));
-    const uint32_t* sp = reinterpret_cast<const uint32_t*>(p.scale) + (block * 8 + (lane >> 2)) * GP;
+    const uint32_t* sp = reinterpret_cast<const uint32_t*>(rec + I4_CODES) + g * GP;
     if constexpr (GP == 1) s[0] = __ldg(sp);
     if constexpr (GP == 2) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp)); s[0] = v.x; s[1] = v.y; }
     if constexpr (GP == 4) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(sp)); s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w; }
     if constexpr (ZERO) {
-      const uint16_t* zp = reinterpret_cast<const uint16_t*>(p.zero) + (block * 8 + (lane >> 2)) * GP;
+      const uint16_t* zp = reinterpret_cast<const uint16_t*>(rec + I4_CODES + 32 * GP) + g * GP;
       if constexpr (GP == 1) z[0] = __ldg(zp);
       if constexpr (GP == 2) { const ushort2 v = __ldg(reinterpret_cast<const ushort2*>(zp)); z[0] = v.x; z[1] = v.y; }
       if constexpr (GP == 4) { const ushort4 v = __ldg(reinterpret_cast<const ushort4*>(zp)); z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w; }
@@ -84,7 +83,8 @@ __global__ void __launch_bounds__(IR_THREADS) int4_rows_kernel(const Int4Rows p)
     }
   }
   const bool live = strip < p.strips;
-  const size_t block0 = ((size_t)e * p.strips + (live ? strip : 0)) * p.steps;
+  constexpr int REC = i4_record(GP, ZERO);
+  const uint8_t* strip_w = p.w + ((size_t)e * p.strips + (live ? strip : 0)) * p.steps * REC;
   for (int tile = blockIdx.z; tile * 8 * NT < count; tile += gridDim.z) {
     const __nv_bfloat16* row[NT];
 #pragma unroll
@@ -105,14 +105,14 @@ __global__ void __launch_bounds__(IR_THREADS) int4_rows_kernel(const Int4Rows p)
     Int4Step<GP, ZERO> buf[IR_DEPTH];
 #pragma unroll
     for (int d = 0; d < IR_DEPTH; ++d)
-      if (live && part + d * WK < p.steps) buf[d].load(p, block0 + part + d * WK, lane);
+      if (live && part + d * WK < p.steps) buf[d].load(strip_w + (size_t)(part + d * WK) * REC, lane);
     for (int s0 = part; s0 < p.steps; s0 += IR_DEPTH * WK) {
 #pragma unroll
       for (int d = 0; d < IR_DEPTH; ++d) {
         const int step = s0 + d * WK;
         if (step >= p.steps || !live) break;
         const Int4Step<GP, ZERO> cur = buf[d];
-        if (step + IR_DEPTH * WK < p.steps) buf[d].load(p, block0 + step + IR_DEPTH * WK, lane);
+        if (step + IR_DEPTH * WK < p.steps) buf[d].load(strip_w + (size_t)(step + IR_DEPTH * WK) * REC, lane);
         float part_sum[NT][4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {             // 32 of K each
@@ -184,26 +184,24 @@ static int pick_pair(const Int4Rows& p, bool pair, int E, int tiles, cudaStream_
   return pair ? launch_rows<NT, GP, ZERO, true, 8>(p, E, tiles, s) : launch_rows<NT, GP, ZERO, false, 8>(p, E, tiles, s);
 }
 template <int NT>
-static int pick_group(const Int4Rows& p, int group, bool pair, int E, int tiles, cudaStream_t s) {
-  if (group == 128) return p.zero ? pick_pair<NT, 1, true>(p, pair, E, tiles, s) : pick_pair<NT, 1, false>(p, pair, E, tiles, s);
-  if (group == 64) return p.zero ? pick_pair<NT, 2, true>(p, pair, E, tiles, s) : pick_pair<NT, 2, false>(p, pair, E, tiles, s);
-  return p.zero ? pick_pair<NT, 4, true>(p, pair, E, tiles, s) : pick_pair<NT, 4, false>(p, pair, E, tiles, s);
+static int pick_group(const Int4Rows& p, int group, bool zero, bool pair, int E, int tiles, cudaStream_t s) {
+  if (group == 128) return zero ? pick_pair<NT, 1, true>(p, pair, E, tiles, s) : pick_pair<NT, 1, false>(p, pair, E, tiles, s);
+  if (group == 64) return zero ? pick_pair<NT, 2, true>(p, pair, E, tiles, s) : pick_pair<NT, 2, false>(p, pair, E, tiles, s);
+  return zero ? pick_pair<NT, 4, true>(p, pair, E, tiles, s) : pick_pair<NT, 4, false>(p, pair, E, tiles, s);
 }
 
 }  // namespace skein
 
-// x [x_rows, x_ld] bf16 (row r of the product reads row src_row[r], or r); codes, scale, zero as in int4.cuh; out and residual [rows, out_ld] bf16
+// x [x_rows, x_ld] bf16 (row r of the product reads row src_row[r], or r); w as in int4.cuh; out and residual [rows, out_ld] bf16
 // or fp32. counts / offsets null: one matrix for all rows. tiles: tiles of rows that an expert's CTAs are dealt over (each walks its share).
-// flags: 1 pair, 2 fp16 scales, 4 fp32 output.
-extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* codes, const void* scale, const void* zero,
-                               const void* residual, void* out, long long out_ld, const int* counts, const int* offsets, int rows, int x_rows,
+// flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
+extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld, const int* counts, const int* offsets, int rows, int x_rows,
                                int E, int F, int K, int group, int rows_hint, int flags, int* status, void* stream) {
   using namespace skein;
   if (rows == 0) return 0;
   if (rows < 0 || E < 1 || E > 65535 || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
   Int4Rows p;
-  p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.codes = (const uint8_t*)codes; p.scale = (const uint16_t*)scale;
-  p.zero = (const uint8_t*)zero; p.residual = residual; p.out = out; p.counts = counts; p.offsets = offsets; p.status = status;
+  p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts; p.offsets = offsets; p.status = status;
   p.x_ld = x_ld; p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.F = F; p.K = K;
   const bool pair = flags & 1;
   p.strips = pair ? (F + 7) / 8 : (F + 15) / 16;
@@ -215,5 +213,5 @@ extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row
   int tiles = (per + 8 * nt - 1) / (8 * nt);
   if (tiles > 65535) tiles = 65535;
   cudaStream_t s = (cudaStream_t)stream;
-  return nt == 1 ? pick_group<1>(p, group, pair, E, tiles, s) : pick_group<2>(p, group, pair, E, tiles, s);
+  return nt == 1 ? pick_group<1>(p, group, flags & 8, pair, E, tiles, s) : pick_group<2>(p, group, flags & 8, pair, E, tiles, s);
 }

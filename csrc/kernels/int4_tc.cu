@@ -1,0 +1,463 @@
+// Products with 4-bit weights (int4.cuh) on tcgen05: y[r, f] = sum over groups j of scale[f, j] * ( sum_{k in j} x[r, k] (code[f, k] - zero[f, j]) ).
+//
+// Weights are the M side (128 rows of a tile), NT rows of x the N side. A CTA owns a tile, or with few tiles a piece of its K (the CTAs of a cluster
+// share the tile). Roles, one pipeline:
+//   producer    one bulk copy per strip (codes, scales and zeros of 16 rows x 128 of K are one record) and TMA tiles of x, or of the rows that
+//               src_row names (tile::gather4), into a ring of shared-memory stages
+//   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (whole numbers, exact), 64 of K a slot, written to tensor
+//               memory as the A operand
+//   MMA         one thread; every group of K has an accumulator of its own (a ring of them)
+//   epilogue    takes a group's accumulator out of tensor memory, multiplies it by the row's scale and adds it to its registers, fp32
+// So no rounding happens before the result, whatever the scales are. (Scaled weights rounded to bf16 would need neither the ring nor the second sum,
+// but double the error of a product, and more for a gate / up pair.)
+// What bounds it: with few rows the conversion keeps pace with HBM (about 1.6 instructions per weight and lane, half of the SM's issue slots at 6.5 TB/s);
+// with 128 rows and groups of 128 a step is 512 cycles of MMA against 420 x 2 issue slots of conversion and 4 x 100 of the epilogue.
+// Pieces of a tile meet in distributed shared memory in rank order: the result does not depend on timing, and no memory outlives the call.
+#include "int4.cuh"
+#include "launch.cuh"
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+namespace skein {
+
+int make_tmap_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t k_elems, uint64_t ld, int elem_bytes, uint32_t box_rows);   // gemm_ws.cu
+
+constexpr int IT_MAX_STAGES = 8;
+constexpr int IT_BAND = 12;              // feature tiles of a band in which the row tiles run (L2 keeps a band's weights)
+
+struct Int4Tc {
+  const int* src_row;
+  const uint8_t* w;
+  const void* residual;
+  void* out;
+  const int *counts, *offsets;
+  int* status;
+  long long out_ld;
+  int rows, x_rows, E, F, K, strips, steps, m_tiles, split, stages, flags;   // flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros
+  uint64_t budget_ns;
+};
+
+__device__ __forceinline__ void it_gather4(uint32_t dst, const void* tmap, uint32_t bar, int x, int r0, int r1, int r2, int r3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+
+// The same answer for every lane, so that a warp leaves a role together.
+__device__ __forceinline__ bool it_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, budget_ns));
+}
+
+// shape of a launch
+template <int NT>
+struct ItShape {
+  static constexpr bool WIDE = NT == 128;                  // one CTA per SM, 512 columns; else two with 256 each
+  static constexpr int CONV_WARPS = WIDE ? 8 : 4, EPI_WARPS = WIDE ? 8 : 4;
+  static constexpr int THREADS = 32 * (4 + CONV_WARPS + EPI_WARPS);       // warps 0 and 1 produce and issue, 2 and 3 only align the quadrants
+  static constexpr int ACC = NT < 32 ? 32 : NT;            // columns of an accumulator
+  static constexpr int BUFS = NT <= 32 ? 4 : 2;
+  static constexpr int SLOTS = WIDE ? 8 : 4;               // 32 columns each
+  static constexpr int COLS = WIDE ? 512 : 256;
+  static constexpr int EPI_COLS = NT / (EPI_WARPS / 4);    // columns of an epilogue warp
+  static_assert(BUFS * ACC + SLOTS * 32 <= COLS, "tensor memory");
+};
+
+template <int NT, int GP>
+__global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Int4Tc p) {
+  namespace cg = cooperative_groups;
+  using S = ItShape<NT>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[IT_MAX_STAGES], bar_empty[IT_MAX_STAGES], bar_cfull[S::SLOTS], bar_cempty[S::SLOTS], bar_dfull[S::BUFS], bar_dempty[S::BUFS];
+  __shared__ uint32_t tmem_base_smem;
+  __shared__ int abort_flag, unit[5];     // expert (-1: no such unit), feature tile, first row of the result, rows, first row in the expert
+  __shared__ int src[NT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const bool zeros = p.flags & 8;
+  const int rec = i4_record(GP, zeros);
+  constexpr int X_BYTES = NT * 256;
+  const int stage_bytes = X_BYTES + ((8 * rec + 1023) & ~1023);
+
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < p.stages; ++s) { mbar_init(smem_u32(&bar_full[s]), 1); mbar_init(smem_u32(&bar_empty[s]), 1 + S::EPI_WARPS); }
+    for (int s = 0; s < S::SLOTS; ++s) { mbar_init(smem_u32(&bar_cfull[s]), 4); mbar_init(smem_u32(&bar_cempty[s]), 1); }
+    for (int b = 0; b < S::BUFS; ++b) { mbar_init(smem_u32(&bar_dfull[b]), 1); mbar_init(smem_u32(&bar_dempty[b]), S::EPI_WARPS); }
+    fence_mbar_init();
+  }
+  if (warp == 1) { tmem_alloc(smem_u32(&tmem_base_smem), S::COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_smem;
+  pdl_trigger();
+  pdl_wait();
+
+  // ---- which tile: experts in order, in each bands of feature tiles, in a band the feature tile runs fastest
+  const int rank = (int)blockIdx.x % p.split;
+  if (warp == 0) {
+    const int u = (int)blockIdx.x / p.split;
+    int found = -1, before = 0, count = p.rows, first = 0;
+    if (p.counts == nullptr) found = u < p.m_tiles * ((p.rows + NT - 1) / NT) ? 0 : -1;
+    else {
+      for (int e0 = 0; e0 < p.E && found < 0; e0 += 32) {
+        int c = 0, o = 0;
+        if (e0 + lane < p.E) {
+          c = p.counts[e0 + lane];
+          o = p.offsets[e0 + lane];
+          if (o < 0 || c < 0 || c > p.rows - o) {
+            if (c != 0) report_status(p.status, ST_BAD_INDEX, e0 + lane);
+            c = 0;
+          }
+        }
+        const int mine = p.m_tiles * ((c + NT - 1) / NT);
+        int inc = mine;
+        for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += v; }
+        const unsigned hit = __ballot_sync(0xffffffffu, u < before + inc);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          found = e0 + l;
+          before = __shfl_sync(0xffffffffu, before + inc - mine, l);
+          count = __shfl_sync(0xffffffffu, c, l);
+          first = __shfl_sync(0xffffffffu, o, l);
+        } else before += __shfl_sync(0xffffffffu, inc, 31);
+      }
+    }
+    if (found >= 0) {
+      const int r = u - before, nt = (count + NT - 1) / NT;
+      const int band = r / (IT_BAND * nt), rb = r - band * IT_BAND * nt, bm = min(IT_BAND, p.m_tiles - band * IT_BAND), n = rb / bm;
+      for (int i = lane; i < NT; i += 32) {
+        const int at = n * NT + i;
+        int row = 0;
+        if (p.src_row != nullptr && at < count) {
+          row = p.src_row[first + at];
+          if (row < 0 || row >= p.x_rows) { report_status(p.status, ST_BAD_INDEX, row); row = 0; }
+        }
+        src[i] = row;
+      }
+      if (lane == 0) { unit[1] = band * IT_BAND + rb - n * bm; unit[2] = first + n * NT; unit[3] = min(NT, count - n * NT); }
+    }
+    if (lane == 0) unit[0] = found;
+  }
+  __syncthreads();
+  const int e = unit[0];
+  const bool live = e >= 0;            // the same for every CTA of a cluster
+  const int m = unit[1], row0 = unit[2], valid = unit[3];
+  const int s0 = (int)((long long)p.steps * rank / p.split), s1 = (int)((long long)p.steps * (rank + 1) / p.split);
+  float acc[S::EPI_COLS];
+
+  if (live) {
+    const uint8_t* w = p.w + ((size_t)e * p.strips + (size_t)m * 8) * p.steps * rec;
+    const int my_strips = min(8, p.strips - m * 8);
+    if (warp == 0) {
+      // ================= producer =================
+      if (elect_one()) {
+        tma_prefetch_desc(&tmX);
+        const uint64_t keep = l2_policy_evict_last();
+        int st = 0;
+        uint32_t ph = 0;
+        for (int s = s0; s < s1; ++s) {
+          if (!mbar_wait(smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
+            report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x);
+            abort_flag = 1;
+            break;
+          }
+          const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
+          mbar_expect_tx(full, X_BYTES + my_strips * rec);
+          for (int i = 0; i < my_strips; ++i) bulk_load_1d(at + X_BYTES + i * rec, w + ((size_t)i * p.steps + s) * rec, rec, full);
+          if (p.src_row == nullptr) {
+            tma_load_2d(at, &tmX, full, s * I4_STEP, row0, keep);
+            tma_load_2d(at + NT * 128, &tmX, full, s * I4_STEP + 64, row0, keep);
+          } else {
+            // a half that lies behind K as a whole has scales of zero: any columns do
+            const int x1 = s * I4_STEP + 64 < p.K ? s * I4_STEP + 64 : 0;
+            for (int i = 0; i < NT; i += 4) {
+              it_gather4(at + i * 128, &tmX, full, s * I4_STEP, src[i], src[i + 1], src[i + 2], src[i + 3]);
+              it_gather4(at + NT * 128 + i * 128, &tmX, full, x1, src[i], src[i + 1], src[i + 2], src[i + 3]);
+            }
+          }
+          if (++st == p.stages) { st = 0; ph ^= 1; }
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // ================= MMA =================
+      if (elect_one()) {
+        const uint32_t idesc = umma_idesc(1, 1, 128, NT);
+        int st = 0, slot = 0, buf = 0;
+        uint32_t ph = 0, sph = 0, bph = 0;
+        bool ok = true;
+        for (int s = s0; s < s1 && ok; ++s) {
+          if (!mbar_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; break; }
+          const uint32_t at = smem_base + st * stage_bytes;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (!ok) break;
+            if (!mbar_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); ok = false; break; }
+            const uint64_t dx = umma_desc_sw128(at + j * NT * 128);
+            const uint32_t a_tmem = tmem_base + S::BUFS * S::ACC + slot * 32;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              constexpr int PER = 8 / GP;              // MMAs of a group
+              const int in = (j * 4 + k) % PER;
+              if (in == 0 && !mbar_wait(smem_u32(&bar_dempty[buf]), bph ^ 1, &abort_flag, p.budget_ns)) {
+                report_status(p.status, ST_TIMEOUT_TMEM_EMPTY, blockIdx.x);
+                ok = false;
+                break;
+              }
+              if (in == 0 || k == 0) tc_fence_after();
+              mma_f16_ts(tmem_base + buf * S::ACC, a_tmem + 8 * k, dx + 2 * k, idesc, in > 0 ? 1u : 0u);
+              if (in == PER - 1) {
+                tc_commit(smem_u32(&bar_dfull[buf]));
+                if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
+              }
+            }
+            if (!ok) break;
+            tc_commit(smem_u32(&bar_cempty[slot]));
+            if (++slot == S::SLOTS) { slot = 0; sph ^= 1; }
+          }
+          if (!ok) { abort_flag = 1; break; }
+          tc_commit(smem_u32(&bar_empty[st]));
+          if (++st == p.stages) { st = 0; ph ^= 1; }
+        }
+      }
+      __syncwarp();
+    } else if (warp >= 4 && warp < 4 + S::CONV_WARPS) {
+      // ================= converters: row r of the tile, half j of a step (both in turn with four warps) =================
+      const int r = (warp & 3) * 32 + lane, group = (warp - 4) >> 2;
+      constexpr int GROUPS = S::CONV_WARPS / 4;
+      const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
+      const int in_stage = X_BYTES + (r >> 4) * rec + (r & 7) * 16 + ((r >> 3) & 1) * 8;
+      const int zero_at = X_BYTES + (r >> 4) * rec + I4_CODES + 32 * GP + (r & 7) * GP * 2 + ((r >> 3) & 1);
+      int st = 0, slot = group;
+      uint32_t ph = 0, sph = 0;
+      bool ok = true;
+      for (int s = s0; s < s1 && ok; ++s) {
+        if (!it_warp_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
+          if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
+          break;
+        }
+        const uint8_t* at = smem_raw + (smem_base - smem_u32(smem_raw)) + st * stage_bytes;
+#pragma unroll
+        for (int j0 = 0; j0 < 2; j0 += GROUPS) {
+          const int j = j0 + group;
+          uint2 c[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) c[t] = *reinterpret_cast<const uint2*>(at + in_stage + j * 512 + t * 128);
+          uint32_t base[2] = {i4_base(8), i4_base(8)};
+          if (zeros) {
+            base[0] = i4_base(at[zero_at + (GP == 1 ? 0 : GP == 2 ? j : 2 * j) * 2]);
+            base[1] = GP == 4 ? i4_base(at[zero_at + (2 * j + 1) * 2]) : base[0];
+          }
+          uint32_t v[32];
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              v[t * 4 + i] = i4_sub(i4_magic(c[t].x, i), base[0]);
+              v[16 + t * 4 + i] = i4_sub(i4_magic(c[t].y, i), base[1]);
+            }
+          if (!it_warp_wait(smem_u32(&bar_cempty[slot]), sph ^ 1, &abort_flag, p.budget_ns)) {
+            if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t to = tmem_base + S::BUFS * S::ACC + slot * 32 + lane_tmem;
+          tmem_st16(to, v);
+          tmem_st16(to + 16, v + 16);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_cfull[slot]));
+          slot += GROUPS;
+          if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
+        }
+        if (++st == p.stages) { st = 0; ph ^= 1; }
+      }
+    } else if (warp >= 4) {
+      // ================= epilogue: row r, columns col0 .. + EPI_COLS =================
+      const int r = (warp & 3) * 32 + lane, col0 = ((warp - 4 - S::CONV_WARPS) >> 2) * S::EPI_COLS;
+      const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
+      const int scale_at = X_BYTES + (r >> 4) * rec + I4_CODES + (r & 7) * GP * 4 + ((r >> 3) & 1) * 2;
+#pragma unroll
+      for (int c = 0; c < S::EPI_COLS; ++c) acc[c] = 0.f;
+      int st = 0, buf = 0;
+      uint32_t ph = 0, bph = 0;
+      bool ok = true;
+      for (int s = s0; s < s1 && ok; ++s) {
+        if (!it_warp_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
+          if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
+          break;
+        }
+        const uint8_t* at = smem_raw + (smem_base - smem_u32(smem_raw)) + st * stage_bytes;
+        float sc[GP];
+#pragma unroll
+        for (int g = 0; g < GP; ++g) sc[g] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_empty[st]));
+        if (++st == p.stages) { st = 0; ph ^= 1; }
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          if (!it_warp_wait(smem_u32(&bar_dfull[buf]), bph, &abort_flag, p.budget_ns)) {
+            if (lane == 0) { report_status(p.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x); abort_flag = 1; }
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem;
+#pragma unroll
+          for (int c0 = 0; c0 < S::EPI_COLS; c0 += 16) {
+            uint32_t v[16];
+            tmem_ld16(from + c0, v);
+            tmem_ld_wait();
+            if (c0 + 16 == S::EPI_COLS) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&bar_dempty[buf]));
+            }
+#pragma unroll
+            for (int c = 0; c < 16; ++c) acc[c0 + c] += sc[g] * __uint_as_float(v[c]);
+          }
+          if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
+        }
+      }
+    }
+  }
+
+  // ---- the pieces of a tile: every CTA finishes NT / split columns, summed in rank order
+  const bool epi = warp >= 4 + S::CONV_WARPS;
+  const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS;
+  const int slice = NT / p.split;
+  float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));      // [rank][slice][128], on stages that nothing reads any more
+  if (p.split > 1 && live) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (epi) {
+#pragma unroll
+      for (int c = 0; c < S::EPI_COLS; ++c) {
+        const int owner = (col0 + c) / slice;
+        cluster.map_shared_rank(recv, owner)[(rank * slice + (col0 + c) % slice) * 128 + r] = acc[c];
+      }
+    }
+    cluster.sync();
+  }
+  if (live && epi && abort_flag == 0) {
+    const bool pair = p.flags & 1, f32 = p.flags & 4;
+    const int f = pair ? (m * 8 + (r >> 4)) * 8 + (r & 7) : m * 128 + r;
+    auto store = [&](int col, float y) {
+      const size_t at = (size_t)(row0 + col) * p.out_ld + f;
+      if (f32) ((float*)p.out)[at] = p.residual ? y + ((const float*)p.residual)[at] : y;
+      else ((__nv_bfloat16*)p.out)[at] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[at]) : y);
+    };
+    // two columns; of a pair the gate's lane finishes the first and the up's the second
+    auto finish = [&](int col, float a, float b) {
+      if (!pair) {
+        if (f < p.F && col < valid) store(col, a);
+        if (f < p.F && col + 1 < valid) store(col + 1, b);
+      } else {
+        const bool up = r & 8;
+        const float other = __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
+        const int c = up ? col + 1 : col;
+        const float y = up ? silu(other) * b : silu(a) * other;
+        if (f < p.F && c < valid) store(c, y);
+      }
+    };
+    if (p.split == 1) {
+#pragma unroll
+      for (int c = 0; c < S::EPI_COLS; c += 2) if (col0 + c < valid) finish(col0 + c, acc[c], acc[c + 1]);
+    } else {
+      for (int c = part * 2; c < slice; c += 2 * (S::EPI_WARPS / 4)) {
+        if (rank * slice + c >= valid) break;
+        float a = 0.f, b = 0.f;
+        for (int q = 0; q < p.split; ++q) {
+          a += recv[(q * slice + c) * 128 + r];
+          b += recv[(q * slice + c + 1) * 128 + r];
+        }
+        finish(rank * slice + c, a, b);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag) {       // copies may still be on their way into this CTA's shared memory
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000) __nanosleep(1000);
+  }
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, S::COLS); }
+}
+
+template <int NT, int GP>
+static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s) {
+  using S = ItShape<NT>;
+  static PerDevice allowed;
+  const int room = (S::WIDE ? 225 : 111) * 1024;
+  const int stage = NT * 256 + ((8 * i4_record(GP, p.flags & 8) + 1023) & ~1023);
+  p.stages = (room - 1024) / stage;
+  if (p.stages > IT_MAX_STAGES) p.stages = IT_MAX_STAGES;
+  const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP>, room);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)tiles * p.split);
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = (size_t)p.stages * stage + 1024;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, int4_tc_kernel<NT, GP>, tmX, p);
+}
+template <int NT>
+static int launch_tc_group(const CUtensorMap& tmX, const Int4Tc& p, int group, int tiles, cudaStream_t s) {
+  return group == 128 ? launch_tc<NT, 1>(tmX, p, tiles, s) : group == 64 ? launch_tc<NT, 2>(tmX, p, tiles, s) : launch_tc<NT, 4>(tmX, p, tiles, s);
+}
+
+}  // namespace skein
+
+// Arguments as skein_int4_rows (int4_rows.cu); x and its rows on 16-byte boundaries. n_tile (16, 32, 64 or 128) rows of a tile, split CTAs that share
+// the K of one (1, 2, 4 or 8); 0: by the rules here from rows_hint, the rows expected of an expert. Returns -1 for what it does not take.
+extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld,
+                             const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int rows_hint, int flags, int n_tile,
+                             int split, int* status, void* stream) {
+  using namespace skein;
+  if (rows == 0) return 0;
+  if (rows < 0 || x_rows < 1 || E < 1 || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
+  if (x_ld % 8 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0) return -1;
+  if (n_tile == 0) n_tile = rows_hint <= 16 ? 16 : rows_hint <= 32 ? 32 : rows_hint <= 64 ? 64 : 128;
+  if (n_tile != 16 && n_tile != 32 && n_tile != 64 && n_tile != 128) return -1;
+  Int4Tc p;
+  p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts; p.offsets = offsets; p.status = status;
+  p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.E = E; p.F = F; p.K = K; p.flags = flags;
+  p.strips = flags & 1 ? (F + 7) / 8 : (F + 15) / 16;
+  p.steps = (K + I4_STEP - 1) / I4_STEP;
+  p.m_tiles = (p.strips + 7) / 8;
+  p.budget_ns = (uint64_t)gemm_wait_budget_ms() * 1000000ull;
+  // row tiles at most: an expert's last one may be part empty
+  const long long row_tiles = counts == nullptr ? (rows + n_tile - 1) / n_tile : (rows + (long long)(n_tile - 1) * (E < rows ? E : rows)) / n_tile;
+  const long long tiles = row_tiles * p.m_tiles;
+  if (split == 0) {
+    const long long expect = counts == nullptr ? tiles : p.m_tiles * (rows < E ? (long long)rows : (long long)E * ((rows_hint + n_tile - 1) / n_tile));
+    const int slots = 148 * (n_tile == 128 ? 1 : 2);
+    split = 1;
+    while (split < 8 && expect * split * 2 <= slots && p.steps / (split * 2) >= 2) split *= 2;
+  }
+  if (split != 1 && split != 2 && split != 4 && split != 8) return -1;
+  if (tiles * split > 0x7fffffffll) return -1;
+  p.split = split;
+  CUtensorMap tmX;
+  const int rc = make_tmap_2d(&tmX, x, (uint64_t)x_rows, (uint64_t)K, (uint64_t)x_ld, 2, src_row != nullptr ? 1 : n_tile);
+  if (rc) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  switch (n_tile) {
+    case 16: return launch_tc_group<16>(tmX, p, group, (int)tiles, s);
+    case 32: return launch_tc_group<32>(tmX, p, group, (int)tiles, s);
+    case 64: return launch_tc_group<64>(tmX, p, group, (int)tiles, s);
+    default: return launch_tc_group<128>(tmX, p, group, (int)tiles, s);
+  }
+}

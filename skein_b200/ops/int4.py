@@ -14,41 +14,43 @@ import torch
 from . import _lib, functional as F, reference_int4 as ri
 
 GROUPS = (32, 64, 128)
-STRIP, STEP = 16, 128      # rows and elements of K of a packed block
+STEP = 128                 # elements of K of a packed block (16 rows)
+CODES = 16 * STEP // 2     # its bytes of codes
 MAX_EXPERTS = 65535
 
 
 class Int4Weight:
-    """codes uint8 [matrices, strips, steps, 1024], scale 16-bit [matrices, strips, steps, 8, 128 / group, 2], zero uint8 of the same shape or None
-    (csrc/kernels/int4.cuh). `shape` is the logical [rows, K] or [experts, rows, K]; `pair`: gate rows, then up rows, packed side by side for the
-    SwiGLU product."""
+    """data uint8 [matrices, strips, steps, bytes of a block]: codes, scales and zeros of 16 rows x 128 of K (csrc/kernels/int4.cuh). `shape` is the logical
+    [rows, K] or [experts, rows, K]; `pair`: gate rows, then up rows, packed side by side for the SwiGLU product."""
 
-    def __init__(self, codes, scale, zero, shape, group, pair):
-        self.codes, self.scale, self.zero = codes, scale, zero
-        self.shape, self.group, self.pair = tuple(shape), group, pair
-        self.device = codes.device
+    def __init__(self, data, shape, group, pair, scales, zeros):
+        self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
+        self.scales, self.zeros = scales, zeros
+        self.device = data.device
         self.features = shape[-2] // 2 if pair else shape[-2]
-        self.flags = int(pair) | (2 if scale.dtype == torch.float16 else 0)
+        self.flags = int(pair) | (2 if scales == torch.float16 else 0) | (8 if zeros else 0)
 
     @property
     def is_cuda(self):
-        return self.codes.is_cuda
+        return self.data.is_cuda
 
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scale.numel() * 2 + (self.zero.numel() if self.zero is not None else 0)
+        return self.data.numel()
 
     def parts(self):
         """(codes [..., rows, K / 2], scale [..., rows, K / group], zero or None) as pack_weight takes them."""
         *lead, rows, K = self.shape
-        n, S, B = self.codes.shape[:3]
-        w = self.codes.view(torch.int32).view(n, S, B, 2, 8, 4, 2, 2).permute(0, 1, 6, 4, 2, 3, 7, 5)      # [n, S, half, g, B, j, h, t]
+        n, S, B = self.data.shape[:3]
+        per = STEP // self.group
+        codes, scale, zero = self.data.split((CODES, 32 * per, 16 * per if self.zeros else 0), -1)
+        w = codes.contiguous().view(torch.int32).view(n, S, B, 2, 4, 8, 2, 2).permute(0, 1, 6, 5, 2, 3, 7, 4)      # [n, S, half, g, B, j, h, t]
         w = _rows_out(w.reshape(n, S, 2, 8, B * 16), self.pair, rows)[:, :, :K // 8]
-        codes = _interleave(w.contiguous()).view(torch.uint8).reshape(*lead, rows, K // 2)
 
         def back(t):
-            u = t.permute(0, 1, 5, 3, 2, 4).reshape(n, S, 2, 8, -1)
+            u = t.view(n, S, B, 8, per, 2).permute(0, 1, 5, 3, 2, 4).reshape(n, S, 2, 8, -1)
             return _rows_out(u, self.pair, rows)[:, :, :K // self.group].reshape(*lead, rows, K // self.group)
-        return codes, back(self.scale), None if self.zero is None else back(self.zero)
+        return (_interleave(w.contiguous()).view(torch.uint8).reshape(*lead, rows, K // 2), back(scale.contiguous().view(self.scales)),
+                back(zero) if self.zeros else None)
 
     def dequant(self) -> torch.Tensor:
         """The weight in fp32, in its logical shape."""
@@ -56,12 +58,9 @@ class Int4Weight:
 
     def copy_(self, src: "Int4Weight"):
         """In-place update (hot swap keeps the storage that captured CUDA graphs point at)."""
-        if (src.shape, src.group, src.pair, src.scale.dtype, src.zero is None) != (self.shape, self.group, self.pair, self.scale.dtype, self.zero is None):
+        if (src.shape, src.group, src.pair, src.scales, src.zeros) != (self.shape, self.group, self.pair, self.scales, self.zeros):
             raise ValueError("int4 weight: another shape, group, pairing or type of scales")
-        self.codes.copy_(src.codes)
-        self.scale.copy_(src.scale)
-        if self.zero is not None:
-            self.zero.copy_(src.zero)
+        self.data.copy_(src.data)
         return self
 
 
@@ -128,15 +127,19 @@ def pack_weight(codes, scale, zero=None, pair=False) -> Int4Weight:
     B = -(-K // STEP)
     w = _rows_in(_deinterleave(codes.reshape(n, rows, half).contiguous().view(torch.int32)), pair, S)        # [n, S, half, g, K / 8]
     w = torch.nn.functional.pad(w, (0, B * 16 - w.shape[-1])) if w.shape[-1] < B * 16 else w
-    w = w.reshape(n, S, 2, 8, B, 2, 2, 4).permute(0, 1, 4, 5, 3, 7, 2, 6).contiguous()                       # [n, S, B, j, g, t, half, h]
     per = STEP // group
+    data = codes.new_empty(n, S, B, CODES + per * (48 if zero is not None else 32))
+    data[..., :CODES].view(torch.int32).view(n, S, B, 2, 4, 8, 2, 2).copy_(w.reshape(n, S, 2, 8, B, 2, 2, 4).permute(0, 1, 4, 5, 7, 3, 2, 6))
 
-    def lay(t):
+    def lay(t, first, wide):
         t = _rows_in(t.reshape(n, rows, -1), pair, S)
         if t.shape[-1] < B * per:
             t = torch.nn.functional.pad(t, (0, B * per - t.shape[-1]))
-        return t.reshape(n, S, 2, 8, B, per).permute(0, 1, 4, 3, 5, 2).contiguous()
-    return Int4Weight(w.view(n, S, B, -1).view(torch.uint8), lay(scale), None if zero is None else lay(zero), (*lead, rows, K), group, bool(pair))
+        data[..., first:first + 16 * per * wide].view(t.dtype).view(n, S, B, 8, per, 2).copy_(t.reshape(n, S, 2, 8, B, per).permute(0, 1, 4, 3, 5, 2))
+    lay(scale, CODES, 2)
+    if zero is not None:
+        lay(zero, CODES + 32 * per, 1)
+    return Int4Weight(data, (*lead, rows, K), group, bool(pair), scale.dtype, zero is not None)
 
 
 def quantize_weight(w: torch.Tensor, group: int = 128, symmetric: bool = True, pair: bool = False) -> Int4Weight:
@@ -177,29 +180,35 @@ def _out(what, out, rows, w, dtype, device):
     return out
 
 
-def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags):
-    rc = _lib.lib().skein_int4_rows(
-        x.data_ptr(), x.stride(0), _lib.ptr(src_row), w.codes.data_ptr(), w.scale.data_ptr(), _lib.ptr(w.zero), _lib.ptr(residual), out.data_ptr(),
-        out.stride(0), _lib.ptr(counts), _lib.ptr(offsets), rows, x.shape[0], w.codes.shape[0], w.features, w.shape[-1], w.group, hint, flags,
-        F.workspace(x.device).status.data_ptr(), _lib.stream_ptr())
+def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags, cfg=None):
+    """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, n_tile 0 for the kernel of few rows."""
+    L, data = _lib.lib(), w.data
+    args = (x.data_ptr(), x.stride(0), _lib.ptr(src_row), data.data_ptr(), _lib.ptr(residual), out.data_ptr(), out.stride(0), _lib.ptr(counts),
+            _lib.ptr(offsets), rows, x.shape[0], data.shape[0], w.features, w.shape[-1], w.group, hint, flags)
+    status, stream = F.workspace(x.device).status.data_ptr(), _lib.stream_ptr()
+    aligned = args[0] % 16 == 0 and args[1] % 8 == 0
+    if aligned and (hint > 8 if cfg is None else cfg[0] > 0):
+        rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), status, stream)
+    else:
+        rc = L.skein_int4_rows(*args, status, stream)
     _lib.check(rc, what)
     _lib.count_launch()
 
 
-def linear(x, w: Int4Weight, out=None, residual=None, out_f32=False):
+def linear(x, w: Int4Weight, out=None, residual=None, out_f32=False, _cfg=None):
     """y[t, f] = sum_k x[t, k] W[f, k] (+ residual[t, f]) for bf16 x [T, K] (rows may be strided). out_f32: y and the residual are fp32, else both are
     bf16. out may be the residual, or a run of columns of a wider matrix."""
     _check("int4 linear", x, w, False, 2)
-    return _dense("int4 linear", x, w, out, residual, out_f32)
+    return _dense("int4 linear", x, w, out, residual, out_f32, _cfg)
 
 
-def swiglu_linear(x, w: Int4Weight, out=None):
+def swiglu_linear(x, w: Int4Weight, out=None, _cfg=None):
     """silu(x Wg^T) * (x Wu^T) with both products from one pass over x; w is packed as a pair."""
     _check("int4 swiglu_linear", x, w, True, 2)
-    return _dense("int4 swiglu_linear", x, w, out, None, False)
+    return _dense("int4 swiglu_linear", x, w, out, None, False, _cfg)
 
 
-def _dense(what, x, w, out, residual, out_f32):
+def _dense(what, x, w, out, residual, out_f32, cfg):
     T = x.shape[0]
     out = _out(what, out, T, w, torch.float32 if out_f32 else torch.bfloat16, x.device)
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
@@ -210,11 +219,11 @@ def _dense(what, x, w, out, residual, out_f32):
     if not x.is_cuda:
         return out.copy_(ri.product(x, w.dequant(), residual, out_f32, w.pair))
     with _lib.on_device(x):
-        _launch(what, x, w, out, residual, None, None, None, T, T, w.flags | (4 if out_f32 else 0))
+        _launch(what, x, w, out, residual, None, None, None, T, T, w.flags | (4 if out_f32 else 0), cfg)
     return out
 
 
-def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None, out=None, rows_hint=None):
+def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None, out=None, rows_hint=None, _cfg=None):
     """Per-expert linear over expert-sorted rows. counts / offsets are int32 device tensors of E (offsets may have E + 1) entries: rows of expert e are
     offsets[e] : offsets[e] + counts[e] of the result. They read the same rows of x, or with src_row (int32, one entry per row of the result) rows
     src_row[r]: the tokens themselves, without a sorted copy. Rows not covered by any expert are left untouched (uninitialised in a result that the call
@@ -231,9 +240,11 @@ def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None
     out = _out(what, out, rows, w, torch.bfloat16, x.device)
     if rows == 0:
         return out
+    if x.shape[0] == 0:
+        raise ValueError(f"{what}: src_row names rows of an empty x")
     if not x.is_cuda:
         return ri.grouped_product(x, w.dequant(), counts[:E], offsets[:E], swiglu, src_row, out)
     hint = -(-(rows if rows_hint is None else max(1, min(int(rows_hint), rows))) // E)
     with _lib.on_device(x):
-        _launch(what, x, w, out, None, counts, offsets, src_row, rows, hint, w.flags)
+        _launch(what, x, w, out, None, counts, offsets, src_row, rows, hint, w.flags, _cfg)
     return out

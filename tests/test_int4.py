@@ -29,13 +29,15 @@ def test_place_of_a_code():
     """csrc/kernels/int4.cuh: code of row 16 s + 8 half + g, k = 128 b + 64 j + 32 h + 8 t + i."""
     codes, scale, zero = parts((), 40, 384, 64, True)
     w = int4.pack_weight(codes, scale, zero)
-    raw = w.codes.view(torch.int32)
+    raw, scales, zeros = w.data[..., :1024].view(torch.int32), w.data[..., 1024:1088].view(torch.float16), w.data[..., 1088:]
+    assert w.data.shape == (1, 3, 3, 1024 + 64 + 32)
     for row, k in ((0, 0), (7, 9), (8, 0), (39, 383), (17, 200), (26, 127), (33, 256 + 77)):
         s, half, g = row // 16, row % 16 // 8, row % 8
         b, j, h, t, i = k // 128, k % 128 // 64, k % 64 // 32, k % 32 // 8, k % 8
-        word = int(raw[0, s, b, (j * 32 + g * 4 + t) * 4 + 2 * half + h]) & 0xffffffff
+        word = int(raw[0, s, b, (j * 32 + t * 8 + g) * 4 + 2 * half + h]) & 0xffffffff
         assert word >> (4 * (i // 2) + 16 * (i % 2)) & 15 == int(codes[row, k // 2]) >> (4 * (k % 2)) & 15
-        assert w.scale[0, s, b, g, k % 128 // 64, half] == scale[row, k // 64] and w.zero[0, s, b, g, k % 128 // 64, half] == zero[row, k // 64]
+        at = (g * 2 + k % 128 // 64) * 2 + half
+        assert scales[0, s, b, at] == scale[row, k // 64] and zeros[0, s, b, at] == zero[row, k // 64]
 
 
 @pytest.mark.parametrize("symmetric", [True, False])

@@ -63,6 +63,25 @@ def test_linear(rows, features, K, group, zeros, scales):
     within(rb, x, full, residual=keep)
 
 
+KERNELS = [(0, 0), (16, 1), (16, 2), (16, 8), (32, 1), (32, 4), (64, 1), (64, 8), (128, 1), (128, 2), (128, 8)]
+
+
+@pytest.mark.parametrize("cfg", KERNELS)
+@pytest.mark.parametrize("rows, features, K, group, zeros, scales", [SIZES[1], SIZES[2], SIZES[3], SIZES[6], SIZES[10], SIZES[11]])
+def test_every_kernel_takes_every_size(rows, features, K, group, zeros, scales, cfg):
+    w, full = weight((), features, K, group, zeros, scales, False)
+    x = acts(rows, K)
+    within(int4.linear(x, w, out_f32=True, _cfg=cfg), x, full, half_step=2.0 ** -24)
+    w, full = weight((3,), 2 * features, K, group, zeros, scales, True)
+    cnt = torch.tensor([rows, 0, 2 * rows], dtype=torch.int32, device=DEV)
+    off = torch.tensor([0, rows, rows, 3 * rows], dtype=torch.int32, device=DEV)
+    src = torch.randint(0, rows, (3 * rows,), device=DEV, dtype=torch.int32)
+    y = int4.grouped_linear(x, w, cnt, off, swiglu=True, src_row=src, _cfg=cfg)
+    within(y[:rows], x[src[:rows].long()], full[0], True)
+    within(y[rows:], x[src[rows:].long()], full[2], True)
+    ops.workspace().check_status()
+
+
 @pytest.mark.parametrize("rows, features, K, group, zeros, scales", SIZES)
 def test_swiglu_linear(rows, features, K, group, zeros, scales):
     w, full = weight((), 2 * features, K, group, zeros, scales, True)

@@ -2,11 +2,12 @@
 //
 //   W[f, k] = scale[f, k / group] * (code[f, k] - zero[f, k / group]),   code 0 .. 15, zero 0 .. 15 (8 where there is none), group 32, 64 or 128
 //
-// A matrix is cut into strips of 16 rows and steps of 128 along K (skein_b200/ops/int4.py packs it; rows and K are padded). For a pair of
-// matrices (gate and up of a SwiGLU) a strip holds 8 gate rows and the 8 up rows of the same features, so that whoever holds accumulator
-// row r of a strip has its partner at r + 8.
-// A block (strip, step) is one record of memory, codes, then scales, then zeros where there are any, so that it arrives in one copy; the records of
-// a strip follow one another along K.
+// A matrix is cut into strips of 16 rows, tiles of eight strips and steps of 128 along K (skein_b200/ops/int4.py packs it; rows and K are padded with
+// zero scales). For a pair of matrices (gate and up of a SwiGLU) a strip holds 8 gate rows and the 8 up rows of the same features, so that whoever
+// holds accumulator row r of a strip has its partner at r + 8.
+// A step of a tile is one run of memory, a multiple of 128 bytes: the codes of its strips, then their scales, then their zeros where there are any. One
+// bulk copy fetches it. (Strips with scales of their own, 1056 bytes each, made the copies start off 128-byte boundaries, which the copy engine
+// takes 16 bytes at a time: 140 cycles per KB, three quarters of the tensor-memory kernel's time.)
 //   codes  [2][t 4][g 8][16 bytes]: lane (g = lane / 4, t = lane % 4) of half j owns rows g and g + 8 at k = 64 j + 8 t .. + 7 and
 //          64 j + 32 + 8 t .. + 7: words {row g, first; row g, second; row g + 8, first; row g + 8, second}. One 16-byte load of a warp is 16 rows x
 //          64 k in the order in which mma.sync's A operand wants them (any order of k is right as long as B has the same). The row's eight
@@ -24,8 +25,11 @@
 namespace skein {
 
 constexpr int I4_STEP = 128;                       // elements of K
-constexpr int I4_CODES = 16 * I4_STEP / 2;         // bytes of a record's codes
-__host__ __device__ constexpr int i4_record(int gp, bool zero) { return I4_CODES + 32 * gp + (zero ? 16 * gp : 0); }     // gp: groups of a step
+constexpr int I4_CODES = 16 * I4_STEP / 2;         // bytes of a strip's codes in a step
+// bytes of a tile's step; gp: groups of a step
+__host__ __device__ constexpr int i4_record(int gp, bool zero) { return 8 * (I4_CODES + 32 * gp + (zero ? 16 * gp : 0)); }
+constexpr int I4_SCALES = 8 * I4_CODES;            // where its scales begin
+__host__ __device__ constexpr int i4_zeros(int gp) { return I4_SCALES + 8 * 32 * gp; }
 
 // code pair -> bf16 pair 128 + code: the codes are the low mantissa bits of a bf16 whose unit in the last place is 1
 __device__ __forceinline__ uint32_t i4_magic(uint32_t word, int i) {

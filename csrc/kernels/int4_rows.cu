@@ -46,17 +46,17 @@ struct Int4Step {       // a lane's part of a step of one strip
   uint4 c[2];
   uint32_t s[GP];       // scales of rows g and g + 8
   uint16_t z[GP];
-  __device__ __forceinline__ void load(const uint8_t* rec, int lane) {
+  __device__ __forceinline__ void load(const uint8_t* rec, int strip, int lane) {
     const int g = lane >> 2;
-    const uint8_t* at = rec + ((lane & 3) * 8 + g) * 16;
+    const uint8_t* at = rec + strip * I4_CODES + ((lane & 3) * 8 + g) * 16;
     c[0] = __ldcs(reinterpret_cast<const uint4*>(at));
     c[1] = __ldcs(reinterpret_cast<const uint4*>(at + 512));
-    const uint32_t* sp = reinterpret_cast<const uint32_t*>(rec + I4_CODES) + g * GP;
+    const uint32_t* sp = reinterpret_cast<const uint32_t*>(rec + I4_SCALES) + (strip * 8 + g) * GP;
     if constexpr (GP == 1) s[0] = __ldg(sp);
     if constexpr (GP == 2) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp)); s[0] = v.x; s[1] = v.y; }
     if constexpr (GP == 4) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(sp)); s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w; }
     if constexpr (ZERO) {
-      const uint16_t* zp = reinterpret_cast<const uint16_t*>(rec + I4_CODES + 32 * GP) + g * GP;
+      const uint16_t* zp = reinterpret_cast<const uint16_t*>(rec + i4_zeros(GP)) + (strip * 8 + g) * GP;
       if constexpr (GP == 1) z[0] = __ldg(zp);
       if constexpr (GP == 2) { const ushort2 v = __ldg(reinterpret_cast<const ushort2*>(zp)); z[0] = v.x; z[1] = v.y; }
       if constexpr (GP == 4) { const ushort4 v = __ldg(reinterpret_cast<const ushort4*>(zp)); z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w; }
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(IR_THREADS) int4_rows_kernel(const Int4Rows p)
   }
   const bool live = strip < p.strips;
   constexpr int REC = i4_record(GP, ZERO);
-  const uint8_t* strip_w = p.w + ((size_t)e * p.strips + (live ? strip : 0)) * p.steps * REC;
+  const uint8_t* tile_w = p.w + ((size_t)e * ((p.strips + 7) / 8) + (live ? strip >> 3 : 0)) * p.steps * REC;
   for (int tile = blockIdx.z; tile * 8 * NT < count; tile += gridDim.z) {
     const __nv_bfloat16* row[NT];
 #pragma unroll
@@ -105,14 +105,14 @@ __global__ void __launch_bounds__(IR_THREADS) int4_rows_kernel(const Int4Rows p)
     Int4Step<GP, ZERO> buf[IR_DEPTH];
 #pragma unroll
     for (int d = 0; d < IR_DEPTH; ++d)
-      if (live && part + d * WK < p.steps) buf[d].load(strip_w + (size_t)(part + d * WK) * REC, lane);
+      if (live && part + d * WK < p.steps) buf[d].load(tile_w + (size_t)(part + d * WK) * REC, strip & 7, lane);
     for (int s0 = part; s0 < p.steps; s0 += IR_DEPTH * WK) {
 #pragma unroll
       for (int d = 0; d < IR_DEPTH; ++d) {
         const int step = s0 + d * WK;
         if (step >= p.steps || !live) break;
         const Int4Step<GP, ZERO> cur = buf[d];
-        if (step + IR_DEPTH * WK < p.steps) buf[d].load(strip_w + (size_t)(step + IR_DEPTH * WK) * REC, lane);
+        if (step + IR_DEPTH * WK < p.steps) buf[d].load(tile_w + (size_t)(step + IR_DEPTH * WK) * REC, strip & 7, lane);
         float part_sum[NT][4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {             // 32 of K each

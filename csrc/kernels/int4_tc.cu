@@ -2,7 +2,7 @@
 //
 // Weights are the M side (128 rows of a tile), NT rows of x the N side. A CTA owns a tile, or with few tiles a piece of its K (the CTAs of a cluster
 // share the tile). Roles, one pipeline:
-//   producer    one bulk copy per strip (codes, scales and zeros of 16 rows x 128 of K are one record) and TMA tiles of x, or of the rows that
+//   producer    one bulk copy per step (codes, scales and zeros of 128 rows x 128 of K are one run) and TMA tiles of x, or of the rows that
 //               src_row names (tile::gather4), into a ring of shared-memory stages
 //   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (whole numbers, exact), 64 of K a slot, written to tensor
 //               memory as the A operand
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   const bool zeros = p.flags & 8;
   const int rec = i4_record(GP, zeros);
   constexpr int X_BYTES = NT * 256;
-  const int stage_bytes = X_BYTES + ((8 * rec + 1023) & ~1023);
+  const int stage_bytes = X_BYTES + ((rec + 1023) & ~1023);
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
@@ -147,37 +147,37 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   float acc[S::EPI_COLS];
 
   if (live) {
-    const uint8_t* w = p.w + ((size_t)e * p.strips + (size_t)m * 8) * p.steps * rec;
-    const int my_strips = min(8, p.strips - m * 8);
+    const uint8_t* w = p.w + ((size_t)e * p.m_tiles + m) * p.steps * rec;
     if (warp == 0) {
       // ================= producer =================
-      if (elect_one()) {
-        tma_prefetch_desc(&tmX);
-        const uint64_t keep = l2_policy_evict_last();
-        int st = 0;
-        uint32_t ph = 0;
-        for (int s = s0; s < s1; ++s) {
-          if (!mbar_wait(smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
-            report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x);
-            abort_flag = 1;
-            break;
-          }
-          const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
-          mbar_expect_tx(full, X_BYTES + my_strips * rec);
-          for (int i = 0; i < my_strips; ++i) bulk_load_1d(at + X_BYTES + i * rec, w + ((size_t)i * p.steps + s) * rec, rec, full);
+      if (lane == 0) tma_prefetch_desc(&tmX);
+      const uint64_t keep = l2_policy_evict_last();
+      int st = 0;
+      uint32_t ph = 0;
+      for (int s = s0; s < s1; ++s) {
+        if (!it_warp_wait(smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
+          if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
+          break;
+        }
+        const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
+        if (lane == 0) {
+          mbar_expect_tx(full, X_BYTES + rec);
+          bulk_load_1d(at + X_BYTES, w + (size_t)s * rec, rec, full);
           if (p.src_row == nullptr) {
             tma_load_2d(at, &tmX, full, s * I4_STEP, row0, keep);
             tma_load_2d(at + NT * 128, &tmX, full, s * I4_STEP + 64, row0, keep);
-          } else {
-            // a half that lies behind K as a whole has scales of zero: any columns do
-            const int x1 = s * I4_STEP + 64 < p.K ? s * I4_STEP + 64 : 0;
-            for (int i = 0; i < NT; i += 4) {
-              it_gather4(at + i * 128, &tmX, full, s * I4_STEP, src[i], src[i + 1], src[i + 2], src[i + 3]);
-              it_gather4(at + NT * 128 + i * 128, &tmX, full, x1, src[i], src[i + 1], src[i + 2], src[i + 3]);
-            }
           }
-          if (++st == p.stages) { st = 0; ph ^= 1; }
         }
+        __syncwarp();
+        if (p.src_row != nullptr) {
+          // a half that lies behind K as a whole has scales of zero: any columns do
+          const int x1 = s * I4_STEP + 64 < p.K ? s * I4_STEP + 64 : 0;
+          for (int i = lane; i < NT / 2; i += 32) {
+            const int j = i & 1, q = (i >> 1) * 4;
+            it_gather4(at + j * NT * 128 + q * 128, &tmX, full, j ? x1 : s * I4_STEP, src[q], src[q + 1], src[q + 2], src[q + 3]);
+          }
+        }
+        if (++st == p.stages) { st = 0; ph ^= 1; }
       }
       __syncwarp();
     } else if (warp == 1) {
@@ -227,8 +227,8 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       const int r = (warp & 3) * 32 + lane, group = (warp - 4) >> 2;
       constexpr int GROUPS = S::CONV_WARPS / 4;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
-      const int in_stage = X_BYTES + (r >> 4) * rec + (r & 7) * 16 + ((r >> 3) & 1) * 8;
-      const int zero_at = X_BYTES + (r >> 4) * rec + I4_CODES + 32 * GP + (r & 7) * GP * 2 + ((r >> 3) & 1);
+      const int in_stage = X_BYTES + (r >> 4) * I4_CODES + (r & 7) * 16 + ((r >> 3) & 1) * 8;
+      const int zero_at = X_BYTES + i4_zeros(GP) + ((r >> 4) * 8 + (r & 7)) * GP * 2 + ((r >> 3) & 1);
       int st = 0, slot = group;
       uint32_t ph = 0, sph = 0;
       bool ok = true;
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       // ================= epilogue: row r, columns col0 .. + EPI_COLS =================
       const int r = (warp & 3) * 32 + lane, col0 = ((warp - 4 - S::CONV_WARPS) >> 2) * S::EPI_COLS;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
-      const int scale_at = X_BYTES + (r >> 4) * rec + I4_CODES + (r & 7) * GP * 4 + ((r >> 3) & 1) * 2;
+      const int scale_at = X_BYTES + I4_SCALES + ((r >> 4) * 8 + (r & 7)) * GP * 4 + ((r >> 3) & 1) * 2;
 #pragma unroll
       for (int c = 0; c < S::EPI_COLS; ++c) acc[c] = 0.f;
       int st = 0, buf = 0;
@@ -392,7 +392,7 @@ static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s
   using S = ItShape<NT>;
   static PerDevice allowed;
   const int room = (S::WIDE ? 225 : 111) * 1024;
-  const int stage = NT * 256 + ((8 * i4_record(GP, p.flags & 8) + 1023) & ~1023);
+  const int stage = NT * 256 + ((i4_record(GP, p.flags & 8) + 1023) & ~1023);
   p.stages = (room - 1024) / stage;
   if (p.stages > IT_MAX_STAGES) p.stages = IT_MAX_STAGES;
   const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP>, room);

@@ -20,8 +20,8 @@ MAX_EXPERTS = 65535
 
 
 class Int4Weight:
-    """data uint8 [matrices, strips, steps, bytes of a block]: codes, scales and zeros of 16 rows x 128 of K (csrc/kernels/int4.cuh). `shape` is the logical
-    [rows, K] or [experts, rows, K]; `pair`: gate rows, then up rows, packed side by side for the SwiGLU product."""
+    """data uint8 [matrices, tiles, steps, bytes]: codes, scales and zeros of 128 rows x 128 of K (csrc/kernels/int4.cuh). `shape` is the logical [rows, K]
+    or [experts, rows, K]; `pair`: gate rows, then up rows, packed side by side for the SwiGLU product."""
 
     def __init__(self, data, shape, group, pair, scales, zeros):
         self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
@@ -40,17 +40,17 @@ class Int4Weight:
     def parts(self):
         """(codes [..., rows, K / 2], scale [..., rows, K / group], zero or None) as pack_weight takes them."""
         *lead, rows, K = self.shape
-        n, S, B = self.data.shape[:3]
-        per = STEP // self.group
-        codes, scale, zero = self.data.split((CODES, 32 * per, 16 * per if self.zeros else 0), -1)
-        w = codes.contiguous().view(torch.int32).view(n, S, B, 2, 4, 8, 2, 2).permute(0, 1, 6, 5, 2, 3, 7, 4)      # [n, S, half, g, B, j, h, t]
+        n, per = self.data.shape[0], STEP // self.group
+        S, B = 8 * self.data.shape[1], self.data.shape[2]
+        codes, scale, zero = self.data.split((8 * CODES, 8 * 32 * per, 8 * 16 * per if self.zeros else 0), -1)
+        w = codes.contiguous().view(torch.int32).view(n, S // 8, B, 8, 2, 4, 8, 2, 2).permute(0, 1, 3, 7, 6, 2, 4, 8, 5)   # [n, S, half, g, B, j, h, t]
         w = _rows_out(w.reshape(n, S, 2, 8, B * 16), self.pair, rows)[:, :, :K // 8]
 
         def back(t):
-            u = t.view(n, S, B, 8, per, 2).permute(0, 1, 5, 3, 2, 4).reshape(n, S, 2, 8, -1)
+            u = t.view(n, S // 8, B, 8, 8, per, 2).permute(0, 1, 3, 6, 4, 2, 5).reshape(n, S, 2, 8, -1)
             return _rows_out(u, self.pair, rows)[:, :, :K // self.group].reshape(*lead, rows, K // self.group)
         return (_interleave(w.contiguous()).view(torch.uint8).reshape(*lead, rows, K // 2), back(scale.contiguous().view(self.scales)),
-                back(zero) if self.zeros else None)
+                back(zero.contiguous()) if self.zeros else None)
 
     def dequant(self) -> torch.Tensor:
         """The weight in fp32, in its logical shape."""
@@ -123,22 +123,23 @@ def pack_weight(codes, scale, zero=None, pair=False) -> Int4Weight:
     n = lead[0] if lead else 1
     if n > MAX_EXPERTS:
         raise ValueError(f"int4 weight: at most {MAX_EXPERTS} experts")
-    S = -(-(rows // 2) // 8) if pair else -(-rows // 16)
-    B = -(-K // STEP)
+    S, B = -(-rows // 128) * 8 if not pair else -(-rows // 2 // 64) * 8, -(-K // STEP)
     w = _rows_in(_deinterleave(codes.reshape(n, rows, half).contiguous().view(torch.int32)), pair, S)        # [n, S, half, g, K / 8]
     w = torch.nn.functional.pad(w, (0, B * 16 - w.shape[-1])) if w.shape[-1] < B * 16 else w
     per = STEP // group
-    data = codes.new_empty(n, S, B, CODES + per * (48 if zero is not None else 32))
-    data[..., :CODES].view(torch.int32).view(n, S, B, 2, 4, 8, 2, 2).copy_(w.reshape(n, S, 2, 8, B, 2, 2, 4).permute(0, 1, 4, 5, 7, 3, 2, 6))
+    data = codes.new_empty(n, S // 8, B, 8 * (CODES + per * (48 if zero is not None else 32)))
+    to = data[..., :8 * CODES].view(torch.int32).view(n, S // 8, B, 8, 2, 4, 8, 2, 2)                        # [n, tile, B, strip, j, t, g, half, h]
+    to.copy_(w.reshape(n, S // 8, 8, 2, 8, B, 2, 2, 4).permute(0, 1, 5, 2, 6, 8, 4, 3, 7))
 
-    def lay(t, first, wide):
+    def lay(t, first, size):
         t = _rows_in(t.reshape(n, rows, -1), pair, S)
         if t.shape[-1] < B * per:
             t = torch.nn.functional.pad(t, (0, B * per - t.shape[-1]))
-        data[..., first:first + 16 * per * wide].view(t.dtype).view(n, S, B, 8, per, 2).copy_(t.reshape(n, S, 2, 8, B, per).permute(0, 1, 4, 3, 5, 2))
-    lay(scale, CODES, 2)
+        to = data[..., first:first + size].view(t.dtype).view(n, S // 8, B, 8, 8, per, 2)                    # [n, tile, B, strip, g, group, half]
+        to.copy_(t.reshape(n, S // 8, 8, 2, 8, B, per).permute(0, 1, 5, 2, 4, 6, 3))
+    lay(scale, 8 * CODES, 8 * 32 * per)
     if zero is not None:
-        lay(zero, CODES + 32 * per, 1)
+        lay(zero, 8 * (CODES + 32 * per), 8 * 16 * per)
     return Int4Weight(data, (*lead, rows, K), group, bool(pair), scale.dtype, zero is not None)
 
 

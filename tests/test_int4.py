@@ -16,7 +16,8 @@ def parts(lead, rows, K, group, zeros, scales=torch.float16):
 
 @pytest.mark.parametrize("lead, rows, K, group, pair, zeros", [
     ((), 1, 32, 32, False, False), ((), 50, 96, 32, False, True), ((3,), 22, 256, 128, True, False), ((2,), 34, 192, 64, True, True),
-    ((), 16, 128, 64, False, False), ((1,), 2, 128, 128, True, True)])
+    ((), 16, 128, 64, False, False), ((1,), 2, 128, 128, True, True),
+    ((2,), 16 * 17 + 5, 160, 32, False, True), ((), 2 * 8 * 8, 256, 64, True, False), ((3,), 2 * 77, 96, 32, True, True)])
 def test_packing_keeps_every_code_scale_and_zero(lead, rows, K, group, pair, zeros):
     given = parts(lead, rows, K, group, zeros)
     w = int4.pack_weight(*given, pair=pair)
@@ -29,15 +30,15 @@ def test_place_of_a_code():
     """csrc/kernels/int4.cuh: code of row 16 s + 8 half + g, k = 128 b + 64 j + 32 h + 8 t + i."""
     codes, scale, zero = parts((), 40, 384, 64, True)
     w = int4.pack_weight(codes, scale, zero)
-    raw, scales, zeros = w.data[..., :1024].view(torch.int32), w.data[..., 1024:1088].view(torch.float16), w.data[..., 1088:]
-    assert w.data.shape == (1, 3, 3, 1024 + 64 + 32)
+    assert w.data.shape == (1, 1, 3, 8 * (1024 + 64 + 32))
     for row, k in ((0, 0), (7, 9), (8, 0), (39, 383), (17, 200), (26, 127), (33, 256 + 77)):
         s, half, g = row // 16, row % 16 // 8, row % 8
         b, j, h, t, i = k // 128, k % 128 // 64, k % 64 // 32, k % 32 // 8, k % 8
-        word = int(raw[0, s, b, (j * 32 + t * 8 + g) * 4 + 2 * half + h]) & 0xffffffff
+        step = w.data[0, 0, b]
+        word = int(step[:8192].view(torch.int32)[((s * 2 + j) * 32 + t * 8 + g) * 4 + 2 * half + h]) & 0xffffffff
         assert word >> (4 * (i // 2) + 16 * (i % 2)) & 15 == int(codes[row, k // 2]) >> (4 * (k % 2)) & 15
-        at = (g * 2 + k % 128 // 64) * 2 + half
-        assert scales[0, s, b, at] == scale[row, k // 64] and zeros[0, s, b, at] == zero[row, k // 64]
+        at = ((s * 8 + g) * 2 + k % 128 // 64) * 2 + half
+        assert step[8192:8704].view(torch.float16)[at] == scale[row, k // 64] and step[8704:][at] == zero[row, k // 64]
 
 
 @pytest.mark.parametrize("symmetric", [True, False])

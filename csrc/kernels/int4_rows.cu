@@ -2,17 +2,21 @@
 //
 //   y[r, f] = sum over groups j of scale[f, j] * ( sum_{k in j} x[r, k] (code[f, k] - zero[f, j]) )
 //
-// With a few rows the weights' bytes bound the time, and what has to be done for each of them besides. A warp reads 16 rows of a strip x 128
-// of K with two 16-byte loads per lane, turns the codes into bf16 whole numbers (exact, three instructions per pair) and multiplies them
-// with mma.sync m16n8k16 against eight rows of x, whose fragments it reads through L1 in the order of the codes. A group's sum is fp32 and is
-// scaled in fp32, so nothing is rounded before the result. The warps of a unit share K and add their sums in shared memory in warp order.
+// With a few rows the weights' bytes bound the time, and what has to be done for each of them besides. A warp reads a step of a strip (16 rows x 128 of
+// K) with two 16-byte loads per lane, turns the codes into bf16 whole numbers (exact, 11 instructions per word of eight) and multiplies them
+// with mma.sync m16n8k16 against eight rows of x in shared memory. A group's sum is fp32 and is scaled in fp32, so nothing is rounded before the result.
+// A CTA per SM stays for the launch. WK of its 16 warps make a team that shares the K of a strip (a warp every WK-th step) and walks its run of strips;
+// the loads of the next four steps, the next strip's among them, are always on their way, and the team's sums meet in shared memory in warp order while
+// they are. The runs are equal shares of all strips that some row goes to, whatever expert they belong to.
 #include "int4.cuh"
 #include "launch.cuh"
 
 namespace skein {
 
-constexpr int IR_WARPS = 8, IR_THREADS = 32 * IR_WARPS;
-constexpr int IR_DEPTH = 4;      // steps whose codes are in flight
+constexpr int IR_WARPS = 16, IR_THREADS = 32 * IR_WARPS;
+constexpr int IR_DEPTH = 4;             // steps whose codes are in flight
+constexpr int IR_MAX_E = 1024;
+constexpr int IR_SMEM = 184 * 1024;     // for the rows of x
 
 struct Int4Rows {
   const __nv_bfloat16* x;
@@ -23,18 +27,26 @@ struct Int4Rows {
   const int *counts, *offsets;
   int* status;
   long long x_ld, out_ld;
-  int rows, x_rows, F, K, strips, steps, scale_half, out_f32, vec;
+  int rows, x_rows, E, F, K, strips, steps, scale_half, out_f32, vec, x_stage;   // x_stage: rows of a tile (8 NT, or as many as fit a team's shared memory)
 };
+
+// bytes of a row of x in shared memory: 64 past a multiple of 128, so that eight rows x 64 bytes lie in different banks
+__host__ __device__ constexpr int ir_x_row(int steps) { return steps * I4_STEP * 2 + 64; }
 
 // eight neighbours of a row of x from k on, zero past its end
 __device__ __forceinline__ uint4 ir_load_x(const __nv_bfloat16* row, int k, int K, int vec) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (row == nullptr || k >= K) return v;
-  if (vec) return *reinterpret_cast<const uint4*>(row + k);   // K is a multiple of 8
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(row + k));   // K is a multiple of 8
   const unsigned short* s = reinterpret_cast<const unsigned short*>(row + k);
   v.x = s[0] | (uint32_t)s[1] << 16; v.y = s[2] | (uint32_t)s[3] << 16;
   v.z = s[4] | (uint32_t)s[5] << 16; v.w = s[6] | (uint32_t)s[7] << 16;
   return v;
+}
+template <int THREADS>
+__device__ __forceinline__ void ir_team_sync(int team) {
+  if constexpr (THREADS == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(THREADS) : "memory");
 }
 __device__ __forceinline__ void ir_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -64,154 +76,222 @@ struct Int4Step {       // a lane's part of a step of one strip
   }
 };
 
-// grid (strips / units of a CTA, experts, tiles of 8 NT rows of an expert, which a CTA walks with that stride). WK warps share a strip's K.
-template <int NT, int GP, bool ZERO, bool PAIR, int WK>
-__global__ void __launch_bounds__(IR_THREADS) int4_rows_kernel(const Int4Rows p) {
-  constexpr int UNITS = IR_WARPS / WK;
-  __shared__ float4 sums[IR_WARPS][NT][32];
+template <int NT, int GP, bool ZERO, int WK>
+__global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows p, const bool pair) {
+  constexpr int TEAMS = IR_WARPS / WK, REC = i4_record(GP, ZERO);
+  extern __shared__ __align__(16) uint8_t x_smem[];
+  __shared__ float4 sums[2][IR_WARPS][NT][32];
+  __shared__ int pre[IR_MAX_E + 1], cnt[IR_MAX_E];      // row tiles before an expert, its rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int unit = warp / WK, part = warp % WK, strip = blockIdx.x * UNITS + unit, e = blockIdx.y;
+  const int team = warp / WK, part = warp % WK;
   pdl_trigger();
   pdl_wait();
-  int first = 0, count = p.rows;
-  if (p.counts != nullptr) {
-    first = p.offsets[e];
-    count = p.counts[e];
-    if (first < 0 || count < 0 || count > p.rows - first) {
-      if (threadIdx.x == 0 && count != 0) report_status(p.status, ST_BAD_INDEX, e);
-      count = 0;
+  if (warp == 0) {
+    int run = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      int c = 0;
+      if (e0 + lane < p.E) {
+        c = p.rows;
+        if (p.counts != nullptr) {
+          const int first = p.offsets[e0 + lane];
+          c = p.counts[e0 + lane];
+          if (first < 0 || c < 0 || c > p.rows - first) {
+            if (c != 0) report_status(p.status, ST_BAD_INDEX, e0 + lane);
+            c = 0;
+          }
+        }
+      }
+      const int tiles = (c + p.x_stage - 1) / p.x_stage;
+      int inc = tiles;
+      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+      if (e0 + lane < p.E) { pre[e0 + lane] = run + inc - tiles; cnt[e0 + lane] = c; }
+      run += __shfl_sync(0xffffffffu, inc, 31);
     }
+    if (lane == 0) pre[p.E] = run;
   }
-  const bool live = strip < p.strips;
-  constexpr int REC = i4_record(GP, ZERO);
-  const uint8_t* tile_w = p.w + ((size_t)e * ((p.strips + 7) / 8) + (live ? strip >> 3 : 0)) * p.steps * REC;
-  for (int tile = blockIdx.z; tile * 8 * NT < count; tile += gridDim.z) {
-    const __nv_bfloat16* row[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int r = tile * 8 * NT + n * 8 + g;
-      row[n] = nullptr;
-      if (r < count) {
-        const int from = p.src_row != nullptr ? p.src_row[first + r] : first + r;
-        if (from >= 0 && from < p.x_rows) row[n] = p.x + (size_t)from * p.x_ld;
-        else report_status(p.status, ST_BAD_INDEX, from);
+  __syncthreads();
+  // the team's run of units (row tile, strip), strips fastest
+  const int who = blockIdx.x * TEAMS + team, teams = gridDim.x * TEAMS;
+  const int u0 = (int)((long long)pre[p.E] * p.strips * who / teams), u1 = (int)((long long)pre[p.E] * p.strips * (who + 1) / teams);
+  const int mine = (p.steps - part + WK - 1) / WK;       // steps of a strip that this warp takes (at least one: WK <= steps)
+  // cursor of the loads, ahead of the products
+  int le = 0, lstrip = 0, li = 0;
+  int lleft = u1 - u0, ltile = 0;
+  if (lleft > 0) {
+    ltile = u0 / p.strips;
+    lstrip = u0 - ltile * p.strips;
+    while (ltile >= pre[le + 1]) ++le;
+  }
+  const size_t matrix = (size_t)((p.strips + 7) / 8) * p.steps * REC;
+  Int4Step<GP, ZERO> buf[IR_DEPTH];
+  auto load = [&](Int4Step<GP, ZERO>& b) {
+    if (lleft <= 0) return;
+    b.load(p.w + le * matrix + ((size_t)(lstrip >> 3) * p.steps + part + li * WK) * REC, lstrip & 7, lane);
+    if (++li == mine) {
+      li = 0;
+      --lleft;
+      if (++lstrip == p.strips) {
+        lstrip = 0;
+        ++ltile;
+        while (le + 1 < p.E && ltile >= pre[le + 1]) ++le;
       }
     }
-    float acc[NT][4];
+  };
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+  for (int d = 0; d < IR_DEPTH; ++d) load(buf[d]);
+
+  const int x_row = ir_x_row(p.steps);
+  uint8_t* x_team = x_smem + (size_t)team * p.x_stage * x_row;
+  int e = 0, i = 0, n_done = 0, valid = 0, row0 = 0;
+  int left = u1 - u0, tile = u0 / p.strips, staged = -1, strip = u0 - tile * p.strips;
+  const uint8_t* xb[NT];
+  float acc[NT][4];
+  while (left > 0) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-    Int4Step<GP, ZERO> buf[IR_DEPTH];
+    for (int d = 0; d < IR_DEPTH; ++d) {
+      if (left <= 0) break;
+      if (i == 0) {
 #pragma unroll
-    for (int d = 0; d < IR_DEPTH; ++d)
-      if (live && part + d * WK < p.steps) buf[d].load(tile_w + (size_t)(part + d * WK) * REC, strip & 7, lane);
-    for (int s0 = part; s0 < p.steps; s0 += IR_DEPTH * WK) {
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int d = 0; d < IR_DEPTH; ++d) {
-        const int step = s0 + d * WK;
-        if (step >= p.steps || !live) break;
-        const Int4Step<GP, ZERO> cur = buf[d];
-        if (step + IR_DEPTH * WK < p.steps) buf[d].load(tile_w + (size_t)(step + IR_DEPTH * WK) * REC, strip & 7, lane);
-        float part_sum[NT][4];
+          for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
+        if (staged != tile) {      // the rows of x of this tile; the team is past its products with those before (its sums met)
+          while (tile >= pre[e + 1]) ++e;
+          const int first = (tile - pre[e]) * p.x_stage, base = p.counts != nullptr ? p.offsets[e] : 0;
+          valid = min(p.x_stage, cnt[e] - first);
+          row0 = base + first;
+          const int chunks = p.steps * (I4_STEP / 8);
+          for (int r = part; r < valid; r += WK) {
+            const int from = p.src_row != nullptr ? p.src_row[row0 + r] : row0 + r;
+            const bool ok = from >= 0 && from < p.x_rows;
+            if (!ok && lane == 0) report_status(p.status, ST_BAD_INDEX, from);
+            const __nv_bfloat16* row = ok ? p.x + (size_t)from * p.x_ld : nullptr;
+            for (int c = lane; c < chunks; c += 32) *reinterpret_cast<uint4*>(x_team + (size_t)r * x_row + c * 16) = ir_load_x(row, c * 8, p.K, p.vec);
+          }
+          staged = tile;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {             // 32 of K each
-          const int grp = q * GP / 4;
-          if (q * GP % 4 == 0)
+          for (int n = 0; n < NT; ++n) xb[n] = x_team + (size_t)min(n * 8 + g, valid - 1) * x_row + t * 16;
+          ir_team_sync<WK * 32>(team);
+        }
+      }
+      const Int4Step<GP, ZERO> cur = buf[d];
+      load(buf[d]);
+      const int at = (part + i * WK) * I4_STEP * 2;
+      float part_sum[NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+      for (int q = 0; q < 4; ++q) {             // 32 of K each
+        const int grp = q * GP / 4;
+        if (q * GP % 4 == 0)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) part_sum[n][i] = 0.f;
-          const uint4 c = cur.c[q >> 1];
-          uint32_t lo[4], hi[4];
-          i4_expand(q & 1 ? c.y : c.x, i4_base(ZERO ? cur.z[grp] & 0xff : 8), lo);
-          i4_expand(q & 1 ? c.w : c.z, i4_base(ZERO ? cur.z[grp] >> 8 : 8), hi);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part_sum[n][k] = 0.f;
+        const uint4 c = cur.c[q >> 1];
+        uint32_t lo[4], hi[4];
+        i4_expand(q & 1 ? c.y : c.x, i4_base(ZERO ? cur.z[grp] & 0xff : 8), lo);
+        i4_expand(q & 1 ? c.w : c.z, i4_base(ZERO ? cur.z[grp] >> 8 : 8), hi);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 b = *reinterpret_cast<const uint4*>(xb[n] + at + q * 64);
+          ir_mma(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+          ir_mma(part_sum[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
+        }
+        if ((q + 1) * GP % 4 == 0) {
+          const float sl = i4_scale(cur.s[grp] & 0xffff, p.scale_half), sh = i4_scale(cur.s[grp] >> 16, p.scale_half);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint4 b = ir_load_x(row[n], step * I4_STEP + q * 32 + t * 8, p.K, p.vec);
-            ir_mma(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-            ir_mma(part_sum[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
-          }
-          if ((q + 1) * GP % 4 == 0) {
-            const float sl = i4_scale(cur.s[grp] & 0xffff, p.scale_half), sh = i4_scale(cur.s[grp] >> 16, p.scale_half);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              acc[n][0] += sl * part_sum[n][0]; acc[n][1] += sl * part_sum[n][1];
-              acc[n][2] += sh * part_sum[n][2]; acc[n][3] += sh * part_sum[n][3];
-            }
+            acc[n][0] += sl * part_sum[n][0]; acc[n][1] += sl * part_sum[n][1];
+            acc[n][2] += sh * part_sum[n][2]; acc[n][3] += sh * part_sum[n][3];
           }
         }
       }
-    }
-    __syncthreads();              // the sums of the tile before are read
+      if (++i < mine) continue;
+      // the strip's sums
+      i = 0;
+      --left;
+      float4 (*mine_sums)[NT][32] = sums[n_done & 1];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) sums[warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-    __syncthreads();
-    for (int n = part; n < NT; n += WK) {
-      float4 v = sums[unit * WK][n][lane];
+      for (int n = 0; n < NT; ++n) mine_sums[warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+      ir_team_sync<WK * 32>(team);
 #pragma unroll
-      for (int w = 1; w < WK; ++w) {
-        const float4 o = sums[unit * WK + w][n][lane];
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-      }
-      // v: (row g, x rows 2t and 2t + 1), (row g + 8, the same)
+      for (int n = 0; n < NT; ++n) {
+        if ((n_done + n) % WK != part) continue;       // the warps take turns
+        float4 v = mine_sums[team * WK][n][lane];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = tile * 8 * NT + n * 8 + 2 * t + j;
-        if (r >= count || !live) continue;
-        const float a = j ? v.y : v.x, b = j ? v.w : v.z;
-        const size_t at = (size_t)(first + r) * p.out_ld;
+        for (int w = 1; w < WK; ++w) {
+          const float4 o = mine_sums[team * WK + w][n][lane];
+          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+        }
+        // v: (row g, x rows 2t and 2t + 1), (row g + 8, the same)
 #pragma unroll
-        for (int h = 0; h < (PAIR ? 1 : 2); ++h) {
-          const int f = PAIR ? strip * 8 + g : strip * 16 + g + 8 * h;
-          if (f >= p.F) continue;
-          float y = PAIR ? silu(a) * b : h ? b : a;
-          if (p.out_f32) ((float*)p.out)[at + f] = p.residual ? y + ((const float*)p.residual)[at + f] : y;
-          else ((__nv_bfloat16*)p.out)[at + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[at + f]) : y);
+        for (int j = 0; j < 2; ++j) {
+          const int r = n * 8 + 2 * t + j;
+          if (r >= valid) continue;
+          const float a = j ? v.y : v.x, b = j ? v.w : v.z;
+          const size_t to = (size_t)(row0 + r) * p.out_ld;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (pair && h) continue;
+            const int f = pair ? strip * 8 + g : strip * 16 + g + 8 * h;
+            if (f >= p.F) continue;
+            const float y = pair ? silu(a) * b : h ? b : a;
+            if (p.out_f32) ((float*)p.out)[to + f] = p.residual ? y + ((const float*)p.residual)[to + f] : y;
+            else ((__nv_bfloat16*)p.out)[to + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[to + f]) : y);
+          }
         }
       }
+      ++n_done;
+      if (++strip == p.strips) { strip = 0; ++tile; }
     }
   }
 }
 
-template <int NT, int GP, bool ZERO, bool PAIR, int WK>
-static int launch_rows(const Int4Rows& p, int E, int tiles, cudaStream_t s) {
-  constexpr int UNITS = IR_WARPS / WK;
-  return (int)launch_pdl(int4_rows_kernel<NT, GP, ZERO, PAIR, WK>, dim3((p.strips + UNITS - 1) / UNITS, E, tiles), dim3(IR_THREADS), 0, s, p);
+template <int NT, int GP, bool ZERO, int WK>
+static int launch_rows(Int4Rows p, bool pair, cudaStream_t s) {
+  static PerDevice allowed;
+  const int fit = IR_SMEM / (IR_WARPS / WK) / ir_x_row(p.steps);
+  p.x_stage = min(min(8 * NT, p.rows), fit);
+  if (p.x_stage < 1 || ((long long)p.rows / p.x_stage + min(p.E, p.rows)) * p.strips > 0x7fffffffll) return -1;
+  const size_t smem = (size_t)(IR_WARPS / WK) * p.x_stage * ir_x_row(p.steps);
+  const cudaError_t e = allow_smem(allowed, (const void*)int4_rows_kernel<NT, GP, ZERO, WK>, IR_SMEM);
+  if (e != cudaSuccess) return (int)e;
+  return (int)launch_pdl(int4_rows_kernel<NT, GP, ZERO, WK>, dim3(148), dim3(IR_THREADS), smem, s, p, pair);
 }
+// warps of a team: as many as leave each three steps or more of a strip, and more where its rows of x do not fit a smaller team's shared memory
 template <int NT, int GP, bool ZERO>
-static int pick_pair(const Int4Rows& p, bool pair, int E, int tiles, cudaStream_t s) {
-  return pair ? launch_rows<NT, GP, ZERO, true, 8>(p, E, tiles, s) : launch_rows<NT, GP, ZERO, false, 8>(p, E, tiles, s);
+static int pick_team(const Int4Rows& p, bool pair, cudaStream_t s) {
+  const int x = min(8 * NT, p.rows) * ir_x_row(p.steps);
+  if (p.steps >= 48 || (p.steps >= 16 && x > IR_SMEM / 2)) return launch_rows<NT, GP, ZERO, 16>(p, pair, s);
+  if (p.steps >= 24 || (p.steps >= 8 && x > IR_SMEM / 4)) return launch_rows<NT, GP, ZERO, 8>(p, pair, s);
+  if (p.steps >= 4) return launch_rows<NT, GP, ZERO, 4>(p, pair, s);
+  return launch_rows<NT, GP, ZERO, 1>(p, pair, s);
 }
 template <int NT>
-static int pick_group(const Int4Rows& p, int group, bool zero, bool pair, int E, int tiles, cudaStream_t s) {
-  if (group == 128) return zero ? pick_pair<NT, 1, true>(p, pair, E, tiles, s) : pick_pair<NT, 1, false>(p, pair, E, tiles, s);
-  if (group == 64) return zero ? pick_pair<NT, 2, true>(p, pair, E, tiles, s) : pick_pair<NT, 2, false>(p, pair, E, tiles, s);
-  return zero ? pick_pair<NT, 4, true>(p, pair, E, tiles, s) : pick_pair<NT, 4, false>(p, pair, E, tiles, s);
+static int pick_group(const Int4Rows& p, int group, bool zero, bool pair, cudaStream_t s) {
+  if (group == 128) return zero ? pick_team<NT, 1, true>(p, pair, s) : pick_team<NT, 1, false>(p, pair, s);
+  if (group == 64) return zero ? pick_team<NT, 2, true>(p, pair, s) : pick_team<NT, 2, false>(p, pair, s);
+  return zero ? pick_team<NT, 4, true>(p, pair, s) : pick_team<NT, 4, false>(p, pair, s);
 }
 
 }  // namespace skein
 
 // x [x_rows, x_ld] bf16 (row r of the product reads row src_row[r], or r); w as in int4.cuh; out and residual [rows, out_ld] bf16
-// or fp32. counts / offsets null: one matrix for all rows. tiles: tiles of rows that an expert's CTAs are dealt over (each walks its share).
-// flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
-extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld, const int* counts, const int* offsets, int rows, int x_rows,
-                               int E, int F, int K, int group, int rows_hint, int flags, int* status, void* stream) {
+// or fp32. counts / offsets null: one matrix for all rows. rows_hint: rows expected of an expert. flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
+// Returns -1 for what it does not take (more than IR_MAX_E experts, or a row of x past the shared memory: K of 94,000).
+extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld,
+                               const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int rows_hint, int flags,
+                               int* status, void* stream) {
   using namespace skein;
   if (rows == 0) return 0;
-  if (rows < 0 || E < 1 || E > 65535 || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
+  if (rows < 0 || E < 1 || E > IR_MAX_E || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
   Int4Rows p;
-  p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts; p.offsets = offsets; p.status = status;
-  p.x_ld = x_ld; p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.F = F; p.K = K;
+  p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts;
+  p.offsets = offsets; p.status = status; p.x_ld = x_ld; p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.E = E; p.F = F; p.K = K;
   const bool pair = flags & 1;
   p.strips = pair ? (F + 7) / 8 : (F + 15) / 16;
   p.steps = (K + I4_STEP - 1) / I4_STEP;
   p.scale_half = (flags >> 1) & 1; p.out_f32 = (flags >> 2) & 1;
   p.vec = x_ld % 8 == 0 && (uintptr_t)x % 16 == 0;
-  const int per = rows_hint < 1 ? 1 : rows_hint;
-  const int nt = per <= 8 ? 1 : 2;
-  int tiles = (per + 8 * nt - 1) / (8 * nt);
-  if (tiles > 65535) tiles = 65535;
   cudaStream_t s = (cudaStream_t)stream;
-  return nt == 1 ? pick_group<1>(p, group, flags & 8, pair, E, tiles, s) : pick_group<2>(p, group, flags & 8, pair, E, tiles, s);
+  return rows_hint > 8 ? pick_group<2>(p, group, flags & 8, pair, s) : pick_group<1>(p, group, flags & 8, pair, s);
 }

@@ -43,9 +43,11 @@ __device__ __forceinline__ void it_gather4(uint32_t dst, const void* tmap, uint3
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 
-// The same answer for every lane, so that a warp leaves a role together.
+// One lane polls (32 that do keep the shared-memory pipe busy), every lane gets its answer, so that a warp leaves a role together.
 __device__ __forceinline__ bool it_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, budget_ns));
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, budget_ns);
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
 // shape of a launch

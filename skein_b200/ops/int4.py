@@ -16,7 +16,7 @@ from . import _lib, functional as F, reference_int4 as ri
 GROUPS = (32, 64, 128)
 STEP = 128                 # elements of K of a packed block (16 rows)
 CODES = 16 * STEP // 2     # its bytes of codes
-MAX_EXPERTS = 65535
+MAX_EXPERTS = 1024
 
 
 class Int4Weight:

@@ -31,26 +31,27 @@ __host__ __device__ constexpr int i4_record(int gp, bool zero) { return 8 * (I4_
 constexpr int I4_SCALES = 8 * I4_CODES;            // where its scales begin
 __host__ __device__ constexpr int i4_zeros(int gp) { return I4_SCALES + 8 * 32 * gp; }
 
-// code pair -> bf16 pair 128 + code: the codes are the low mantissa bits of a bf16 whose unit in the last place is 1
-__device__ __forceinline__ uint32_t i4_magic(uint32_t word, int i) {
+// Codes as bf16 pairs (code - zero) / 64. A 16-bit pattern P below 256 is the bf16 number P 2^-133 (subnormals, and the first exponent whose steps are
+// as wide), so a masked code needs no exponent of its own: one multiply-add by 2^127 (2^123 for a code four bits up) and -zero / 64 gives the
+// difference, a whole number below 16 over 64, exactly. Nine instructions per word of eight codes: a shift, four masks, four multiply-adds.
+// Spelled out so that no fast-math flag flushes the subnormal operands.
+__device__ __forceinline__ uint32_t i4_fma(uint32_t v, uint32_t m, uint32_t a) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(word >> (4 * i)));
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(m), "r"(a));
   return r;
 }
-// (128 + code) - (128 + zero): both are whole numbers below 256, so the difference is exact in bf16
-__device__ __forceinline__ uint32_t i4_sub(uint32_t v, uint32_t base) {
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(base));
-  return r;
+constexpr uint32_t I4_EIGHT = 0xbe00be00u;      // -8 / 64
+__device__ __forceinline__ uint32_t i4_zero(uint32_t zero) { return i4_fma(zero | (zero << 16), 0xff00ff00u, 0x80008000u); }   // -zero / 64
+__device__ __forceinline__ void i4_expand(uint32_t word, uint32_t zero, uint32_t* r) {
+  const uint32_t up = word >> 8;
+  r[0] = i4_fma(word & 0x000f000fu, 0x7f007f00u, zero);
+  r[1] = i4_fma(word & 0x00f000f0u, 0x7d007d00u, zero);
+  r[2] = i4_fma(up & 0x000f000fu, 0x7f007f00u, zero);
+  r[3] = i4_fma(up & 0x00f000f0u, 0x7d007d00u, zero);
 }
-__device__ __forceinline__ void i4_expand(uint32_t word, uint32_t base, uint32_t (&r)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = i4_sub(i4_magic(word, i), base);
-}
-// a zero as the pair that i4_sub takes
-__device__ __forceinline__ uint32_t i4_base(uint32_t zero) { return 0x43004300u | zero | (zero << 16); }
+// a scale times the 64 of its codes
 __device__ __forceinline__ float i4_scale(uint32_t raw, bool half) {
-  return half ? __half2float(__ushort_as_half((unsigned short)raw)) : __uint_as_float(raw << 16);
+  return 64.f * (half ? __half2float(__ushort_as_half((unsigned short)raw)) : __uint_as_float(raw << 16));
 }
 
 }  // namespace skein

@@ -3,7 +3,7 @@
 //   y[r, f] = sum over groups j of scale[f, j] * ( sum_{k in j} x[r, k] (code[f, k] - zero[f, j]) )
 //
 // With a few rows the weights' bytes bound the time, and what has to be done for each of them besides. A warp reads a step of a strip (16 rows x 128 of
-// K) with two 16-byte loads per lane, turns the codes into bf16 whole numbers (exact, 11 instructions per word of eight) and multiplies them
+// K) with two 16-byte loads per lane, turns the codes into bf16 (exact, nine instructions per word of eight) and multiplies them
 // with mma.sync m16n8k16 against eight rows of x in shared memory. A group's sum is fp32 and is scaled in fp32, so nothing is rounded before the result.
 // A CTA per SM stays for the launch. WK of its 16 warps make a team that shares the K of a strip (a warp every WK-th step) and walks its run of strips;
 // the loads of the next four steps, the next strip's among them, are always on their way, and the team's sums meet in shared memory in warp order while
@@ -27,6 +27,7 @@ struct Int4Rows {
   const int *counts, *offsets;
   int* status;
   long long x_ld, out_ld;
+  uint64_t budget_ns;
   int rows, x_rows, E, F, K, strips, steps, scale_half, out_f32, vec, x_stage;   // x_stage: rows of a tile (8 NT, or as many as fit a team's shared memory)
 };
 
@@ -57,21 +58,17 @@ template <int GP, bool ZERO>
 struct Int4Step {       // a lane's part of a step of one strip
   uint4 c[2];
   uint32_t s[GP];       // scales of rows g and g + 8
-  uint16_t z[GP];
-  __device__ __forceinline__ void load(const uint8_t* rec, int strip, int lane) {
-    const int g = lane >> 2;
-    const uint8_t* at = rec + strip * I4_CODES + ((lane & 3) * 8 + g) * 16;
-    c[0] = __ldcs(reinterpret_cast<const uint4*>(at));
-    c[1] = __ldcs(reinterpret_cast<const uint4*>(at + 512));
-    const uint32_t* sp = reinterpret_cast<const uint32_t*>(rec + I4_SCALES) + (strip * 8 + g) * GP;
-    if constexpr (GP == 1) s[0] = __ldg(sp);
-    if constexpr (GP == 2) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(sp)); s[0] = v.x; s[1] = v.y; }
-    if constexpr (GP == 4) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(sp)); s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w; }
+  uint16_t z[ZERO ? GP : 1];
+  __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* scales, const uint8_t* zeros) {
+    c[0] = __ldcs(reinterpret_cast<const uint4*>(codes));
+    c[1] = __ldcs(reinterpret_cast<const uint4*>(codes + 512));
+    if constexpr (GP == 1) s[0] = __ldcs(reinterpret_cast<const uint32_t*>(scales));
+    if constexpr (GP == 2) { const uint2 v = __ldcs(reinterpret_cast<const uint2*>(scales)); s[0] = v.x; s[1] = v.y; }
+    if constexpr (GP == 4) { const uint4 v = __ldcs(reinterpret_cast<const uint4*>(scales)); s[0] = v.x; s[1] = v.y; s[2] = v.z; s[3] = v.w; }
     if constexpr (ZERO) {
-      const uint16_t* zp = reinterpret_cast<const uint16_t*>(rec + i4_zeros(GP)) + (strip * 8 + g) * GP;
-      if constexpr (GP == 1) z[0] = __ldg(zp);
-      if constexpr (GP == 2) { const ushort2 v = __ldg(reinterpret_cast<const ushort2*>(zp)); z[0] = v.x; z[1] = v.y; }
-      if constexpr (GP == 4) { const ushort4 v = __ldg(reinterpret_cast<const ushort4*>(zp)); z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w; }
+      if constexpr (GP == 1) z[0] = __ldcs(reinterpret_cast<const uint16_t*>(zeros));
+      if constexpr (GP == 2) { const ushort2 v = __ldcs(reinterpret_cast<const ushort2*>(zeros)); z[0] = v.x; z[1] = v.y; }
+      if constexpr (GP == 4) { const ushort4 v = __ldcs(reinterpret_cast<const ushort4*>(zeros)); z[0] = v.x; z[1] = v.y; z[2] = v.z; z[3] = v.w; }
     }
   }
 };
@@ -83,7 +80,14 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
   __shared__ float4 sums[2][IR_WARPS][NT][32];
   __shared__ int pre[IR_MAX_E + 1], cnt[IR_MAX_E];      // row tiles before an expert, its rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  __shared__ __align__(8) uint64_t bar[TEAMS];          // a team's sums of a strip are parked
+  __shared__ int abort_flag;
   const int team = warp / WK, part = warp % WK;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < TEAMS; ++i) mbar_init(smem_u32(&bar[i]), WK);
+    fence_mbar_init();
+  }
   pdl_trigger();
   pdl_wait();
   if (warp == 0) {
@@ -115,26 +119,30 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
   const int u0 = (int)((long long)pre[p.E] * p.strips * who / teams), u1 = (int)((long long)pre[p.E] * p.strips * (who + 1) / teams);
   const int mine = (p.steps - part + WK - 1) / WK;       // steps of a strip that this warp takes (at least one: WK <= steps)
   // cursor of the loads, ahead of the products
-  int le = 0, lstrip = 0, li = 0;
-  int lleft = u1 - u0, ltile = 0;
-  if (lleft > 0) {
-    ltile = u0 / p.strips;
-    lstrip = u0 - ltile * p.strips;
-    while (ltile >= pre[le + 1]) ++le;
-  }
   const size_t matrix = (size_t)((p.strips + 7) / 8) * p.steps * REC;
+  int le = 0, lleft = u1 - u0, ltile = u0 / p.strips, lstrip = u0 - ltile * p.strips, li = 0;
+  const uint8_t *lc = nullptr, *ls = nullptr, *lz = nullptr;
+  auto seek = [&]() {
+    while (ltile >= pre[le + 1]) ++le;
+    const uint8_t* at = p.w + le * matrix + ((size_t)(lstrip >> 3) * p.steps + part) * REC;
+    const int row = (lstrip & 7) * 8 + g;
+    lc = at + (lstrip & 7) * I4_CODES + (t * 8 + g) * 16;
+    ls = at + I4_SCALES + row * GP * 4;
+    if constexpr (ZERO) lz = at + i4_zeros(GP) + row * GP * 2;
+  };
+  if (lleft > 0) seek();
   Int4Step<GP, ZERO> buf[IR_DEPTH];
   auto load = [&](Int4Step<GP, ZERO>& b) {
     if (lleft <= 0) return;
-    b.load(p.w + le * matrix + ((size_t)(lstrip >> 3) * p.steps + part + li * WK) * REC, lstrip & 7, lane);
-    if (++li == mine) {
+    b.load(lc, ls, lz);
+    if (++li < mine) {
+      lc += WK * REC;
+      ls += WK * REC;
+      if constexpr (ZERO) lz += WK * REC;
+    } else {
       li = 0;
-      --lleft;
-      if (++lstrip == p.strips) {
-        lstrip = 0;
-        ++ltile;
-        while (le + 1 < p.E && ltile >= pre[le + 1]) ++le;
-      }
+      if (++lstrip == p.strips) { lstrip = 0; ++ltile; }
+      if (--lleft > 0) seek();
     }
   };
 #pragma unroll
@@ -142,10 +150,41 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
 
   const int x_row = ir_x_row(p.steps);
   uint8_t* x_team = x_smem + (size_t)team * p.x_stage * x_row;
-  int e = 0, i = 0, n_done = 0, valid = 0, row0 = 0;
+  int e = 0, i = 0, n_done = 0, valid = 0, row0 = 0, old_valid = 0, old_row0 = 0, old_strip = 0;
   int left = u1 - u0, tile = u0 / p.strips, staged = -1, strip = u0 - tile * p.strips;
   const uint8_t* xb[NT];
   float acc[NT][4];
+  // adds up the team's sums of the strip before (its turn goes round the warps) and stores them
+  auto finish = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if ((n_done - 1 + n) % WK != part) continue;
+      float4 (*parked)[NT][32] = sums[(n_done - 1) & 1] + team * WK;
+      float4 v = parked[0][n][lane];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) {
+        const float4 o = parked[w][n][lane];
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      // v: (row g, x rows 2t and 2t + 1), (row g + 8, the same)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = n * 8 + 2 * t + j;
+        if (r >= old_valid) continue;
+        const float a = j ? v.y : v.x, b = j ? v.w : v.z;
+        const size_t to = (size_t)(old_row0 + r) * p.out_ld;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (pair && h) continue;
+          const int f = pair ? old_strip * 8 + g : old_strip * 16 + g + 8 * h;
+          if (f >= p.F) continue;
+          const float y = pair ? silu(a) * b : h ? b : a;
+          if (p.out_f32) ((float*)p.out)[to + f] = p.residual ? y + ((const float*)p.residual)[to + f] : y;
+          else ((__nv_bfloat16*)p.out)[to + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[to + f]) : y);
+        }
+      }
+    }
+  };
   while (left > 0) {
 #pragma unroll
     for (int d = 0; d < IR_DEPTH; ++d) {
@@ -155,12 +194,13 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
-        if (staged != tile) {      // the rows of x of this tile; the team is past its products with those before (its sums met)
+        if (staged != tile) {      // the rows of x of this tile
           while (tile >= pre[e + 1]) ++e;
           const int first = (tile - pre[e]) * p.x_stage, base = p.counts != nullptr ? p.offsets[e] : 0;
           valid = min(p.x_stage, cnt[e] - first);
           row0 = base + first;
           const int chunks = p.steps * (I4_STEP / 8);
+          if (staged >= 0) ir_team_sync<WK * 32>(team);      // every warp is past its products with the rows before
           for (int r = part; r < valid; r += WK) {
             const int from = p.src_row != nullptr ? p.src_row[row0 + r] : row0 + r;
             const bool ok = from >= 0 && from < p.x_rows;
@@ -170,14 +210,13 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
           }
           staged = tile;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) xb[n] = x_team + (size_t)min(n * 8 + g, valid - 1) * x_row + t * 16;
+          for (int n = 0; n < NT; ++n) xb[n] = x_team + (size_t)min(n * 8 + g, valid - 1) * x_row + t * 16 + part * I4_STEP * 2;
           ir_team_sync<WK * 32>(team);
         }
       }
-      const Int4Step<GP, ZERO> cur = buf[d];
-      load(buf[d]);
-      const int at = (part + i * WK) * I4_STEP * 2;
+      const int at = i * (WK * I4_STEP * 2);
       float part_sum[NT][4];
+      uint32_t lo[4], hi[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {             // 32 of K each
         const int grp = q * GP / 4;
@@ -186,10 +225,9 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int k = 0; k < 4; ++k) part_sum[n][k] = 0.f;
-        const uint4 c = cur.c[q >> 1];
-        uint32_t lo[4], hi[4];
-        i4_expand(q & 1 ? c.y : c.x, i4_base(ZERO ? cur.z[grp] & 0xff : 8), lo);
-        i4_expand(q & 1 ? c.w : c.z, i4_base(ZERO ? cur.z[grp] >> 8 : 8), hi);
+        const uint4 c = buf[d].c[q >> 1];
+        i4_expand(q & 1 ? c.y : c.x, ZERO ? i4_zero(buf[d].z[ZERO ? grp : 0] & 0xff) : I4_EIGHT, lo);
+        i4_expand(q & 1 ? c.w : c.z, ZERO ? i4_zero(buf[d].z[ZERO ? grp : 0] >> 8) : I4_EIGHT, hi);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4 b = *reinterpret_cast<const uint4*>(xb[n] + at + q * 64);
@@ -197,7 +235,7 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
           ir_mma(part_sum[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
         }
         if ((q + 1) * GP % 4 == 0) {
-          const float sl = i4_scale(cur.s[grp] & 0xffff, p.scale_half), sh = i4_scale(cur.s[grp] >> 16, p.scale_half);
+          const float sl = i4_scale(buf[d].s[grp] & 0xffff, p.scale_half), sh = i4_scale(buf[d].s[grp] >> 16, p.scale_half);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             acc[n][0] += sl * part_sum[n][0]; acc[n][1] += sl * part_sum[n][1];
@@ -205,44 +243,32 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
           }
         }
       }
+      load(buf[d]);
       if (++i < mine) continue;
-      // the strip's sums
+      // The strip is done: the sums of the one before are complete and added up, then this one's are parked in the other half. Whoever parks those of
+      // strip n + 2 has seen all warps arrive with n + 1, which they do after they have added up n.
       i = 0;
       --left;
-      float4 (*mine_sums)[NT][32] = sums[n_done & 1];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) mine_sums[warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-      ir_team_sync<WK * 32>(team);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if ((n_done + n) % WK != part) continue;       // the warps take turns
-        float4 v = mine_sums[team * WK][n][lane];
-#pragma unroll
-        for (int w = 1; w < WK; ++w) {
-          const float4 o = mine_sums[team * WK + w][n][lane];
-          v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-        }
-        // v: (row g, x rows 2t and 2t + 1), (row g + 8, the same)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int r = n * 8 + 2 * t + j;
-          if (r >= valid) continue;
-          const float a = j ? v.y : v.x, b = j ? v.w : v.z;
-          const size_t to = (size_t)(row0 + r) * p.out_ld;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (pair && h) continue;
-            const int f = pair ? strip * 8 + g : strip * 16 + g + 8 * h;
-            if (f >= p.F) continue;
-            const float y = pair ? silu(a) * b : h ? b : a;
-            if (p.out_f32) ((float*)p.out)[to + f] = p.residual ? y + ((const float*)p.residual)[to + f] : y;
-            else ((__nv_bfloat16*)p.out)[to + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[to + f]) : y);
-          }
-        }
+      if (n_done > 0) {
+        if (WK > 1 && !mbar_wait(smem_u32(&bar[team]), (n_done - 1) & 1, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
+        __syncwarp();
+        finish();
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sums[n_done & 1][warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+      __syncwarp();
+      if (WK > 1 && lane == 0) mbar_arrive(smem_u32(&bar[team]));
       ++n_done;
+      old_valid = valid;
+      old_row0 = row0;
+      old_strip = strip;
       if (++strip == p.strips) { strip = 0; ++tile; }
     }
+  }
+  if (n_done > 0) {
+    if (WK > 1 && !mbar_wait(smem_u32(&bar[team]), (n_done - 1) & 1, &abort_flag, p.budget_ns)) report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x);
+    __syncwarp();
+    finish();
   }
 }
 
@@ -287,6 +313,7 @@ extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row
   Int4Rows p;
   p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts;
   p.offsets = offsets; p.status = status; p.x_ld = x_ld; p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.E = E; p.F = F; p.K = K;
+  p.budget_ns = (uint64_t)gemm_wait_budget_ms() * 1000000ull;
   const bool pair = flags & 1;
   p.strips = pair ? (F + 7) / 8 : (F + 15) / 16;
   p.steps = (K + I4_STEP - 1) / I4_STEP;

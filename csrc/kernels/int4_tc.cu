@@ -4,7 +4,7 @@
 // share the tile). Roles, one pipeline:
 //   producer    one bulk copy per step (codes, scales and zeros of 128 rows x 128 of K are one run) and TMA tiles of x, or of the rows that
 //               src_row names (tile::gather4), into a ring of shared-memory stages
-//   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (whole numbers, exact), 64 of K a slot, written to tensor
+//   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (exact), 64 of K a slot, written to tensor
 //               memory as the A operand
 //   MMA         one thread; every group of K has an accumulator of its own (a ring of them)
 //   epilogue    takes a group's accumulator out of tensor memory, multiplies it by the row's scale and adds it to its registers, fp32
@@ -246,19 +246,17 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
           uint2 c[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t) c[t] = *reinterpret_cast<const uint2*>(at + in_stage + j * 512 + t * 128);
-          uint32_t base[2] = {i4_base(8), i4_base(8)};
+          uint32_t base[2] = {I4_EIGHT, I4_EIGHT};
           if (zeros) {
-            base[0] = i4_base(at[zero_at + (GP == 1 ? 0 : GP == 2 ? j : 2 * j) * 2]);
-            base[1] = GP == 4 ? i4_base(at[zero_at + (2 * j + 1) * 2]) : base[0];
+            base[0] = i4_zero(at[zero_at + (GP == 1 ? 0 : GP == 2 ? j : 2 * j) * 2]);
+            base[1] = GP == 4 ? i4_zero(at[zero_at + (2 * j + 1) * 2]) : base[0];
           }
           uint32_t v[32];
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              v[t * 4 + i] = i4_sub(i4_magic(c[t].x, i), base[0]);
-              v[16 + t * 4 + i] = i4_sub(i4_magic(c[t].y, i), base[1]);
-            }
+          for (int t = 0; t < 4; ++t) {
+            i4_expand(c[t].x, base[0], v + t * 4);
+            i4_expand(c[t].y, base[1], v + 16 + t * 4);
+          }
           if (!it_warp_wait(smem_u32(&bar_cempty[slot]), sph ^ 1, &abort_flag, p.budget_ns)) {
             if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
             ok = false;

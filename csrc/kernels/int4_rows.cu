@@ -37,7 +37,7 @@ __host__ __device__ constexpr int ir_x_row(int steps) { return steps * I4_STEP *
 // eight neighbours of a row of x from k on, zero past its end
 __device__ __forceinline__ uint4 ir_load_x(const __nv_bfloat16* row, int k, int K, int vec) {
   uint4 v = make_uint4(0, 0, 0, 0);
-  if (row == nullptr || k >= K) return v;
+  if (k >= K) return v;
   if (vec) return __ldg(reinterpret_cast<const uint4*>(row + k));   // K is a multiple of 8
   const unsigned short* s = reinterpret_cast<const unsigned short*>(row + k);
   v.x = s[0] | (uint32_t)s[1] << 16; v.y = s[2] | (uint32_t)s[3] << 16;
@@ -201,12 +201,24 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
           row0 = base + first;
           const int chunks = p.steps * (I4_STEP / 8);
           if (staged >= 0) ir_team_sync<WK * 32>(team);      // every warp is past its products with the rows before
-          for (int r = part; r < valid; r += WK) {
-            const int from = p.src_row != nullptr ? p.src_row[row0 + r] : row0 + r;
-            const bool ok = from >= 0 && from < p.x_rows;
-            if (!ok && lane == 0) report_status(p.status, ST_BAD_INDEX, from);
-            const __nv_bfloat16* row = ok ? p.x + (size_t)from * p.x_ld : nullptr;
-            for (int c = lane; c < chunks; c += 32) *reinterpret_cast<uint4*>(x_team + (size_t)r * x_row + c * 16) = ir_load_x(row, c * 8, p.K, p.vec);
+          // all threads of the team over the rows' 16-byte pieces, four loads at a time
+          for (int i0 = part * 32 + lane; i0 < valid * chunks; i0 += 4 * WK * 32) {
+            uint4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = i0 + k * WK * 32, r = at / chunks, c = at - r * chunks;
+              v[k] = make_uint4(0, 0, 0, 0);
+              if (r < valid) {
+                const int from = p.src_row != nullptr ? p.src_row[row0 + r] : row0 + r;
+                if (from >= 0 && from < p.x_rows) v[k] = ir_load_x(p.x + (size_t)from * p.x_ld, c * 8, p.K, p.vec);
+                else if (c == 0) report_status(p.status, ST_BAD_INDEX, from);
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = i0 + k * WK * 32, r = at / chunks, c = at - r * chunks;
+              if (r < valid) *reinterpret_cast<uint4*>(x_team + (size_t)r * x_row + c * 16) = v[k];
+            }
           }
           staged = tile;
 #pragma unroll

@@ -28,7 +28,7 @@ struct Int4Rows {
   int* status;
   long long x_ld, out_ld;
   uint64_t budget_ns;
-  int rows, x_rows, E, F, K, strips, steps, scale_half, out_f32, vec, x_stage;   // x_stage: rows of a tile (8 NT, or as many as fit a team's shared memory)
+  int rows, x_rows, E, F, K, tiles, strips, steps, out_f32, vec, pair, x_stage;   // x_stage: rows of a tile (8 NT, or as many as fit a team's shared memory)
 };
 
 // bytes of a row of x in shared memory: 64 past a multiple of 128, so that eight rows x 64 bytes lie in different banks
@@ -48,6 +48,11 @@ template <int THREADS>
 __device__ __forceinline__ void ir_team_sync(int team) {
   if constexpr (THREADS == 32) __syncwarp();
   else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(THREADS) : "memory");
+}
+// the first product of a group: no sum to add to
+__device__ __forceinline__ void ir_mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void ir_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -73,8 +78,8 @@ struct Int4Step {       // a lane's part of a step of one strip
   }
 };
 
-template <int NT, int GP, bool ZERO, int WK>
-__global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows p, const bool pair) {
+template <int NT, int GP, bool ZERO, bool HALF, int WK>
+__global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_constant__ Int4Rows p) {
   constexpr int TEAMS = IR_WARPS / WK, REC = i4_record(GP, ZERO);
   extern __shared__ __align__(16) uint8_t x_smem[];
   __shared__ float4 sums[2][IR_WARPS][NT][32];
@@ -171,14 +176,14 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
       for (int j = 0; j < 2; ++j) {
         const int r = n * 8 + 2 * t + j;
         if (r >= old_valid) continue;
-        const float a = j ? v.y : v.x, b = j ? v.w : v.z;
+        const float a = 64.f * (j ? v.y : v.x), b = 64.f * (j ? v.w : v.z);       // (the codes were 64ths)
         const size_t to = (size_t)(old_row0 + r) * p.out_ld;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (pair && h) continue;
-          const int f = pair ? old_strip * 8 + g : old_strip * 16 + g + 8 * h;
+          if (p.pair && h) continue;
+          const int f = p.pair ? old_strip * 8 + g : old_strip * 16 + g + 8 * h;
           if (f >= p.F) continue;
-          const float y = pair ? silu(a) * b : h ? b : a;
+          const float y = p.pair ? silu(a) * b : h ? b : a;
           if (p.out_f32) ((float*)p.out)[to + f] = p.residual ? y + ((const float*)p.residual)[to + f] : y;
           else ((__nv_bfloat16*)p.out)[to + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[to + f]) : y);
         }
@@ -227,27 +232,26 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
         }
       }
       const int at = i * (WK * I4_STEP * 2);
+      constexpr int per = 4 / GP;               // quarters of a step in a group
       float part_sum[NT][4];
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {             // 32 of K each
-        const int grp = q * GP / 4;
-        if (q * GP % 4 == 0)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) part_sum[n][k] = 0.f;
+        const int grp = q / per;
         const uint4 c = buf[d].c[q >> 1];
         i4_expand(q & 1 ? c.y : c.x, ZERO ? i4_zero(buf[d].z[ZERO ? grp : 0] & 0xff) : I4_EIGHT, lo);
         i4_expand(q & 1 ? c.w : c.z, ZERO ? i4_zero(buf[d].z[ZERO ? grp : 0] >> 8) : I4_EIGHT, hi);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4 b = *reinterpret_cast<const uint4*>(xb[n] + at + q * 64);
-          ir_mma(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+          if (q % per == 0) ir_mma0(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+          else ir_mma(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
           ir_mma(part_sum[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
         }
-        if ((q + 1) * GP % 4 == 0) {
-          const float sl = i4_scale(buf[d].s[grp] & 0xffff, p.scale_half), sh = i4_scale(buf[d].s[grp] >> 16, p.scale_half);
+        if (q % per == per - 1) {
+          float sl, sh;
+          if constexpr (HALF) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&buf[d].s[grp])); sl = f.x; sh = f.y; }
+          else { sl = __uint_as_float(buf[d].s[grp] << 16); sh = __uint_as_float(buf[d].s[grp] & 0xffff0000u); }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             acc[n][0] += sl * part_sum[n][0]; acc[n][1] += sl * part_sum[n][1];
@@ -284,40 +288,48 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const Int4Rows
   }
 }
 
-template <int NT, int GP, bool ZERO, int WK>
-static int launch_rows(Int4Rows p, bool pair, cudaStream_t s) {
+template <int NT, int GP, bool ZERO, bool HALF, int WK>
+static int launch_rows(Int4Rows p, cudaStream_t s) {
   static PerDevice allowed;
-  const int fit = IR_SMEM / (IR_WARPS / WK) / ir_x_row(p.steps);
-  p.x_stage = min(min(8 * NT, p.rows), fit);
+  constexpr int TEAMS = IR_WARPS / WK;
+  p.x_stage = min(8 * NT, p.rows);
+  while (p.x_stage > 0 && TEAMS * (p.x_stage * ir_x_row(p.steps)) > IR_SMEM) --p.x_stage;
   if (p.x_stage < 1 || ((long long)p.rows / p.x_stage + min(p.E, p.rows)) * p.strips > 0x7fffffffll) return -1;
-  const size_t smem = (size_t)(IR_WARPS / WK) * p.x_stage * ir_x_row(p.steps);
-  const cudaError_t e = allow_smem(allowed, (const void*)int4_rows_kernel<NT, GP, ZERO, WK>, IR_SMEM);
+  const cudaError_t e = allow_smem(allowed, (const void*)int4_rows_kernel<NT, GP, ZERO, HALF, WK>, IR_SMEM);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(int4_rows_kernel<NT, GP, ZERO, WK>, dim3(148), dim3(IR_THREADS), smem, s, p, pair);
+  return (int)launch_pdl(int4_rows_kernel<NT, GP, ZERO, HALF, WK>, dim3(148), dim3(IR_THREADS), (size_t)TEAMS * (p.x_stage * ir_x_row(p.steps)), s, p);
 }
 // warps of a team: as many as leave each three steps or more of a strip, and more where its rows of x do not fit a smaller team's shared memory
-template <int NT, int GP, bool ZERO>
-static int pick_team(const Int4Rows& p, bool pair, cudaStream_t s) {
+template <int NT, int GP, bool ZERO, bool HALF>
+static int pick_team(const Int4Rows& p, int team, cudaStream_t s) {
   const int x = min(8 * NT, p.rows) * ir_x_row(p.steps);
-  if (p.steps >= 48 || (p.steps >= 16 && x > IR_SMEM / 2)) return launch_rows<NT, GP, ZERO, 16>(p, pair, s);
-  if (p.steps >= 24 || (p.steps >= 8 && x > IR_SMEM / 4)) return launch_rows<NT, GP, ZERO, 8>(p, pair, s);
-  if (p.steps >= 4) return launch_rows<NT, GP, ZERO, 4>(p, pair, s);
-  return launch_rows<NT, GP, ZERO, 1>(p, pair, s);
+  if (team == 0) team = p.steps >= 48 || (p.steps >= 16 && x > IR_SMEM / 2) ? 16 : p.steps >= 24 || (p.steps >= 8 && x > IR_SMEM / 4) ? 8 : p.steps >= 4 ? 4 : 1;
+  if (team > p.steps) return -1;
+  switch (team) {
+    case 16: return launch_rows<NT, GP, ZERO, HALF, 16>(p, s);
+    case 8: return launch_rows<NT, GP, ZERO, HALF, 8>(p, s);
+    case 4: return launch_rows<NT, GP, ZERO, HALF, 4>(p, s);
+    case 1: return launch_rows<NT, GP, ZERO, HALF, 1>(p, s);
+    default: return -1;
+  }
+}
+template <int NT, int GP>
+static int pick_form(const Int4Rows& p, bool zero, bool half, int team, cudaStream_t s) {
+  if (zero) return half ? pick_team<NT, GP, true, true>(p, team, s) : pick_team<NT, GP, true, false>(p, team, s);
+  return half ? pick_team<NT, GP, false, true>(p, team, s) : pick_team<NT, GP, false, false>(p, team, s);
 }
 template <int NT>
-static int pick_group(const Int4Rows& p, int group, bool zero, bool pair, cudaStream_t s) {
-  if (group == 128) return zero ? pick_team<NT, 1, true>(p, pair, s) : pick_team<NT, 1, false>(p, pair, s);
-  if (group == 64) return zero ? pick_team<NT, 2, true>(p, pair, s) : pick_team<NT, 2, false>(p, pair, s);
-  return zero ? pick_team<NT, 4, true>(p, pair, s) : pick_team<NT, 4, false>(p, pair, s);
+static int pick_group(const Int4Rows& p, int group, bool zero, bool half, int team, cudaStream_t s) {
+  return group == 128 ? pick_form<NT, 1>(p, zero, half, team, s) : group == 64 ? pick_form<NT, 2>(p, zero, half, team, s) : pick_form<NT, 4>(p, zero, half, team, s);
 }
 
 }  // namespace skein
 
 // x [x_rows, x_ld] bf16 (row r of the product reads row src_row[r], or r); w as in int4.cuh; out and residual [rows, out_ld] bf16
 // or fp32. counts / offsets null: one matrix for all rows. rows_hint: rows expected of an expert. flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
-// Returns -1 for what it does not take (more than IR_MAX_E experts, or a row of x past the shared memory: K of 94,000).
+// team: warps that share a strip (1, 4, 8 or 16, at most its steps), 0: by the rule above. Returns -1 for what it does not take (more than IR_MAX_E experts, or a row of x past the shared memory: K of 94,000).
 extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld,
-                               const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int rows_hint, int flags,
+                               const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int rows_hint, int flags, int team,
                                int* status, void* stream) {
   using namespace skein;
   if (rows == 0) return 0;
@@ -326,11 +338,12 @@ extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row
   p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts;
   p.offsets = offsets; p.status = status; p.x_ld = x_ld; p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.E = E; p.F = F; p.K = K;
   p.budget_ns = (uint64_t)gemm_wait_budget_ms() * 1000000ull;
-  const bool pair = flags & 1;
-  p.strips = pair ? (F + 7) / 8 : (F + 15) / 16;
+  p.pair = flags & 1;
+  p.strips = p.pair ? (F + 7) / 8 : (F + 15) / 16;
+  p.tiles = (p.strips + 7) / 8;
   p.steps = (K + I4_STEP - 1) / I4_STEP;
-  p.scale_half = (flags >> 1) & 1; p.out_f32 = (flags >> 2) & 1;
+  p.out_f32 = (flags >> 2) & 1;
   p.vec = x_ld % 8 == 0 && (uintptr_t)x % 16 == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  return rows_hint > 8 ? pick_group<2>(p, group, flags & 8, pair, s) : pick_group<1>(p, group, flags & 8, pair, s);
+  return rows_hint > 8 ? pick_group<2>(p, group, flags & 8, flags & 2, team, s) : pick_group<1>(p, group, flags & 8, flags & 2, team, s);
 }

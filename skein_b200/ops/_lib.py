@@ -232,7 +232,7 @@ def lib():
     _sig(L, "skein_route_balanced",
          i32, [vp, i64, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, f32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp])
     _sig(L, "skein_int4_tc", i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp])
-    _sig(L, "skein_int4_rows", i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp])
+    _sig(L, "skein_int4_rows", i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp, vp])
     for name, rt, at in _OPTIONAL:
         if hasattr(L, name):
             _sig(L, name, rt, at)

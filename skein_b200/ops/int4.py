@@ -182,16 +182,16 @@ def _out(what, out, rows, w, dtype, device):
 
 
 def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags, cfg=None):
-    """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, n_tile 0 for the kernel of few rows."""
+    """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, (0, team) of the kernel of few rows."""
     L, data = _lib.lib(), w.data
     args = (x.data_ptr(), x.stride(0), _lib.ptr(src_row), data.data_ptr(), _lib.ptr(residual), out.data_ptr(), out.stride(0), _lib.ptr(counts),
             _lib.ptr(offsets), rows, x.shape[0], data.shape[0], w.features, w.shape[-1], w.group, hint, flags)
     status, stream = F.workspace(x.device).status.data_ptr(), _lib.stream_ptr()
     aligned = args[0] % 16 == 0 and args[1] % 8 == 0
-    if aligned and (hint > 8 if cfg is None else cfg[0] > 0):
+    if aligned and (hint > 16 if cfg is None else cfg[0] > 0):
         rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), status, stream)
     else:
-        rc = L.skein_int4_rows(*args, status, stream)
+        rc = L.skein_int4_rows(*args, cfg[1] if cfg else 0, status, stream)
     _lib.check(rc, what)
     _lib.count_launch()
 

@@ -43,25 +43,57 @@ __device__ __forceinline__ void it_gather4(uint32_t dst, const void* tmap, uint3
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 
-// One lane polls (32 that do keep the shared-memory pipe busy), every lane gets its answer, so that a warp leaves a role together.
+// Wait of a whole warp: the same answer for every lane, so that a warp leaves a role together. Bounded by budget_ns.
 __device__ __forceinline__ bool it_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, budget_ns);
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+  uint64_t t0 = 0;
+#pragma unroll 1
+  for (uint32_t n = 1;; ++n) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((n & 255) == 0) {
+      if (t0 == 0) t0 = global_timer_ns();
+      if (__any_sync(0xffffffffu, *abort_flag || global_timer_ns() - t0 > budget_ns)) return false;
+    }
+  }
+}
+// The same of one thread.
+__device__ __forceinline__ bool it_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
+  uint64_t t0 = 0;
+#pragma unroll 1
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 255) == 0) {
+      if (t0 == 0) t0 = global_timer_ns();
+      if (*abort_flag || global_timer_ns() - t0 > budget_ns) return false;
+    }
+  }
+}
+// a += b * s on two neighbours at a time
+__device__ __forceinline__ void it_fma2(uint64_t& a, uint32_t b0, uint32_t b1, uint64_t s) {
+  asm("{\n\t.reg .b64 b;\n\tmov.b64 b, {%1, %2};\n\tfma.rn.f32x2 %0, b, %3, %0;\n\t}" : "+l"(a) : "r"(b0), "r"(b1), "l"(s));
+}
+__device__ __forceinline__ uint64_t it_pack(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 it_unpack(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
 }
 
 // shape of a launch
 template <int NT>
 struct ItShape {
   static constexpr bool WIDE = NT == 128;                  // one CTA per SM, 512 columns; else two with 256 each
-  static constexpr int CONV_WARPS = WIDE ? 8 : 4, EPI_WARPS = WIDE ? 8 : 4;
+  static constexpr int CONV_WARPS = WIDE ? 8 : 4, EPI_WARPS = NT >= 64 ? 8 : 4;
   static constexpr int THREADS = 32 * (4 + CONV_WARPS + EPI_WARPS);       // warps 0 and 1 produce and issue, 2 and 3 only align the quadrants
   static constexpr int ACC = NT < 32 ? 32 : NT;            // columns of an accumulator
   static constexpr int BUFS = NT <= 32 ? 4 : 2;
-  static constexpr int SLOTS = WIDE ? 8 : 4;               // 32 columns each
+  static constexpr int SLOTS = WIDE ? 4 : 2;               // of a converted step, 64 columns each
   static constexpr int COLS = WIDE ? 512 : 256;
   static constexpr int EPI_COLS = NT / (EPI_WARPS / 4);    // columns of an epilogue warp
-  static_assert(BUFS * ACC + SLOTS * 32 <= COLS, "tensor memory");
+  static_assert(BUFS * ACC + SLOTS * 64 <= COLS, "tensor memory");
 };
 
 template <int NT, int GP>
@@ -146,7 +178,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   const bool live = e >= 0;            // the same for every CTA of a cluster
   const int m = unit[1], row0 = unit[2], valid = unit[3];
   const int s0 = (int)((long long)p.steps * rank / p.split), s1 = (int)((long long)p.steps * (rank + 1) / p.split);
-  float acc[S::EPI_COLS];
+  uint64_t acc[S::EPI_COLS / 2];       // two columns each
 
   if (live) {
     const uint8_t* w = p.w + ((size_t)e * p.m_tiles + m) * p.steps * rec;
@@ -187,62 +219,59 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       if (elect_one()) {
         const uint32_t idesc = umma_idesc(1, 1, 128, NT);
         int st = 0, slot = 0, buf = 0;
-        uint32_t ph = 0, sph = 0, bph = 0;
+        uint32_t sph = 0, bph = 0;
         bool ok = true;
-        for (int s = s0; s < s1 && ok; ++s) {
-          if (!mbar_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; break; }
+        for (int s = s0; s < s1; ++s) {
+          // (the converters have seen the stage arrive, x included)
+          if (!it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; break; }
           const uint32_t at = smem_base + st * stage_bytes;
+          const uint64_t dx0 = umma_desc_sw128(at), dx1 = umma_desc_sw128(at + NT * 128);
+          const uint32_t a_tmem = tmem_base + S::BUFS * S::ACC + slot * 64;
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (!ok) break;
-            if (!mbar_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); ok = false; break; }
-            const uint64_t dx = umma_desc_sw128(at + j * NT * 128);
-            const uint32_t a_tmem = tmem_base + S::BUFS * S::ACC + slot * 32;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              constexpr int PER = 8 / GP;              // MMAs of a group
-              const int in = (j * 4 + k) % PER;
-              if (in == 0 && !mbar_wait(smem_u32(&bar_dempty[buf]), bph ^ 1, &abort_flag, p.budget_ns)) {
-                report_status(p.status, ST_TIMEOUT_TMEM_EMPTY, blockIdx.x);
-                ok = false;
-                break;
-              }
-              if (in == 0 || k == 0) tc_fence_after();
-              mma_f16_ts(tmem_base + buf * S::ACC, a_tmem + 8 * k, dx + 2 * k, idesc, in > 0 ? 1u : 0u);
-              if (in == PER - 1) {
-                tc_commit(smem_u32(&bar_dfull[buf]));
-                if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
-              }
+          for (int g = 0; g < GP; ++g) {
+            if (!it_wait(smem_u32(&bar_dempty[buf]), bph ^ 1, &abort_flag, p.budget_ns)) {
+              report_status(p.status, ST_TIMEOUT_TMEM_EMPTY, blockIdx.x);
+              ok = false;
+              break;
             }
-            if (!ok) break;
-            tc_commit(smem_u32(&bar_cempty[slot]));
-            if (++slot == S::SLOTS) { slot = 0; sph ^= 1; }
+            tc_fence_after();
+            constexpr int PER = 8 / GP;              // MMAs of a group
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              const int k = g * PER + i;
+              mma_f16_ts(tmem_base + buf * S::ACC, a_tmem + 8 * k, (k < 4 ? dx0 : dx1) + 2 * (k & 3), idesc, i > 0 ? 1u : 0u);
+            }
+            tc_commit(smem_u32(&bar_dfull[buf]));
+            if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
           }
           if (!ok) { abort_flag = 1; break; }
+          tc_commit(smem_u32(&bar_cempty[slot]));
           tc_commit(smem_u32(&bar_empty[st]));
-          if (++st == p.stages) { st = 0; ph ^= 1; }
+          if (++slot == S::SLOTS) { slot = 0; sph ^= 1; }
+          if (++st == p.stages) st = 0;
         }
       }
       __syncwarp();
     } else if (warp >= 4 && warp < 4 + S::CONV_WARPS) {
-      // ================= converters: row r of the tile, half j of a step (both in turn with four warps) =================
-      const int r = (warp & 3) * 32 + lane, group = (warp - 4) >> 2;
+      // ================= converters: row r of the tile; with eight warps the two groups take the steps in turn =================
+      const int r = (warp & 3) * 32 + lane;
       constexpr int GROUPS = S::CONV_WARPS / 4;
+      const int group = (warp - 4) >> 2;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
       const int in_stage = X_BYTES + (r >> 4) * I4_CODES + (r & 7) * 16 + ((r >> 3) & 1) * 8;
       const int zero_at = X_BYTES + i4_zeros(GP) + ((r >> 4) * 8 + (r & 7)) * GP * 2 + ((r >> 3) & 1);
-      int st = 0, slot = group;
+      int st = group % p.stages, slot = group;
       uint32_t ph = 0, sph = 0;
-      bool ok = true;
-      for (int s = s0; s < s1 && ok; ++s) {
+      for (int s = s0 + group; s < s1; s += GROUPS) {
         if (!it_warp_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
           break;
         }
         const uint8_t* at = smem_raw + (smem_base - smem_u32(smem_raw)) + st * stage_bytes;
+        const uint32_t to = tmem_base + S::BUFS * S::ACC + slot * 64 + lane_tmem;
+        bool ok = true;
 #pragma unroll
-        for (int j0 = 0; j0 < 2; j0 += GROUPS) {
-          const int j = j0 + group;
+        for (int j = 0; j < 2; ++j) {
           uint2 c[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t) c[t] = *reinterpret_cast<const uint2*>(at + in_stage + j * 512 + t * 128);
@@ -257,23 +286,26 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             i4_expand(c[t].x, base[0], v + t * 4);
             i4_expand(c[t].y, base[1], v + 16 + t * 4);
           }
-          if (!it_warp_wait(smem_u32(&bar_cempty[slot]), sph ^ 1, &abort_flag, p.budget_ns)) {
-            if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
-            ok = false;
-            break;
+          if (j == 0) {
+            if (!it_warp_wait(smem_u32(&bar_cempty[slot]), sph ^ 1, &abort_flag, p.budget_ns)) {
+              if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
+              ok = false;
+              break;
+            }
+            tc_fence_after();
           }
-          tc_fence_after();
-          const uint32_t to = tmem_base + S::BUFS * S::ACC + slot * 32 + lane_tmem;
-          tmem_st16(to, v);
-          tmem_st16(to + 16, v + 16);
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bar_cfull[slot]));
-          slot += GROUPS;
-          if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
+          tmem_st16(to + j * 32, v);
+          tmem_st16(to + j * 32 + 16, v + 16);
         }
-        if (++st == p.stages) { st = 0; ph ^= 1; }
+        if (!ok) break;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_cfull[slot]));
+        slot += GROUPS;
+        if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
+        st += GROUPS;
+        if (st >= p.stages) { st -= p.stages; ph ^= 1; }
       }
     } else if (warp >= 4) {
       // ================= epilogue: row r, columns col0 .. + EPI_COLS =================
@@ -281,7 +313,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
       const int scale_at = X_BYTES + I4_SCALES + ((r >> 4) * 8 + (r & 7)) * GP * 4 + ((r >> 3) & 1) * 2;
 #pragma unroll
-      for (int c = 0; c < S::EPI_COLS; ++c) acc[c] = 0.f;
+      for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[c] = 0ull;
       int st = 0, buf = 0;
       uint32_t ph = 0, bph = 0;
       bool ok = true;
@@ -306,18 +338,21 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
           }
           tc_fence_after();
           const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem;
+          const uint64_t s2 = it_pack(sc[g], sc[g]);
+          constexpr int STEP = S::EPI_COLS < 32 ? 16 : 32;
 #pragma unroll
-          for (int c0 = 0; c0 < S::EPI_COLS; c0 += 16) {
-            uint32_t v[16];
+          for (int c0 = 0; c0 < S::EPI_COLS; c0 += STEP) {
+            uint32_t v[STEP];
             tmem_ld16(from + c0, v);
+            if constexpr (STEP == 32) tmem_ld16(from + c0 + 16, v + 16);
             tmem_ld_wait();
-            if (c0 + 16 == S::EPI_COLS) {
+            if (c0 + STEP == S::EPI_COLS) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(smem_u32(&bar_dempty[buf]));
             }
 #pragma unroll
-            for (int c = 0; c < 16; ++c) acc[c0 + c] += sc[g] * __uint_as_float(v[c]);
+            for (int c = 0; c < STEP; c += 2) it_fma2(acc[(c0 + c) / 2], v[c], v[c + 1], s2);
           }
           if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
         }
@@ -335,9 +370,11 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
     cluster.sync();
     if (epi) {
 #pragma unroll
-      for (int c = 0; c < S::EPI_COLS; ++c) {
-        const int owner = (col0 + c) / slice;
-        cluster.map_shared_rank(recv, owner)[(rank * slice + (col0 + c) % slice) * 128 + r] = acc[c];
+      for (int c = 0; c < S::EPI_COLS; c += 2) {       // (a slice is an even number of columns)
+        const float2 v = it_unpack(acc[c / 2]);
+        float* to = cluster.map_shared_rank(recv, (col0 + c) / slice) + (rank * slice + (col0 + c) % slice) * 128 + r;
+        to[0] = v.x;
+        to[128] = v.y;
       }
     }
     cluster.sync();
@@ -365,7 +402,8 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
     };
     if (p.split == 1) {
 #pragma unroll
-      for (int c = 0; c < S::EPI_COLS; c += 2) if (col0 + c < valid) finish(col0 + c, acc[c], acc[c + 1]);
+      for (int c = 0; c < S::EPI_COLS; c += 2)
+        if (col0 + c < valid) { const float2 v = it_unpack(acc[c / 2]); finish(col0 + c, v.x, v.y); }
     } else {
       for (int c = part * 2; c < slice; c += 2 * (S::EPI_WARPS / 4)) {
         if (rank * slice + c >= valid) break;

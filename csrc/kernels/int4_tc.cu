@@ -23,6 +23,7 @@ namespace skein {
 int make_tmap_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t k_elems, uint64_t ld, int elem_bytes, uint32_t box_rows);   // gemm_ws.cu
 
 constexpr int IT_MAX_STAGES = 8;
+constexpr int IT_SCALES = 8;             // steps of the ring of scales
 constexpr int IT_BAND = 12;              // feature tiles of a band in which the row tiles run (L2 keeps a band's weights)
 
 struct Int4Tc {
@@ -43,19 +44,7 @@ __device__ __forceinline__ void it_gather4(uint32_t dst, const void* tmap, uint3
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
 }
 
-// Wait of a whole warp: the same answer for every lane, so that a warp leaves a role together. Bounded by budget_ns.
-__device__ __forceinline__ bool it_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
-  uint64_t t0 = 0;
-#pragma unroll 1
-  for (uint32_t n = 1;; ++n) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    if ((n & 255) == 0) {
-      if (t0 == 0) t0 = global_timer_ns();
-      if (__any_sync(0xffffffffu, *abort_flag || global_timer_ns() - t0 > budget_ns)) return false;
-    }
-  }
-}
-// The same of one thread.
+// Bounded wait of a thread.
 __device__ __forceinline__ bool it_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
   uint64_t t0 = 0;
 #pragma unroll 1
@@ -67,6 +56,15 @@ __device__ __forceinline__ bool it_wait(uint32_t bar, uint32_t parity, volatile 
     }
   }
 }
+// The same of a warp, with the same answer for every lane, so that a warp leaves a role together. seen: the lane knows already (it_peek).
+__device__ __forceinline__ bool it_warp_wait(uint32_t seen, uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
+  if (!seen) seen = it_wait(bar, parity, abort_flag, budget_ns);
+  return __all_sync(0xffffffffu, seen);
+}
+// Looks at a phase without waiting, well before the answer is needed: a wait on a phase that is long complete takes a hundred cycles and more. Only for
+// a phase whose predecessor on that barrier the asking role has seen complete.
+__device__ __forceinline__ uint32_t it_peek(uint32_t bar, uint32_t parity) { return mbar_test_wait(bar, parity) ? 1u : 0u; }
+
 // a += b * s on two neighbours at a time
 __device__ __forceinline__ void it_fma2(uint64_t& a, uint32_t b0, uint32_t b1, uint64_t s) {
   asm("{\n\t.reg .b64 b;\n\tmov.b64 b, {%1, %2};\n\tfma.rn.f32x2 %0, b, %3, %0;\n\t}" : "+l"(a) : "r"(b0), "r"(b1), "l"(s));
@@ -86,13 +84,16 @@ __device__ __forceinline__ float2 it_unpack(uint64_t a) {
 template <int NT>
 struct ItShape {
   static constexpr bool WIDE = NT == 128;                  // one CTA per SM, 512 columns; else two with 256 each
-  static constexpr int CONV_WARPS = WIDE ? 8 : 4, EPI_WARPS = NT >= 64 ? 8 : 4;
+  static constexpr int CONV_WARPS = NT == 64 ? 4 : 8, EPI_WARPS = NT >= 64 ? 8 : 4;
   static constexpr int THREADS = 32 * (4 + CONV_WARPS + EPI_WARPS);       // warps 0 and 1 produce and issue, 2 and 3 only align the quadrants
-  static constexpr int ACC = NT < 32 ? 32 : NT;            // columns of an accumulator
-  static constexpr int BUFS = NT <= 32 ? 4 : 2;
-  static constexpr int SLOTS = WIDE ? 4 : 2;               // of a converted step, 64 columns each
+  static constexpr int ACC = NT;                           // columns of an accumulator
+  static constexpr int BUFS = WIDE ? 3 : NT == 16 ? 4 : 2;
+  static constexpr int SLOTS = NT == 16 || NT == 32 ? 3 : 2;       // of a converted step, 64 columns each
   static constexpr int COLS = WIDE ? 512 : 256;
   static constexpr int EPI_COLS = NT / (EPI_WARPS / 4);    // columns of an epilogue warp
+  // Scales of the steps that are converted and not drained: a converter that writes those of step s + IT_SCALES has seen the MMAs of step s + IT_SCALES
+  // - SLOTS done, which began after the epilogue had freed the accumulators of step s + IT_SCALES - SLOTS - BUFS, and had read their scales before
+  static_assert(SLOTS + BUFS < IT_SCALES, "the ring of scales");
   static_assert(BUFS * ACC + SLOTS * 64 <= COLS, "tensor memory");
 };
 
@@ -105,6 +106,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag, unit[5];     // expert (-1: no such unit), feature tile, first row of the result, rows, first row in the expert
   __shared__ int src[NT];
+  __shared__ float scales[IT_SCALES][GP][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const bool zeros = p.flags & 8;
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < p.stages; ++s) { mbar_init(smem_u32(&bar_full[s]), 1); mbar_init(smem_u32(&bar_empty[s]), 1 + S::EPI_WARPS); }
+    for (int s = 0; s < p.stages; ++s) { mbar_init(smem_u32(&bar_full[s]), 1); mbar_init(smem_u32(&bar_empty[s]), 1); }
     for (int s = 0; s < S::SLOTS; ++s) { mbar_init(smem_u32(&bar_cfull[s]), 4); mbar_init(smem_u32(&bar_cempty[s]), 1); }
     for (int b = 0; b < S::BUFS; ++b) { mbar_init(smem_u32(&bar_dfull[b]), 1); mbar_init(smem_u32(&bar_dempty[b]), S::EPI_WARPS); }
     fence_mbar_init();
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       int st = 0;
       uint32_t ph = 0;
       for (int s = s0; s < s1; ++s) {
-        if (!it_warp_wait(smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
+        if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
           break;
         }
@@ -219,17 +221,20 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       if (elect_one()) {
         const uint32_t idesc = umma_idesc(1, 1, 128, NT);
         int st = 0, slot = 0, buf = 0;
-        uint32_t sph = 0, bph = 0;
+        uint32_t sph = 0, bph = 0, seen_c = 0, seen_d = 0;
         bool ok = true;
         for (int s = s0; s < s1; ++s) {
           // (the converters have seen the stage arrive, x included)
-          if (!it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; break; }
+          if (!seen_c && !it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; break; }
           const uint32_t at = smem_base + st * stage_bytes;
           const uint64_t dx0 = umma_desc_sw128(at), dx1 = umma_desc_sw128(at + NT * 128);
           const uint32_t a_tmem = tmem_base + S::BUFS * S::ACC + slot * 64;
+          const uint32_t cempty = smem_u32(&bar_cempty[slot]), empty = smem_u32(&bar_empty[st]);
+          if (++slot == S::SLOTS) { slot = 0; sph ^= 1; }
+          if (++st == p.stages) st = 0;
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
-            if (!it_wait(smem_u32(&bar_dempty[buf]), bph ^ 1, &abort_flag, p.budget_ns)) {
+            if (!seen_d && !it_wait(smem_u32(&bar_dempty[buf]), bph ^ 1, &abort_flag, p.budget_ns)) {
               report_status(p.status, ST_TIMEOUT_TMEM_EMPTY, blockIdx.x);
               ok = false;
               break;
@@ -243,32 +248,37 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             }
             tc_commit(smem_u32(&bar_dfull[buf]));
             if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
+            seen_d = it_peek(smem_u32(&bar_dempty[buf]), bph ^ 1);
           }
           if (!ok) { abort_flag = 1; break; }
-          tc_commit(smem_u32(&bar_cempty[slot]));
-          tc_commit(smem_u32(&bar_empty[st]));
-          if (++slot == S::SLOTS) { slot = 0; sph ^= 1; }
-          if (++st == p.stages) st = 0;
+          seen_c = it_peek(smem_u32(&bar_cfull[slot]), sph);
+          tc_commit(cempty);
+          tc_commit(empty);
         }
       }
       __syncwarp();
     } else if (warp >= 4 && warp < 4 + S::CONV_WARPS) {
       // ================= converters: row r of the tile; with eight warps the two groups take the steps in turn =================
-      const int r = (warp & 3) * 32 + lane;
       constexpr int GROUPS = S::CONV_WARPS / 4;
-      const int group = (warp - 4) >> 2;
+      const int r = (warp & 3) * 32 + lane, group = (warp - 4) >> 2;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
-      const int in_stage = X_BYTES + (r >> 4) * I4_CODES + (r & 7) * 16 + ((r >> 3) & 1) * 8;
-      const int zero_at = X_BYTES + i4_zeros(GP) + ((r >> 4) * 8 + (r & 7)) * GP * 2 + ((r >> 3) & 1);
-      int st = group % p.stages, slot = group;
-      uint32_t ph = 0, sph = 0;
+      const int in_stage = X_BYTES + (r >> 4) * I4_CODES + (r & 7) * 16 + ((r >> 3) & 1) * 8, row_at = (r >> 4) * 8 + (r & 7), odd = (r >> 3) & 1;
+      const int zero_at = X_BYTES + i4_zeros(GP) + row_at * GP * 2 + odd, scale_at = X_BYTES + I4_SCALES + row_at * GP * 4 + odd * 2;
+      int st = group, slot = group;
+      uint32_t ph = 0, sph = 0, seen = 0;
       for (int s = s0 + group; s < s1; s += GROUPS) {
-        if (!it_warp_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
+        if (!it_warp_wait(seen, smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
           break;
         }
         const uint8_t* at = smem_raw + (smem_base - smem_u32(smem_raw)) + st * stage_bytes;
-        const uint32_t to = tmem_base + S::BUFS * S::ACC + slot * 64 + lane_tmem;
+        const uint32_t to = tmem_base + S::BUFS * S::ACC + slot * 64 + lane_tmem, cfull = smem_u32(&bar_cfull[slot]), cempty = smem_u32(&bar_cempty[slot]);
+        uint32_t free_slot = it_peek(cempty, sph ^ 1);
+        const uint32_t sph_now = sph;
+        slot += GROUPS;
+        if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
+        st += GROUPS;                         // (an even number of stages: a group sees every phase of its own)
+        if (st >= p.stages) { st -= p.stages; ph ^= 1; }
         bool ok = true;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -287,58 +297,49 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             i4_expand(c[t].y, base[1], v + 16 + t * 4);
           }
           if (j == 0) {
-            if (!it_warp_wait(smem_u32(&bar_cempty[slot]), sph ^ 1, &abort_flag, p.budget_ns)) {
+            if (!it_warp_wait(free_slot, cempty, sph_now ^ 1, &abort_flag, p.budget_ns)) {
               if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
               ok = false;
               break;
             }
             tc_fence_after();
+#pragma unroll
+            for (int g = 0; g < GP; ++g)
+              scales[(s - s0) & (IT_SCALES - 1)][g][r] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
           }
           tmem_st16(to + j * 32, v);
           tmem_st16(to + j * 32 + 16, v + 16);
         }
         if (!ok) break;
+        seen = it_peek(smem_u32(&bar_full[st]), ph);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_cfull[slot]));
-        slot += GROUPS;
-        if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
-        st += GROUPS;
-        if (st >= p.stages) { st -= p.stages; ph ^= 1; }
+        if (lane == 0) mbar_arrive(cfull);
       }
     } else if (warp >= 4) {
       // ================= epilogue: row r, columns col0 .. + EPI_COLS =================
       const int r = (warp & 3) * 32 + lane, col0 = ((warp - 4 - S::CONV_WARPS) >> 2) * S::EPI_COLS;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
-      const int scale_at = X_BYTES + I4_SCALES + ((r >> 4) * 8 + (r & 7)) * GP * 4 + ((r >> 3) & 1) * 2;
 #pragma unroll
       for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[c] = 0ull;
-      int st = 0, buf = 0;
-      uint32_t ph = 0, bph = 0;
+      int buf = 0;
+      uint32_t bph = 0, seen = 0;
       bool ok = true;
       for (int s = s0; s < s1 && ok; ++s) {
-        if (!it_warp_wait(smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
-          if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
-          break;
-        }
-        const uint8_t* at = smem_raw + (smem_base - smem_u32(smem_raw)) + st * stage_bytes;
-        float sc[GP];
-#pragma unroll
-        for (int g = 0; g < GP; ++g) sc[g] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_empty[st]));
-        if (++st == p.stages) { st = 0; ph ^= 1; }
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          if (!it_warp_wait(smem_u32(&bar_dfull[buf]), bph, &abort_flag, p.budget_ns)) {
+          if (!it_warp_wait(seen, smem_u32(&bar_dfull[buf]), bph, &abort_flag, p.budget_ns)) {
             if (lane == 0) { report_status(p.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x); abort_flag = 1; }
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem;
-          const uint64_t s2 = it_pack(sc[g], sc[g]);
+          const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem, dempty = smem_u32(&bar_dempty[buf]);
+          // (written before the arrival that let the step's MMAs begin)
+          const float sc = *reinterpret_cast<volatile float*>(&scales[(s - s0) & (IT_SCALES - 1)][g][r]);
+          const uint64_t s2 = it_pack(sc, sc);
+          if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
           constexpr int STEP = S::EPI_COLS < 32 ? 16 : 32;
 #pragma unroll
           for (int c0 = 0; c0 < S::EPI_COLS; c0 += STEP) {
@@ -349,12 +350,12 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             if (c0 + STEP == S::EPI_COLS) {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(smem_u32(&bar_dempty[buf]));
+              if (lane == 0) mbar_arrive(dempty);
+              seen = it_peek(smem_u32(&bar_dfull[buf]), bph);
             }
 #pragma unroll
             for (int c = 0; c < STEP; c += 2) it_fma2(acc[(c0 + c) / 2], v[c], v[c + 1], s2);
           }
-          if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
         }
       }
     }
@@ -429,10 +430,11 @@ template <int NT, int GP>
 static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s) {
   using S = ItShape<NT>;
   static PerDevice allowed;
-  const int room = (S::WIDE ? 225 : 111) * 1024;
+  const int room = (S::WIDE ? 224 : 112) * 1024 - IT_SCALES * GP * 512 - 2048;     // (beside the static part)
   const int stage = NT * 256 + ((i4_record(GP, p.flags & 8) + 1023) & ~1023);
   p.stages = (room - 1024) / stage;
   if (p.stages > IT_MAX_STAGES) p.stages = IT_MAX_STAGES;
+  p.stages &= ~1;        // every stage belongs to one group of converters
   const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP>, room);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};

@@ -1,7 +1,7 @@
 // Products with 4-bit weights (int4.cuh) on tcgen05: y[r, f] = sum over groups j of scale[f, j] * ( sum_{k in j} x[r, k] (code[f, k] - zero[f, j]) ).
 //
-// Weights are the M side (128 rows of a tile), NT rows of x the N side. A CTA owns a tile, or with few tiles a piece of its K (the CTAs of a cluster
-// share the tile). Roles, one pipeline:
+// Weights are the M side (128 rows of a tile), NT rows of x the N side. A CTA walks tiles, or with few of them owns a piece of the K of one (the CTAs of
+// a cluster share the tile). Roles, one pipeline:
 //   producer    one bulk copy per step (codes, scales and zeros of 128 rows x 128 of K are one run) and TMA tiles of x, or of the rows that
 //               src_row names (tile::gather4), into a ring of shared-memory stages
 //   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (exact), 64 of K a slot, written to tensor
@@ -104,8 +104,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[IT_MAX_STAGES], bar_empty[IT_MAX_STAGES], bar_cfull[S::SLOTS], bar_cempty[S::SLOTS], bar_dfull[S::BUFS], bar_dempty[S::BUFS];
   __shared__ uint32_t tmem_base_smem;
-  __shared__ int abort_flag, unit[5];     // expert (-1: no such unit), feature tile, first row of the result, rows, first row in the expert
-  __shared__ int src[NT];
+  __shared__ int abort_flag;
   __shared__ float scales[IT_SCALES][GP][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -129,16 +128,16 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   pdl_trigger();
   pdl_wait();
 
-  // ---- which tile: experts in order, in each bands of feature tiles, in a band the feature tile runs fastest
-  const int rank = (int)blockIdx.x % p.split;
+  // ---- the tiles: experts in order, in each bands of feature tiles, in a band the feature tile runs fastest. pre: tiles before an expert
+  int* pre = reinterpret_cast<int*>(smem_raw + (smem_base - smem_u32(smem_raw)) + p.stages * stage_bytes);
+  int *cnt = pre + p.E + 1, *off = cnt + p.E;
   if (warp == 0) {
-    const int u = (int)blockIdx.x / p.split;
-    int found = -1, before = 0, count = p.rows, first = 0;
-    if (p.counts == nullptr) found = u < p.m_tiles * ((p.rows + NT - 1) / NT) ? 0 : -1;
-    else {
-      for (int e0 = 0; e0 < p.E && found < 0; e0 += 32) {
-        int c = 0, o = 0;
-        if (e0 + lane < p.E) {
+    int run = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      int c = 0, o = 0;
+      if (e0 + lane < p.E) {
+        c = p.rows;
+        if (p.counts != nullptr) {
           c = p.counts[e0 + lane];
           o = p.offsets[e0 + lane];
           if (o < 0 || c < 0 || c > p.rows - o) {
@@ -146,76 +145,104 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             c = 0;
           }
         }
-        const int mine = p.m_tiles * ((c + NT - 1) / NT);
-        int inc = mine;
-        for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += v; }
-        const unsigned hit = __ballot_sync(0xffffffffu, u < before + inc);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          found = e0 + l;
-          before = __shfl_sync(0xffffffffu, before + inc - mine, l);
-          count = __shfl_sync(0xffffffffu, c, l);
-          first = __shfl_sync(0xffffffffu, o, l);
-        } else before += __shfl_sync(0xffffffffu, inc, 31);
       }
+      const int mine = p.m_tiles * ((c + NT - 1) / NT);
+      int inc = mine;
+      for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, inc, d); if (lane >= d) inc += v; }
+      if (e0 + lane < p.E) { pre[e0 + lane] = run + inc - mine; cnt[e0 + lane] = c; off[e0 + lane] = o; }
+      run += __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (found >= 0) {
-      const int r = u - before, nt = (count + NT - 1) / NT;
-      const int band = r / (IT_BAND * nt), rb = r - band * IT_BAND * nt, bm = min(IT_BAND, p.m_tiles - band * IT_BAND), n = rb / bm;
-      for (int i = lane; i < NT; i += 32) {
-        const int at = n * NT + i;
-        int row = 0;
-        if (p.src_row != nullptr && at < count) {
-          row = p.src_row[first + at];
-          if (row < 0 || row >= p.x_rows) { report_status(p.status, ST_BAD_INDEX, row); row = 0; }
-        }
-        src[i] = row;
-      }
-      if (lane == 0) { unit[1] = band * IT_BAND + rb - n * bm; unit[2] = first + n * NT; unit[3] = min(NT, count - n * NT); }
-    }
-    if (lane == 0) unit[0] = found;
+    if (lane == 0) pre[p.E] = run;
   }
   __syncthreads();
-  const int e = unit[0];
-  const bool live = e >= 0;            // the same for every CTA of a cluster
-  const int m = unit[1], row0 = unit[2], valid = unit[3];
+  const int total = pre[p.E];
+  // A CTA walks tiles `first`, first + hop, ..., every role at its own pace: the next tile's steps begin while the last one's results are stored. The
+  // CTAs of a cluster share one tile.
+  const int rank = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, hop = (int)gridDim.x / p.split;
   const int s0 = (int)((long long)p.steps * rank / p.split), s1 = (int)((long long)p.steps * (rank + 1) / p.split);
-  uint64_t acc[S::EPI_COLS / 2];       // two columns each
+  struct Tile { int e, m, row0, valid; };
+  auto tile_at = [&](int u, int& e) {        // e: the expert of the role's tile before
+    while (u >= pre[e + 1]) ++e;
+    const int r = u - pre[e], nt = (cnt[e] + NT - 1) / NT, band = r / (IT_BAND * nt), rb = r - band * IT_BAND * nt, bm = min(IT_BAND, p.m_tiles - band * IT_BAND), n = rb / bm;
+    return Tile{e, band * IT_BAND + rb - n * bm, off[e] + n * NT, min(NT, cnt[e] - n * NT)};
+  };
+  const bool live = first < total;           // the same for every CTA of a cluster
+  uint64_t acc[S::EPI_COLS / 2];             // two columns each
+  const bool pair = p.flags & 1, f32 = p.flags & 4;
+  // stores two columns of the result; of a pair the gate's lane finishes the first and the up's the second
+  auto finish = [&](const Tile& tl, int col, float a, float b) {
+    const int r = (warp & 3) * 32 + lane, f = pair ? (tl.m * 8 + (r >> 4)) * 8 + (r & 7) : tl.m * 128 + r;
+    auto store = [&](int c, float y) {
+      const size_t at = (size_t)(tl.row0 + c) * p.out_ld + f;
+      if (f32) ((float*)p.out)[at] = p.residual ? y + ((const float*)p.residual)[at] : y;
+      else ((__nv_bfloat16*)p.out)[at] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[at]) : y);
+    };
+    if (!pair) {
+      if (f < p.F && col < tl.valid) store(col, a);
+      if (f < p.F && col + 1 < tl.valid) store(col + 1, b);
+    } else {
+      const bool up = r & 8;
+      const float other = __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
+      const int c = up ? col + 1 : col;
+      const float y = up ? silu(other) * b : silu(a) * other;
+      if (f < p.F && c < tl.valid) store(c, y);
+    }
+  };
 
   if (live) {
-    const uint8_t* w = p.w + ((size_t)e * p.m_tiles + m) * p.steps * rec;
     if (warp == 0) {
       // ================= producer =================
       if (lane == 0) tma_prefetch_desc(&tmX);
       const uint64_t keep = l2_policy_evict_last();
-      int st = 0;
+      int st = 0, e = 0;
       uint32_t ph = 0;
-      for (int s = s0; s < s1; ++s) {
-        if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
-          if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
-          break;
-        }
-        const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
-        if (lane == 0) {
-          mbar_expect_tx(full, X_BYTES + rec);
-          bulk_load_1d(at + X_BYTES, w + (size_t)s * rec, rec, full);
-          if (p.src_row == nullptr) {
-            tma_load_2d(at, &tmX, full, s * I4_STEP, row0, keep);
-            tma_load_2d(at + NT * 128, &tmX, full, s * I4_STEP + 64, row0, keep);
-          }
-        }
-        __syncwarp();
+      bool ok = true;
+      for (int u = first; u < total && ok; u += hop) {
+        const Tile tl = tile_at(u, e);
+        const uint8_t* w = p.w + ((size_t)tl.e * p.m_tiles + tl.m) * p.steps * rec;
+        // a lane's part of a gathered tile: four rows of a half, twice with 128 rows
+        constexpr int PARTS = NT == 128 ? 2 : 1;
+        int from[PARTS][4];
         if (p.src_row != nullptr) {
-          // a half that lies behind K as a whole has scales of zero: any columns do
-          const int x1 = s * I4_STEP + 64 < p.K ? s * I4_STEP + 64 : 0;
-          for (int i = lane; i < NT / 2; i += 32) {
-            const int j = i & 1, q = (i >> 1) * 4;
-            it_gather4(at + j * NT * 128 + q * 128, &tmX, full, j ? x1 : s * I4_STEP, src[q], src[q + 1], src[q + 2], src[q + 3]);
-          }
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int at = ((lane + 32 * i) >> 1) * 4 + k;
+              int row = 0;
+              if (at < tl.valid) {
+                row = p.src_row[tl.row0 + at];
+                if (row < 0 || row >= p.x_rows) { report_status(p.status, ST_BAD_INDEX, row); row = 0; }
+              }
+              from[i][k] = row;
+            }
         }
-        if (++st == p.stages) { st = 0; ph ^= 1; }
+        for (int s = s0; s < s1; ++s) {
+          if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
+            if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
+            ok = false;
+            break;
+          }
+          const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
+          if (lane == 0) {
+            mbar_expect_tx(full, X_BYTES + rec);
+            bulk_load_1d(at + X_BYTES, w + (size_t)s * rec, rec, full);
+            if (p.src_row == nullptr) {
+              tma_load_2d(at, &tmX, full, s * I4_STEP, tl.row0, keep);
+              tma_load_2d(at + NT * 128, &tmX, full, s * I4_STEP + 64, tl.row0, keep);
+            }
+          }
+          __syncwarp();
+          if (p.src_row != nullptr) {
+            // a half that lies behind K as a whole has scales of zero: any columns do
+            const int x = lane & 1 ? (s * I4_STEP + 64 < p.K ? s * I4_STEP + 64 : 0) : s * I4_STEP;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i)
+              if (lane + 32 * i < NT / 2) it_gather4(at + (lane & 1) * NT * 128 + ((lane + 32 * i) >> 1) * 512, &tmX, full, x, from[i][0], from[i][1], from[i][2], from[i][3]);
+          }
+          if (++st == p.stages) { st = 0; ph ^= 1; }
+        }
       }
-      __syncwarp();
     } else if (warp == 1) {
       // ================= MMA =================
       if (elect_one()) {
@@ -223,9 +250,10 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
         int st = 0, slot = 0, buf = 0;
         uint32_t sph = 0, bph = 0, seen_c = 0, seen_d = 0;
         bool ok = true;
+        for (int u = first; u < total && ok; u += hop)
         for (int s = s0; s < s1; ++s) {
           // (the converters have seen the stage arrive, x included)
-          if (!seen_c && !it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; break; }
+          if (!seen_c && !it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; ok = false; break; }
           const uint32_t at = smem_base + st * stage_bytes;
           const uint64_t dx0 = umma_desc_sw128(at), dx1 = umma_desc_sw128(at + NT * 128);
           const uint32_t a_tmem = tmem_base + S::BUFS * S::ACC + slot * 64;
@@ -266,7 +294,9 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       const int zero_at = X_BYTES + i4_zeros(GP) + row_at * GP * 2 + odd, scale_at = X_BYTES + I4_SCALES + row_at * GP * 4 + odd * 2;
       int st = group, slot = group;
       uint32_t ph = 0, sph = 0, seen = 0;
-      for (int s = s0 + group; s < s1; s += GROUPS) {
+      // (a step is a step here, whatever tile it belongs to)
+      const int n_steps = (total - first + hop - 1) / hop * (s1 - s0);
+      for (int s = group; s < n_steps; s += GROUPS) {
         if (!it_warp_wait(seen, smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
           break;
@@ -305,7 +335,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             tc_fence_after();
 #pragma unroll
             for (int g = 0; g < GP; ++g)
-              scales[(s - s0) & (IT_SCALES - 1)][g][r] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
+              scales[s & (IT_SCALES - 1)][g][r] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
           }
           tmem_st16(to + j * 32, v);
           tmem_st16(to + j * 32 + 16, v + 16);
@@ -321,52 +351,58 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       // ================= epilogue: row r, columns col0 .. + EPI_COLS =================
       const int r = (warp & 3) * 32 + lane, col0 = ((warp - 4 - S::CONV_WARPS) >> 2) * S::EPI_COLS;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
-#pragma unroll
-      for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[c] = 0ull;
-      int buf = 0;
+      int buf = 0, it = 0, e = 0;
       uint32_t bph = 0, seen = 0;
       bool ok = true;
-      for (int s = s0; s < s1 && ok; ++s) {
+      for (int u = first; u < total; u += hop) {
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          if (!it_warp_wait(seen, smem_u32(&bar_dfull[buf]), bph, &abort_flag, p.budget_ns)) {
-            if (lane == 0) { report_status(p.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x); abort_flag = 1; }
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem, dempty = smem_u32(&bar_dempty[buf]);
-          // (written before the arrival that let the step's MMAs begin)
-          const float sc = *reinterpret_cast<volatile float*>(&scales[(s - s0) & (IT_SCALES - 1)][g][r]);
-          const uint64_t s2 = it_pack(sc, sc);
-          if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
-          constexpr int STEP = S::EPI_COLS < 32 ? 16 : 32;
+        for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[c] = 0ull;
+        for (int s = s0; s < s1 && ok; ++s, ++it) {
 #pragma unroll
-          for (int c0 = 0; c0 < S::EPI_COLS; c0 += STEP) {
-            uint32_t v[STEP];
-            tmem_ld16(from + c0, v);
-            if constexpr (STEP == 32) tmem_ld16(from + c0 + 16, v + 16);
-            tmem_ld_wait();
-            if (c0 + STEP == S::EPI_COLS) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(dempty);
-              seen = it_peek(smem_u32(&bar_dfull[buf]), bph);
+          for (int g = 0; g < GP; ++g) {
+            if (!it_warp_wait(seen, smem_u32(&bar_dfull[buf]), bph, &abort_flag, p.budget_ns)) {
+              if (lane == 0) { report_status(p.status, ST_TIMEOUT_TMEM_FULL, blockIdx.x); abort_flag = 1; }
+              ok = false;
+              break;
             }
+            tc_fence_after();
+            const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem, dempty = smem_u32(&bar_dempty[buf]);
+            // (written before the arrival that let the step's MMAs begin)
+            const float sc = *reinterpret_cast<volatile float*>(&scales[it & (IT_SCALES - 1)][g][r]);
+            const uint64_t s2 = it_pack(sc, sc);
+            if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
+            constexpr int STEP = S::EPI_COLS < 32 ? 16 : 32;
 #pragma unroll
-            for (int c = 0; c < STEP; c += 2) it_fma2(acc[(c0 + c) / 2], v[c], v[c + 1], s2);
+            for (int c0 = 0; c0 < S::EPI_COLS; c0 += STEP) {
+              uint32_t v[STEP];
+              tmem_ld16(from + c0, v);
+              if constexpr (STEP == 32) tmem_ld16(from + c0 + 16, v + 16);
+              tmem_ld_wait();
+              if (c0 + STEP == S::EPI_COLS) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(dempty);
+                seen = it_peek(smem_u32(&bar_dfull[buf]), bph);
+              }
+#pragma unroll
+              for (int c = 0; c < STEP; c += 2) it_fma2(acc[(c0 + c) / 2], v[c], v[c + 1], s2);
+            }
           }
         }
+        if (!ok || p.split > 1) break;
+        const Tile tl = tile_at(u, e);
+#pragma unroll
+        for (int c = 0; c < S::EPI_COLS; c += 2)
+          if (col0 + c < tl.valid) { const float2 v = it_unpack(acc[c / 2]); finish(tl, col0 + c, v.x, v.y); }
       }
     }
   }
 
   // ---- the pieces of a tile: every CTA finishes NT / split columns, summed in rank order
-  const bool epi = warp >= 4 + S::CONV_WARPS;
-  const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS;
-  const int slice = NT / p.split;
-  float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));      // [rank][slice][128], on stages that nothing reads any more
   if (p.split > 1 && live) {
+    const bool epi = warp >= 4 + S::CONV_WARPS;
+    const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS, slice = NT / p.split;
+    float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));      // [rank][slice][128], on stages that nothing reads any more
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (epi) {
@@ -379,41 +415,17 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       }
     }
     cluster.sync();
-  }
-  if (live && epi && abort_flag == 0) {
-    const bool pair = p.flags & 1, f32 = p.flags & 4;
-    const int f = pair ? (m * 8 + (r >> 4)) * 8 + (r & 7) : m * 128 + r;
-    auto store = [&](int col, float y) {
-      const size_t at = (size_t)(row0 + col) * p.out_ld + f;
-      if (f32) ((float*)p.out)[at] = p.residual ? y + ((const float*)p.residual)[at] : y;
-      else ((__nv_bfloat16*)p.out)[at] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[at]) : y);
-    };
-    // two columns; of a pair the gate's lane finishes the first and the up's the second
-    auto finish = [&](int col, float a, float b) {
-      if (!pair) {
-        if (f < p.F && col < valid) store(col, a);
-        if (f < p.F && col + 1 < valid) store(col + 1, b);
-      } else {
-        const bool up = r & 8;
-        const float other = __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
-        const int c = up ? col + 1 : col;
-        const float y = up ? silu(other) * b : silu(a) * other;
-        if (f < p.F && c < valid) store(c, y);
-      }
-    };
-    if (p.split == 1) {
-#pragma unroll
-      for (int c = 0; c < S::EPI_COLS; c += 2)
-        if (col0 + c < valid) { const float2 v = it_unpack(acc[c / 2]); finish(col0 + c, v.x, v.y); }
-    } else {
+    if (epi && abort_flag == 0) {
+      int e = 0;
+      const Tile tl = tile_at(first, e);
       for (int c = part * 2; c < slice; c += 2 * (S::EPI_WARPS / 4)) {
-        if (rank * slice + c >= valid) break;
+        if (rank * slice + c >= tl.valid) break;
         float a = 0.f, b = 0.f;
         for (int q = 0; q < p.split; ++q) {
           a += recv[(q * slice + c) * 128 + r];
           b += recv[(q * slice + c + 1) * 128 + r];
         }
-        finish(rank * slice + c, a, b);
+        finish(tl, rank * slice + c, a, b);
       }
     }
   }
@@ -430,17 +442,19 @@ template <int NT, int GP>
 static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s) {
   using S = ItShape<NT>;
   static PerDevice allowed;
-  const int room = (S::WIDE ? 224 : 112) * 1024 - IT_SCALES * GP * 512 - 2048;     // (beside the static part)
+  const int list = 4 * (3 * p.E + 1), room = (S::WIDE ? 224 : 112) * 1024 - IT_SCALES * GP * 512 - 2048;     // (beside the static part)
   const int stage = NT * 256 + ((i4_record(GP, p.flags & 8) + 1023) & ~1023);
-  p.stages = (room - 1024) / stage;
+  p.stages = (room - 1024 - list) / stage;
   if (p.stages > IT_MAX_STAGES) p.stages = IT_MAX_STAGES;
   p.stages &= ~1;        // every stage belongs to one group of converters
+  if (p.stages < 2) return -1;
   const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP>, room);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)tiles * p.split);
+  // a cluster has one tile, else a CTA per place on the GPU walks them
+  cfg.gridDim = dim3(p.split > 1 ? (unsigned)tiles * p.split : (unsigned)min(tiles, S::WIDE ? 148 : 296));
   cfg.blockDim = dim3(S::THREADS);
-  cfg.dynamicSmemBytes = (size_t)p.stages * stage + 1024;
+  cfg.dynamicSmemBytes = (size_t)p.stages * stage + 1024 + list;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -467,7 +481,7 @@ extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, 
                              int split, int* status, void* stream) {
   using namespace skein;
   if (rows == 0) return 0;
-  if (rows < 0 || x_rows < 1 || E < 1 || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
+  if (rows < 0 || x_rows < 1 || E < 1 || E > 1024 || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
   if (x_ld % 8 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0) return -1;
   if (n_tile == 0) n_tile = rows_hint <= 16 ? 16 : rows_hint <= 32 ? 32 : rows_hint <= 64 ? 64 : 128;
   if (n_tile != 16 && n_tile != 32 && n_tile != 64 && n_tile != 128) return -1;

@@ -309,24 +309,33 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
         if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
         st += GROUPS;                         // (an even number of stages: a group sees every phase of its own)
         if (st >= p.stages) { st -= p.stages; ph ^= 1; }
+        // With registers for it the whole step is ready before the slot is asked for: what follows the wait is in the chain slot - MMAs - slot.
+        constexpr int READY = S::WIDE ? 2 : 1;       // halves of a step
         bool ok = true;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint2 c[4];
+        for (int j0 = 0; j0 < 2; j0 += READY) {
+          uint32_t v[READY][32];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) c[t] = *reinterpret_cast<const uint2*>(at + in_stage + j * 512 + t * 128);
-          uint32_t base[2] = {I4_EIGHT, I4_EIGHT};
-          if (zeros) {
-            base[0] = i4_zero(at[zero_at + (GP == 1 ? 0 : GP == 2 ? j : 2 * j) * 2]);
-            base[1] = GP == 4 ? i4_zero(at[zero_at + (2 * j + 1) * 2]) : base[0];
-          }
-          uint32_t v[32];
+          for (int i = 0; i < READY; ++i) {
+            const int j = j0 + i;
+            uint2 c[4];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            i4_expand(c[t].x, base[0], v + t * 4);
-            i4_expand(c[t].y, base[1], v + 16 + t * 4);
+            for (int t = 0; t < 4; ++t) c[t] = *reinterpret_cast<const uint2*>(at + in_stage + j * 512 + t * 128);
+            uint32_t base[2] = {I4_EIGHT, I4_EIGHT};
+            if (zeros) {
+              base[0] = i4_zero(at[zero_at + (GP == 1 ? 0 : GP == 2 ? j : 2 * j) * 2]);
+              base[1] = GP == 4 ? i4_zero(at[zero_at + (2 * j + 1) * 2]) : base[0];
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              i4_expand(c[t].x, base[0], v[i] + t * 4);
+              i4_expand(c[t].y, base[1], v[i] + 16 + t * 4);
+            }
           }
-          if (j == 0) {
+          if (j0 == 0) {
+            float sc[GP];
+#pragma unroll
+            for (int g = 0; g < GP; ++g) sc[g] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
             if (!it_warp_wait(free_slot, cempty, sph_now ^ 1, &abort_flag, p.budget_ns)) {
               if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
               ok = false;
@@ -334,11 +343,13 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             }
             tc_fence_after();
 #pragma unroll
-            for (int g = 0; g < GP; ++g)
-              scales[s & (IT_SCALES - 1)][g][r] = i4_scale(*reinterpret_cast<const uint16_t*>(at + scale_at + g * 4), p.flags & 2);
+            for (int g = 0; g < GP; ++g) scales[s & (IT_SCALES - 1)][g][r] = sc[g];
           }
-          tmem_st16(to + j * 32, v);
-          tmem_st16(to + j * 32 + 16, v + 16);
+#pragma unroll
+          for (int i = 0; i < READY; ++i) {
+            tmem_st16(to + (j0 + i) * 32, v[i]);
+            tmem_st16(to + (j0 + i) * 32 + 16, v[i] + 16);
+          }
         }
         if (!ok) break;
         seen = it_peek(smem_u32(&bar_full[st]), ph);

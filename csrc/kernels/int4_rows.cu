@@ -299,11 +299,18 @@ static int launch_rows(Int4Rows p, cudaStream_t s) {
   if (e != cudaSuccess) return (int)e;
   return (int)launch_pdl(int4_rows_kernel<NT, GP, ZERO, HALF, WK>, dim3(148), dim3(IR_THREADS), (size_t)TEAMS * (p.x_stage * ir_x_row(p.steps)), s, p);
 }
-// warps of a team: as many as leave each three steps or more of a strip, and more where its rows of x do not fit a smaller team's shared memory
+// Warps of a team: as many as leave each three steps or more of a strip, and more where its rows of x do not fit a smaller team's shared memory or the
+// strips are few (one row of 4096 x 4096, 256 strips: 7.3 us with 8 warps, 7.7 with 16, but four rows 8.9 and 8.8, and 1024 x 4096 5.9 and 5.3;
+// 28672 x 4096 25.2 and 27.7; 2048 x 1408 over experts 32.7 with 4, 34.8 with 8).
 template <int NT, int GP, bool ZERO, bool HALF>
 static int pick_team(const Int4Rows& p, int team, cudaStream_t s) {
   const int x = min(8 * NT, p.rows) * ir_x_row(p.steps);
-  if (team == 0) team = p.steps >= 48 || (p.steps >= 16 && x > IR_SMEM / 2) ? 16 : p.steps >= 24 || (p.steps >= 8 && x > IR_SMEM / 4) ? 8 : p.steps >= 4 ? 4 : 1;
+  const long long strips = (long long)p.strips * min(p.E, p.rows);
+  if (team == 0)
+    team = p.steps >= 48 || (p.steps >= 24 && strips <= 296 && (p.rows > 2 || strips <= 148)) || (p.steps >= 16 && x > IR_SMEM / 2)  ? 16
+           : p.steps >= 24 || (p.steps >= 8 && x > IR_SMEM / 4) ? 8
+           : p.steps >= 4                                       ? 4
+                                                                : 1;
   if (team > p.steps) return -1;
   switch (team) {
     case 16: return launch_rows<NT, GP, ZERO, HALF, 16>(p, s);

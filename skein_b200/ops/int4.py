@@ -26,7 +26,7 @@ class Int4Weight:
     def __init__(self, data, shape, group, pair, scales, zeros):
         self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
         self.scales, self.zeros = scales, zeros
-        self.device = data.device
+        self.device, self.K = data.device, shape[-1]
         self.features = shape[-2] // 2 if pair else shape[-2]
         self.flags = int(pair) | (2 if scales == torch.float16 else 0) | (8 if zeros else 0)
 
@@ -181,17 +181,28 @@ def _out(what, out, rows, w, dtype, device):
     return out
 
 
+def _few_rows(hint: int, K: int) -> bool:
+    """Whether a product with `hint` rows per matrix runs on the kernel of few rows (csrc/kernels/int4_rows.cu) instead of the one on tensor memory
+    (int4_tc.cu), which has more to set up and is the quicker one from where a warp's share of the rows of x costs more than the conversion. Measured, few
+    rows / tensor memory, us: 4096 x 4096 7.3 / 9.7 at 1 row, 9.8 / 10.1 at 8, 11.7 / 10.1 at 12; 4096 x 14336 13.9 / 17.4 at 1, 17.1 / 17.6 at 4, 19.0 / 17.6
+    at 6; gate / up 14336 x 4096 25.2 / 30.3 at 1, 29.1 / 30.9 at 8, 37.0 / 31.1 at 12; 8 experts of it 35.5 / 65.5 at 1 token, 156 / 188 at a mean of 8
+    rows, 277 / 251 at 16; 64 experts 2048 x 1408 32.7 / 33.4 at a mean of 1.5, 48.4 / 45.7 at 4.5."""
+    return hint <= 8 and hint * K <= 1 << 16
+
+
 def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags, cfg=None):
     """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, (0, team) of the kernel of few rows."""
     L, data = _lib.lib(), w.data
-    args = (x.data_ptr(), x.stride(0), _lib.ptr(src_row), data.data_ptr(), _lib.ptr(residual), out.data_ptr(), out.stride(0), _lib.ptr(counts),
-            _lib.ptr(offsets), rows, x.shape[0], data.shape[0], w.features, w.shape[-1], w.group, hint, flags)
+    xp, x_ld = x.data_ptr(), x.stride(0)
+    args = (xp, x_ld, src_row.data_ptr() if src_row is not None else None, data.data_ptr(), residual.data_ptr() if residual is not None else None,
+            out.data_ptr(), out.stride(0), counts.data_ptr() if counts is not None else None, offsets.data_ptr() if counts is not None else None, rows,
+            x.shape[0], data.shape[0], w.features, w.K, w.group, hint, flags)
     status, stream = F.workspace(x.device).status.data_ptr(), _lib.stream_ptr()
-    aligned = args[0] % 16 == 0 and args[1] % 8 == 0
-    if aligned and (hint > 16 if cfg is None else cfg[0] > 0):
-        rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), status, stream)
+    few = _few_rows(hint, w.K) if cfg is None else cfg[0] == 0
+    if few or xp % 16 or x_ld % 8:
+        rc = L.skein_int4_rows(*args, cfg[1] if cfg and few else 0, status, stream)
     else:
-        rc = L.skein_int4_rows(*args, cfg[1] if cfg else 0, status, stream)
+        rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), status, stream)
     _lib.check(rc, what)
     _lib.count_launch()
 

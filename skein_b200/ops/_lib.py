@@ -272,7 +272,12 @@ _HERE = _Here()
 
 def on_device(t):
     """Context in which the tensor's device is the current one (streams, allocations and launches follow it)."""
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def stream_on(device) -> int:
+    """Handle of the device's current stream: stream_ptr() without making a stream object (3 us less of a call that takes 10)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check(rc: int, what: str) -> None:

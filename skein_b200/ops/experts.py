@@ -12,6 +12,7 @@ from . import _lib, reference_int4 as ri
 
 MAX_EXPERTS, MAX_TOP, MAX_GROUPS = 512, 16, 64
 SCORES = ("softmax", "sigmoid")
+ONE_LAUNCH = 256       # tokens up to which one kernel does it all, without scratch
 
 
 def route_balanced(logits, top, bias=None, groups=1, keep=1, score="sigmoid", group_best=2, renorm=True, scale=1.0, e_first=0, e_count=None):
@@ -25,7 +26,8 @@ def route_balanced(logits, top, bias=None, groups=1, keep=1, score="sigmoid", gr
     Returns (ids int32 [T, top], weights fp32 [T, top], counts [E], offsets [E + 1], row_of [T * top], src_token [T * top]) as `ops.route` does: pair
     (t, j) sits at row_of[t * top + j] of the expert-sorted rows (-1: an expert outside e_first .. + e_count), src_token is its inverse; rows of
     src_token from offsets[E] on are unset."""
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    dtype = logits.dtype
+    if logits.dim() != 2 or dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("route_balanced: logits must be [tokens, experts] fp32 or bf16 with contiguous rows")
     T, E = logits.shape
     e_count = E - e_first if e_count is None else e_count
@@ -43,18 +45,18 @@ def route_balanced(logits, top, bias=None, groups=1, keep=1, score="sigmoid", gr
         return ri.route_balanced(logits, top, bias, groups, keep, score, group_best, renorm, scale, e_first, e_count)
     with _lib.on_device(logits):
         L, dev, n = _lib.lib(), logits.device, T * top
-        need = L.skein_route_balanced_scratch(T, E)
+        need = L.skein_route_balanced_scratch(T, E) if T > ONE_LAUNCH else 0
         if need < 0:
             raise ValueError(f"route_balanced: {T} tokens are more than one call takes")
-        ids = torch.empty(T, top, dtype=torch.int32, device=dev)
-        w = torch.empty(T, top, dtype=torch.float32, device=dev)
+        ids = torch.empty((T, top), dtype=torch.int32, device=dev)
+        w = torch.empty((T, top), dtype=torch.float32, device=dev)
         meta = torch.empty(2 * E + 1 + 2 * n, dtype=torch.int32, device=dev)
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         at = meta.data_ptr()
         rc = L.skein_route_balanced(
-            logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.bfloat16), _lib.ptr(bias), T, E, top, groups, keep, group_best, int(renorm),
-            int(score == "sigmoid"), float(scale), e_first, e_count, ids.data_ptr(), w.data_ptr(), at, at + 4 * E, at + 4 * (2 * E + 1),
-            at + 4 * (2 * E + 1 + n), _lib.ptr(scratch), _lib.stream_ptr())
+            logits.data_ptr(), logits.stride(0), dtype == torch.bfloat16, None if bias is None else bias.data_ptr(), T, E, top, groups, keep, group_best,
+            renorm, score == "sigmoid", scale, e_first, e_count, ids.data_ptr(), w.data_ptr(), at, at + 4 * E, at + 4 * (2 * E + 1),
+            at + 4 * (2 * E + 1 + n), scratch.data_ptr() if need else None, _lib.stream_on(dev))
         _lib.check(rc, "route_balanced")
         _lib.count_launch(2 if need else 1)
-    return (ids, w) + torch.split(meta, (E, E + 1, n, n))
+    return (ids, w, *meta.split_with_sizes((E, E + 1, n, n)))

@@ -27,6 +27,7 @@ class Int4Weight:
         self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
         self.scales, self.zeros = scales, zeros
         self.device, self.K = data.device, shape[-1]
+        self.ptr, self.matrices = data.data_ptr(), data.shape[0]
         self.features = shape[-2] // 2 if pair else shape[-2]
         self.flags = int(pair) | (2 if scales == torch.float16 else 0) | (8 if zeros else 0)
 
@@ -167,15 +168,15 @@ def _check(what, x, w: Int4Weight, pair, dims):
         raise ValueError(f"{what}: the weight must be an Int4Weight of {dims} dimensions")
     if w.pair != pair:
         raise ValueError(f"{what}: the weight is {'' if w.pair else 'not '}packed as a gate / up pair")
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != w.shape[-1] or x.stride(1) != 1:
-        raise ValueError(f"{what}: x must be bf16 [rows, {w.shape[-1]}] with contiguous rows")
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != w.K or x.stride(1) != 1:
+        raise ValueError(f"{what}: x must be bf16 [rows, {w.K}] with contiguous rows")
     if x.device != w.device:
         raise ValueError(f"{what}: x is on {x.device}, the weight on {w.device}")
 
 
 def _out(what, out, rows, w, dtype, device):
     if out is None:
-        return torch.empty(rows, w.features, dtype=dtype, device=device)
+        return torch.empty((rows, w.features), dtype=dtype, device=device)
     if out.shape != (rows, w.features) or out.dtype != dtype or out.device != device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
         raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
     return out
@@ -190,19 +191,28 @@ def _few_rows(hint: int, K: int) -> bool:
     return hint <= 8 and hint * K <= 1 << 16
 
 
+_STATUS: dict = {}      # device -> address of the status word of its workspace, which is made once
+
+
+def _status(device) -> int:
+    at = _STATUS.get(device)
+    if at is None:
+        at = _STATUS[device] = F.workspace(device).status.data_ptr()
+    return at
+
+
 def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags, cfg=None):
     """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, (0, team) of the kernel of few rows."""
-    L, data = _lib.lib(), w.data
+    L, dev = _lib.lib(), w.device
     xp, x_ld = x.data_ptr(), x.stride(0)
-    args = (xp, x_ld, src_row.data_ptr() if src_row is not None else None, data.data_ptr(), residual.data_ptr() if residual is not None else None,
-            out.data_ptr(), out.stride(0), counts.data_ptr() if counts is not None else None, offsets.data_ptr() if counts is not None else None, rows,
-            x.shape[0], data.shape[0], w.features, w.K, w.group, hint, flags)
-    status, stream = F.workspace(x.device).status.data_ptr(), _lib.stream_ptr()
     few = _few_rows(hint, w.K) if cfg is None else cfg[0] == 0
+    args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.ptr, None if residual is None else residual.data_ptr(), out.data_ptr(),
+            out.stride(0), None if counts is None else counts.data_ptr(), None if counts is None else offsets.data_ptr(), rows, x.shape[0], w.matrices,
+            w.features, w.K, w.group, hint, flags)
     if few or xp % 16 or x_ld % 8:
-        rc = L.skein_int4_rows(*args, cfg[1] if cfg and few else 0, status, stream)
+        rc = L.skein_int4_rows(*args, cfg[1] if cfg and few else 0, _status(dev), _lib.stream_on(dev))
     else:
-        rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), status, stream)
+        rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), _status(dev), _lib.stream_on(dev))
     _lib.check(rc, what)
     _lib.count_launch()
 
@@ -224,7 +234,7 @@ def _dense(what, x, w, out, residual, out_f32, cfg):
     T = x.shape[0]
     out = _out(what, out, T, w, torch.float32 if out_f32 else torch.bfloat16, x.device)
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
-                                 or residual.stride() != out.stride()):
+                                 or residual.stride(1) != 1 or (T > 1 and residual.stride(0) != out.stride(0))):
         raise ValueError(f"{what}: the residual must have the result's shape, type and strides")
     if T == 0:
         return out

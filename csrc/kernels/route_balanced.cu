@@ -6,14 +6,16 @@
 //
 // The bias steers the choice only. Scores are 64-bit: the choices of a step decide which rows meet which weights, and experts whose scores differ by
 // less than the error of a 32-bit exponential would be chosen by the build that computes them (with 256 experts one token in about 3000). A GPU of
-// this kind has the 64-bit rate for it. A logit that is not a number counts as the lowest; logits and choices are clamped to +-3e38, so that no
+// this kind has the 64-bit rate for it. A logit that is not a number counts as the lowest; logits and biases are clamped to +-3e38, so that no
 // input makes an index invalid.
 //
-// A warp owns a token; choices are kept as ordered 64-bit integers, a round of the choice is a maximum over the lanes' upper halves (one instruction)
-// and, where several lanes have it, over the lower halves and indices. The layout is a counting sort that keeps the tokens' order: for every
-// expert a CTA has one bit per token of its tile, so that a pair's place among the tile's is a count of bits, whatever order the warps came in.
-// Up to 256 tokens the tiles are the CTAs of one cluster, which add their counts up in distributed shared memory; beyond, the first
-// kernel leaves the tiles' counts in memory and a second one finishes the places.
+// A warp owns a token. Choices are kept as ordered 64-bit integers, whose last four bits give way to the expert's place in its lane (two choices within 16
+// units in the last place count as equal); a lane sorts its own, and a round of the choice is a maximum over the lanes' heads: one instruction on
+// the upper halves, two more where several lanes have the largest. Without the order a round compared all of them again (4096 tokens, 256 experts:
+// 3250 instructions per token, 35 us). The layout is a counting sort that keeps the tokens' order: for every expert a CTA has one bit per token of its
+// tile, so that a pair's place among the tile's is a count of bits, whatever order the warps came in. Up to 256 tokens the tiles are the CTAs of one
+// cluster, which add their counts up in distributed shared memory; beyond, the first kernel leaves the tiles' counts in memory and a second one
+// finishes the places.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include <cooperative_groups.h>
@@ -24,8 +26,8 @@ namespace skein {
 
 constexpr int RB_MAX_E = 512, RB_MAX_TOP = 16, RB_MAX_GROUPS = 64;
 constexpr int RB_CLUSTER = 8, RB_CLUSTER_TOKENS = 256;
-constexpr int RB_TILE = 32;              // tokens of a tile at least (a word of the bit masks)
-constexpr int RB_MAX_TILES = 256;
+constexpr int RB_TILE = 32;              // tokens of a tile at least: a warp each
+constexpr int RB_MAX_TILES = 148;        // (every CTA of the second kernel reads all tiles' counts: 256 tiles of 16 tokens took 35 us, 128 of 32 23)
 constexpr int RB_MAX_WORDS = 48;
 
 struct RouteBalanced {
@@ -34,9 +36,10 @@ struct RouteBalanced {
   int* ids;
   float* w;
   int *counts, *offsets, *row_of, *src_token;
-  uint16_t* tile_counts;   // [E][tiles_ld]
+  uint16_t* tile_counts;   // [tiles][E, rounded up to an even number]
   long long ld;
-  int T, E, top, groups, keep, group_best, renorm, sigmoid, bf16, e_first, e_count, per_tile, tiles, tiles_ld;
+  uint32_t per_inverse;    // 2^32 over the experts of a group, rounded up: e * per_inverse >> 32 is the group of e < 512 (more than one of them)
+  int T, E, top, groups, keep, group_best, renorm, sigmoid, bf16, e_first, e_count, per_tile, tiles;
   float scale;
 };
 
@@ -45,44 +48,62 @@ __device__ __forceinline__ unsigned long long rb_key(double v) {
   const long long b = __double_as_longlong(v);
   return (unsigned long long)b ^ (b < 0 ? ~0ull : 1ull << 63);
 }
-__device__ __forceinline__ double rb_clamp(double v) { return v != v ? -3e38 : fmin(fmax(v, -3e38), 3e38); }
+// (fmaxf gives its other operand for one that is not a number)
+__device__ __forceinline__ float rb_clamp(float v) { return fminf(fmaxf(v, -3e38f), 3e38f); }
+__device__ __forceinline__ double rb_max(double a, double b) { return a > b ? a : b; }
+__device__ __forceinline__ double rb_min(double a, double b) { return a > b ? b : a; }
 
-// The lane whose key is the largest, ties to the lowest index; idx of the winner on every lane (keys of 0 are no candidates).
-__device__ __forceinline__ int rb_argmax(unsigned long long key, int idx) {
-  const unsigned hi = (unsigned)(key >> 32);
-  const unsigned mh = __reduce_max_sync(0xffffffffu, hi);
+// The lane whose key is the largest, the lowest of several.
+__device__ __forceinline__ int rb_first(unsigned long long key) {
+  const unsigned hi = (unsigned)(key >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
   unsigned who = __ballot_sync(0xffffffffu, hi == mh);
   if (who & (who - 1)) {
-    const unsigned lo = hi == mh ? (unsigned)key : 0u;
-    const unsigned ml = __reduce_max_sync(0xffffffffu, lo);
-    return (int)__reduce_min_sync(0xffffffffu, hi == mh && lo == ml ? (unsigned)idx : 0x7fffffffu);
+    const unsigned lo = hi == mh ? (unsigned)key : 0u, ml = __reduce_max_sync(0xffffffffu, lo);
+    who = __ballot_sync(0xffffffffu, hi == mh && lo == ml);
   }
-  return __shfl_sync(0xffffffffu, idx, __ffs(who) - 1);
+  return __ffs(who) - 1;
+}
+// Descending order of N (a power of two) keys: merges of ever longer runs, the second of two turned round.
+template <int N>
+__device__ __forceinline__ void rb_sort(unsigned long long (&k)[N]) {
+#pragma unroll
+  for (int run = 2; run <= N; run *= 2)
+#pragma unroll
+    for (int hop = run / 2; hop > 0; hop /= 2)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int j = hop == run / 2 ? (i & ~(run - 1)) + run - 1 - (i & (run - 1)) : i ^ hop;
+        if (j <= i) continue;
+        const bool turn = k[j] > k[i];
+        const unsigned long long a = turn ? k[j] : k[i], b = turn ? k[i] : k[j];
+        k[i] = a;
+        k[j] = b;
+      }
 }
 
-// A warp's token: ids and weights to global memory, the tile's bit of every chosen expert. pool: E doubles of this warp.
+__device__ __forceinline__ double rb_logit(const RouteBalanced& p, int t, int e) {
+  const size_t at = (size_t)t * p.ld + e;
+  return (double)rb_clamp(p.bf16 ? __bfloat162float(((const __nv_bfloat16*)p.logits)[at]) : ((const float*)p.logits)[at]);
+}
+
+// A warp's token: ids and weights to global memory, the tile's bit of every chosen expert. pool: 32 PER doubles of this warp.
 template <int PER>
 __device__ __forceinline__ void rb_token(const RouteBalanced& p, int t, int slot, double* pool, uint32_t* masks, int words) {
   const int lane = threadIdx.x & 31;
-  double s[PER], mx = -3e38;
+  double s[PER], mx = (double)-3e38f, den = 1.0;
   unsigned long long key[PER];
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
     const int e = q * 32 + lane;
-    s[q] = 0.0;
-    if (e < p.E) {
-      const size_t at = (size_t)t * p.ld + e;
-      const float z = p.bf16 ? __bfloat162float(((const __nv_bfloat16*)p.logits)[at]) : ((const float*)p.logits)[at];
-      s[q] = rb_clamp((double)z);
-      mx = fmax(mx, s[q]);
-    }
+    s[q] = e < p.E ? rb_logit(p, t, e) : (double)-3e38f;
+    mx = rb_max(mx, s[q]);
   }
   if (p.sigmoid) {
 #pragma unroll
     for (int q = 0; q < PER; ++q) s[q] = 1.0 / (1.0 + exp(-s[q]));
   } else {
-    for (int o = 16; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    double den = 0.0;
+    for (int o = 16; o > 0; o >>= 1) mx = rb_max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    den = 0.0;
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
       s[q] = q * 32 + lane < p.E ? exp(s[q] - mx) : 0.0;
@@ -95,62 +116,102 @@ __device__ __forceinline__ void rb_token(const RouteBalanced& p, int t, int slot
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
     const int e = q * 32 + lane;
-    const double c = e < p.E ? rb_clamp(p.bias != nullptr ? s[q] + (double)p.bias[e] : s[q]) : 0.0;
-    key[q] = e < p.E ? rb_key(c) : 0ull;
-    if (p.keep < p.groups && e < p.E) pool[e] = c;
+    key[q] = 0ull;
+    if (e < p.E) {
+      const double c = p.bias != nullptr ? s[q] + (double)rb_clamp(p.bias[e]) : s[q];
+      key[q] = (rb_key(c) & ~15ull) | (unsigned)(15 - q);
+      if (p.keep < p.groups) pool[e] = c;
+    }
   }
   if (p.keep < p.groups) {
     __syncwarp();
     const int per = p.E / p.groups;
     unsigned long long worth[RB_MAX_GROUPS / 32], kept = 0;
+    worth[0] = worth[1] = 0ull;
+    // Lanes of a group: as many as there are for all groups. They take its members in turn, each group from another place on (neighbouring groups begin in
+    // the same bank), and join their two best.
+    int share_log = 5;
+    while (share_log > 0 && p.groups << share_log > 32) --share_log;
+    const int share = 1 << share_log;
+    const int sub = lane & (share - 1), turns = (per + share - 1) >> share_log;
 #pragma unroll
     for (int h = 0; h < RB_MAX_GROUPS / 32; ++h) {
-      const int grp = h * 32 + lane;
-      worth[h] = 0ull;
+      if (h * 32 >= p.groups) break;
+      const int grp = h * 32 + (lane >> share_log);
+      double b1 = -INFINITY, b2 = -INFINITY;
       if (grp < p.groups) {
-        double b1 = -INFINITY, b2 = -INFINITY;
-        for (int i = 0; i < per; ++i) {
-          const double c = pool[grp * per + i];
-          if (c > b1) { b2 = b1; b1 = c; }
-          else if (c > b2) b2 = c;
+        int k = grp % turns;
+        for (int n = 0; n < turns; ++n) {
+          const int i = k * share + sub;
+          if (++k == turns) k = 0;
+          const double c = i < per ? pool[grp * per + i] : -INFINITY;
+          b2 = rb_max(b2, rb_min(b1, c));
+          b1 = rb_max(b1, c);
         }
-        worth[h] = rb_key(p.group_best > 1 && per > 1 ? b1 + b2 : b1);
       }
+      for (int o = 1; o < share; o <<= 1) {
+        const double c1 = __shfl_xor_sync(0xffffffffu, b1, o), c2 = __shfl_xor_sync(0xffffffffu, b2, o);
+        b2 = rb_max(rb_max(b2, c2), rb_min(b1, c1));
+        b1 = rb_max(b1, c1);
+      }
+      // (to lane grp % 32, which owns the group from here on)
+      const unsigned long long v = grp < p.groups ? rb_key(p.group_best > 1 && per > 1 ? b1 + b2 : b1) : 0ull;
+      const unsigned long long mine = __shfl_sync(0xffffffffu, v, (lane * share) & 31);
+      worth[h] = h * 32 + lane < p.groups ? mine : 0ull;
     }
     for (int k = 0; k < p.keep; ++k) {
-      const bool up = p.groups > 32 && worth[1] > worth[0];       // the lower group where both are equal
-      const int got = rb_argmax(up ? worth[1] : worth[0], up ? 32 + lane : lane);
+      // the lower group where two are equal: of a lane's two the first, of several lanes' first ones the lowest before any second one
+      const unsigned long long first = worth[0], second = p.groups > 32 ? worth[1] : 0ull;
+      const int l = rb_first(first > second ? first : second);
+      const bool up = __shfl_sync(0xffffffffu, first >= second ? 0 : 1, l);
+      int got = l + (up ? 32 : 0);
+      if (p.groups > 32) {
+        const unsigned long long best = __shfl_sync(0xffffffffu, first > second ? first : second, l);
+        const unsigned in_first = __ballot_sync(0xffffffffu, first == best);
+        if (in_first) got = __ffs(in_first) - 1;
+      }
       kept |= 1ull << got;
-      if ((got & 31) == lane) worth[got >> 5] = 0ull;
+      if (got == lane) worth[0] = 0ull;
+      if (got == lane + 32) worth[1] = 0ull;
     }
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
       const int e = q * 32 + lane;
-      if (e < p.E && !((kept >> (e / per)) & 1ull)) key[q] = 0ull;
+      const int of = per == 1 ? e : (int)__umulhi(e, p.per_inverse);
+      if (e < p.E && !((kept >> of) & 1ull)) key[q] = 0ull;
     }
-    __syncwarp();                // the pool is free for the warp's next token
   }
-  int my_id = 0;
-  double my_s = 0.0, sum = 0.0;
+  rb_sort<PER>(key);
+  __syncwarp();                // the pool's choices are read
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(pool);
+#pragma unroll
+  for (int q = 1; q < PER; ++q) list[q * 32 + lane] = key[q];
+  unsigned long long head = key[0];
+  int next = 1, my_id = 0;
   for (int j = 0; j < p.top; ++j) {
-    unsigned long long best = key[0];
-    int bq = 0;
-#pragma unroll
-    for (int q = 1; q < PER; ++q) if (key[q] > best) { best = key[q]; bq = q; }
-    const int e = rb_argmax(best, bq * 32 + lane);
-    double mine = 0.0;
-#pragma unroll
-    for (int q = 0; q < PER; ++q) if (q * 32 + lane == e) { mine = s[q]; key[q] = 0ull; }
-    const double got = __shfl_sync(0xffffffffu, mine, e & 31);
-    sum += got;
-    if (lane == j) { my_id = e; my_s = got; }
+    const int l = rb_first(head);
+    const int e = (15 - (int)(__shfl_sync(0xffffffffu, (unsigned)head, l) & 15u)) * 32 + l;
+    if (lane == l) {
+      head = next < PER ? list[next * 32 + lane] : 0ull;
+      ++next;
+    }
+    if (lane == j) my_id = e;
   }
+  // the chosen scores, once more from the logits
+  double mine = 0.0;
+  if (lane < p.top) {
+    const double z = rb_logit(p, t, my_id);
+    mine = p.sigmoid ? 1.0 / (1.0 + exp(-z)) : exp(z - mx) / den;
+  }
+  double sum = mine;
+  for (int o = 1; o < RB_MAX_TOP; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane < p.top) {
     const size_t at = (size_t)t * p.top + lane;
     p.ids[at] = my_id;
-    p.w[at] = (float)(my_s * (double)p.scale / (p.renorm ? sum + 1e-20 : 1.0));
+    p.w[at] = (float)(mine * (double)p.scale / (p.renorm ? sum + 1e-20 : 1.0));
     atomicOr(&masks[my_id * words + (slot >> 5)], 1u << (slot & 31));
   }
+  __syncwarp();                // the pool is free for the warp's next token
 }
 
 // Exclusive sums of total[0 .. E) into off[0 .. E], by the first warp.
@@ -198,7 +259,7 @@ __global__ void __launch_bounds__(1024) route_balanced_cluster_kernel(const Rout
   pdl_trigger();
   pdl_wait();
   __syncthreads();
-  if (warp < n_tokens) rb_token<PER>(p, t0 + warp, warp, pool + (size_t)warp * p.E, masks, 1);
+  if (warp < n_tokens) rb_token<PER>(p, t0 + warp, warp, pool + (size_t)warp * PER * 32, masks, 1);
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) cnt[e] = e >= p.e_first && e < p.e_first + p.e_count ? __popc(masks[e]) : 0;
   if (n > 1) cluster.sync(); else __syncthreads();
@@ -227,21 +288,22 @@ __global__ void __launch_bounds__(1024) route_balanced_cluster_kernel(const Rout
 
 // Many tokens, first kernel: the choices of a tile, its counts and, in row_of, the pairs' places among the tile's.
 template <int PER>
-__global__ void __launch_bounds__(512) route_balanced_tile_kernel(const RouteBalanced p) {
+__global__ void __launch_bounds__(1024) route_balanced_tile_kernel(const RouteBalanced p) {
   extern __shared__ double pool[];
   const int words = (p.per_tile + 31) / 32, n_warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-  uint32_t* masks = reinterpret_cast<uint32_t*>(pool + (size_t)n_warps * p.E);
+  uint32_t* masks = reinterpret_cast<uint32_t*>(pool + (size_t)n_warps * PER * 32);
   const int t0 = blockIdx.x * p.per_tile, n_tokens = max(0, min(p.per_tile, p.T - t0));
   for (int i = threadIdx.x; i < p.E * words; i += blockDim.x) masks[i] = 0u;
   pdl_wait();
   __syncthreads();
-  for (int i = warp; i < n_tokens; i += n_warps) rb_token<PER>(p, t0 + i, i, pool + (size_t)warp * p.E, masks, words);
+  for (int i = warp; i < n_tokens; i += n_warps) rb_token<PER>(p, t0 + i, i, pool + (size_t)warp * PER * 32, masks, words);
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
     int c = 0;
     for (int w = 0; w < words; ++w) c += __popc(masks[e * words + w]);
-    p.tile_counts[(size_t)e * p.tiles_ld + blockIdx.x] = (uint16_t)(e >= p.e_first && e < p.e_first + p.e_count ? c : 0);
+    p.tile_counts[(size_t)blockIdx.x * ((p.E + 1) & ~1) + e] = (uint16_t)(e >= p.e_first && e < p.e_first + p.e_count ? c : 0);
   }
+  if ((p.E & 1) && threadIdx.x == 0) p.tile_counts[(size_t)blockIdx.x * (p.E + 1) + p.E] = 0;
   for (int i = threadIdx.x; i < n_tokens * p.top; i += blockDim.x)
     p.row_of[(size_t)t0 * p.top + i] = rb_rank(masks, words, p.ids[(size_t)t0 * p.top + i], i / p.top);
   pdl_trigger();
@@ -249,25 +311,25 @@ __global__ void __launch_bounds__(512) route_balanced_tile_kernel(const RouteBal
 
 // Second kernel: the tiles' counts become bases, the places become rows.
 __global__ void __launch_bounds__(512) route_balanced_place_kernel(const RouteBalanced p) {
-  __shared__ int base[RB_MAX_E], total[RB_MAX_E], off[RB_MAX_E + 1];
+  __shared__ int base[RB_MAX_E + 1], total[RB_MAX_E + 1], off[RB_MAX_E + 1];
+  const int tile = blockIdx.x, words = (p.E + 1) / 2, parts = blockDim.x / words;      // (at most 256 words)
+  for (int e = threadIdx.x; e <= p.E; e += blockDim.x) base[e] = total[e] = 0;
+  __syncthreads();
   pdl_wait();
-  const int tile = blockIdx.x;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    const uint4* row = reinterpret_cast<const uint4*>(p.tile_counts + (size_t)e * p.tiles_ld);   // eight tiles each
-    int before = 0, all = 0;
-    for (int b = 0; b * 8 < p.tiles; ++b) {
-      const uint4 v = row[b];
-      const uint32_t r[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = b * 8 + i;
-        const int c = at < p.tiles ? (int)((r[i >> 1] >> (16 * (i & 1))) & 0xffffu) : 0;
-        before += at < tile ? c : 0;
-        all += c;
-      }
+  // two experts per thread, the tiles dealt over the parts of the block
+  const int w = threadIdx.x % words, part = threadIdx.x / words;
+  if (part < parts) {
+    const uint32_t* at = reinterpret_cast<const uint32_t*>(p.tile_counts) + w;
+    int before[2] = {0, 0}, all[2] = {0, 0};
+#pragma unroll 8
+    for (int i = part; i < p.tiles; i += parts) {
+      const uint32_t v = at[(size_t)i * words];
+      const int lo = (int)(v & 0xffffu), hi = (int)(v >> 16);
+      all[0] += lo; all[1] += hi;
+      if (i < tile) { before[0] += lo; before[1] += hi; }
     }
-    base[e] = before;
-    total[e] = all;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) { atomicAdd(&base[2 * w + k], before[k]); atomicAdd(&total[2 * w + k], all[k]); }
   }
   __syncthreads();
   if (threadIdx.x < 32) rb_scan(total, off, p.E);
@@ -295,7 +357,7 @@ __global__ void route_balanced_empty_kernel(const RouteBalanced p) {
 
 static int rb_tiles(int T, int* per_tile) {
   int per = RB_TILE;
-  if ((T + per - 1) / per > RB_MAX_TILES) per = ((T + RB_MAX_TILES - 1) / RB_MAX_TILES + 31) / 32 * 32;
+  if ((T + per - 1) / per > RB_MAX_TILES) per = (T + RB_MAX_TILES - 1) / RB_MAX_TILES;
   *per_tile = per;
   return (T + per - 1) / per;
 }
@@ -306,7 +368,7 @@ static int rb_launch(RouteBalanced p, cudaStream_t s) {
     static PerDevice allowed;
     const int n = p.T <= 8 ? 1 : RB_CLUSTER;
     p.per_tile = (p.T + n - 1) / n;
-    const size_t smem = p.keep < p.groups ? (size_t)p.per_tile * p.E * sizeof(double) : 0;
+    const size_t smem = (size_t)p.per_tile * PER * 32 * sizeof(double);
     if (smem > 36 * 1024) {
       const cudaError_t e = allow_smem(allowed, (const void*)route_balanced_cluster_kernel<PER>, 32 * RB_MAX_E * (int)sizeof(double));
       if (e != cudaSuccess) return (int)e;
@@ -329,10 +391,9 @@ static int rb_launch(RouteBalanced p, cudaStream_t s) {
   }
   static PerDevice allowed;
   p.tiles = rb_tiles(p.T, &p.per_tile);
-  p.tiles_ld = (p.tiles + 7) / 8 * 8;
-  const int words = (p.per_tile + 31) / 32, warps = 16;
-  const size_t smem = (size_t)warps * p.E * sizeof(double) + (size_t)p.E * words * 4;
-  cudaError_t e = allow_smem(allowed, (const void*)route_balanced_tile_kernel<PER>, 16 * RB_MAX_E * (int)sizeof(double) + RB_MAX_E * RB_MAX_WORDS * 4);
+  const int words = (p.per_tile + 31) / 32, warps = 32;
+  const size_t smem = (size_t)warps * PER * 32 * sizeof(double) + (size_t)p.E * words * 4;
+  cudaError_t e = allow_smem(allowed, (const void*)route_balanced_tile_kernel<PER>, 32 * PER * 32 * (int)sizeof(double) + PER * 32 * RB_MAX_WORDS * 4);
   if (e != cudaSuccess) return (int)e;
   e = launch_pdl(route_balanced_tile_kernel<PER>, dim3(p.tiles), dim3(32 * warps), smem, s, p);
   if (e != cudaSuccess) return (int)e;
@@ -347,7 +408,7 @@ extern "C" long long skein_route_balanced_scratch(int T, int E) {
   if (T <= RB_CLUSTER_TOKENS) return 0;
   int per;
   const int tiles = rb_tiles(T, &per);
-  return per > RB_MAX_WORDS * 32 ? -1 : (long long)E * ((tiles + 7) / 8 * 8) * 2;
+  return per > RB_MAX_WORDS * 32 ? -1 : (long long)tiles * ((E + 1) & ~1) * 2;
 }
 
 // logits [T, ld] fp32 or bf16 (bf16 != 0); bias [E] fp32 or null. ids / w [T, top], counts [E], offsets [E + 1], row_of / src_token [T * top].
@@ -359,8 +420,8 @@ extern "C" int skein_route_balanced(const void* logits, long long ld, int bf16, 
       keep > groups || top > keep * (E / groups) || group_best < 1 || group_best > 2 || e_first < 0 || e_count < 0 || e_first + e_count > E)
     return -1;
   if (skein_route_balanced_scratch(T, E) < 0 || (skein_route_balanced_scratch(T, E) > 0 && scratch == nullptr)) return -2;
-  RouteBalanced p{logits, bias, ids, w, counts, offsets, row_of, src_token, (uint16_t*)scratch, ld, T, E, top, groups, keep, group_best, renorm, sigmoid, bf16,
-                  e_first, e_count, 0, 0, 0, scale};
+  RouteBalanced p{logits, bias, ids, w, counts, offsets, row_of, src_token, (uint16_t*)scratch, ld, (uint32_t)((0x100000000ull + E / groups - 1) / (E / groups)), T, E, top, groups, keep, group_best, renorm, sigmoid, bf16,
+                  e_first, e_count, 0, 0, scale};
   cudaStream_t s = (cudaStream_t)stream;
   if (T == 0) {
     route_balanced_empty_kernel<<<1, 256, 0, s>>>(p);

@@ -39,8 +39,7 @@ def select_balanced(logits, top, bias, groups, keep, score, group_best, renorm, 
     z = logits.double()
     z = torch.where(z == z, z, torch.full_like(z, -3e38)).clamp(-3e38, 3e38)
     s = torch.sigmoid(z) if score == "sigmoid" else torch.softmax(z, 1)
-    c = s if bias is None else s + bias.double()
-    c = torch.where(c == c, c, torch.full_like(c, -3e38)).clamp(-3e38, 3e38)
+    c = s if bias is None else s + torch.where(bias == bias, bias, torch.full_like(bias, -3e38)).clamp(-3e38, 3e38).double()
     if keep < groups:
         per = E // groups
         worth = c.view(T, groups, per).sort(dim=2, descending=True).values[:, :, :min(group_best, per)].sum(2)

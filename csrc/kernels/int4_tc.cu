@@ -169,24 +169,15 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   const bool live = first < total;           // the same for every CTA of a cluster
   uint64_t acc[S::EPI_COLS / 2];             // two columns each
   const bool pair = p.flags & 1, f32 = p.flags & 4;
-  // stores two columns of the result; of a pair the gate's lane finishes the first and the up's the second
-  auto finish = [&](const Tile& tl, int col, float a, float b) {
-    const int r = (warp & 3) * 32 + lane, f = pair ? (tl.m * 8 + (r >> 4)) * 8 + (r & 7) : tl.m * 128 + r;
-    auto store = [&](int c, float y) {
-      const size_t at = (size_t)(tl.row0 + c) * p.out_ld + f;
-      if (f32) ((float*)p.out)[at] = p.residual ? y + ((const float*)p.residual)[at] : y;
-      else ((__nv_bfloat16*)p.out)[at] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[at]) : y);
-    };
-    if (!pair) {
-      if (f < p.F && col < tl.valid) store(col, a);
-      if (f < p.F && col + 1 < tl.valid) store(col + 1, b);
-    } else {
-      const bool up = r & 8;
-      const float other = __shfl_xor_sync(0xffffffffu, up ? a : b, 8);
-      const int c = up ? col + 1 : col;
-      const float y = up ? silu(other) * b : silu(a) * other;
-      if (f < p.F && c < tl.valid) store(c, y);
-    }
+  auto store = [&](size_t at, float y) {
+    if (f32) ((float*)p.out)[at] = p.residual ? y + ((const float*)p.residual)[at] : y;
+    else ((__nv_bfloat16*)p.out)[at] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[at]) : y);
+  };
+  // Of a pair the gate's lane finishes the first of two columns and the up's the second.
+  auto of_pair = [&](float a, float b) {
+    const bool up = lane & 8;
+    const float other = __shfl_xor_sync(0xffffffffu, up ? a : b, 8), g = up ? other : a, u = up ? b : other;
+    return silu(g) * u;
   };
 
   if (live) {
@@ -402,9 +393,37 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
         }
         if (!ok || p.split > 1) break;
         const Tile tl = tile_at(u, e);
+        // (MMAs of the next tile wait for these warps once the accumulators are full: what is the same for all columns stays out of the loops)
+        const int f = pair ? (tl.m * 8 + (r >> 4)) * 8 + (r & 7) : tl.m * 128 + r, mine = pair ? (lane >> 3) & 1 : 0;
+        const int left = f < p.F ? tl.valid - col0 - mine : 0;
+        const size_t at = (size_t)(tl.row0 + col0 + mine) * p.out_ld + f;
+        if (pair) {
+          __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
 #pragma unroll
-        for (int c = 0; c < S::EPI_COLS; c += 2)
-          if (col0 + c < tl.valid) { const float2 v = it_unpack(acc[c / 2]); finish(tl, col0 + c, v.x, v.y); }
+          for (int c = 0; c < S::EPI_COLS; c += 2) {
+            const float2 v = it_unpack(acc[c / 2]);
+            const float y = of_pair(v.x, v.y);
+            if (c < left) *to = __float2bfloat16(y);
+            to += 2 * p.out_ld;
+          }
+        } else if (!f32 && p.residual == nullptr) {
+          __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
+#pragma unroll
+          for (int c = 0; c < S::EPI_COLS; c += 2) {
+            const float2 v = it_unpack(acc[c / 2]);
+            if (c < left) *to = __float2bfloat16(v.x);
+            to += p.out_ld;
+            if (c + 1 < left) *to = __float2bfloat16(v.y);
+            to += p.out_ld;
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < S::EPI_COLS; c += 2) {
+            const float2 v = it_unpack(acc[c / 2]);
+            if (c < left) store(at + (size_t)c * p.out_ld, v.x);
+            if (c + 1 < left) store(at + (size_t)(c + 1) * p.out_ld, v.y);
+          }
+        }
       }
     }
   }
@@ -436,7 +455,15 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
           a += recv[(q * slice + c) * 128 + r];
           b += recv[(q * slice + c + 1) * 128 + r];
         }
-        finish(tl, rank * slice + c, a, b);
+        const int col = rank * slice + c, f = pair ? (tl.m * 8 + (r >> 4)) * 8 + (r & 7) : tl.m * 128 + r;
+        if (pair) {
+          const float y = of_pair(a, b);
+          const int own = col + ((lane >> 3) & 1);
+          if (f < p.F && own < tl.valid) store((size_t)(tl.row0 + own) * p.out_ld + f, y);
+        } else if (f < p.F) {
+          store((size_t)(tl.row0 + col) * p.out_ld + f, a);
+          if (col + 1 < tl.valid) store((size_t)(tl.row0 + col + 1) * p.out_ld + f, b);
+        }
       }
     }
   }

@@ -6,8 +6,12 @@
 // K) with two 16-byte loads per lane, turns the codes into bf16 (exact, nine instructions per word of eight) and multiplies them
 // with mma.sync m16n8k16 against eight rows of x in shared memory. A group's sum is fp32 and is scaled in fp32, so nothing is rounded before the result.
 // A CTA per SM stays for the launch. WK of its 16 warps make a team that shares the K of a strip (a warp every WK-th step) and walks its run of strips;
-// the loads of the next four steps, the next strip's among them, are always on their way, and the team's sums meet in shared memory in warp order while
-// they are. The runs are equal shares of all strips that some row goes to, whatever expert they belong to.
+// the loads of the next four steps, the next strip's among them, are always on their way. The team's sums meet in shared memory and are added up in warp order
+// a strip later, so that no warp waits for the slowest. The runs are equal shares of all strips that some row goes to, whatever expert they belong to.
+// What bounds it: the instructions. A step of a strip is about 150 of them, 72 for the codes and 8 products, and the 16 warps that the registers leave
+// room for issue half of the cycles (28672 x 8192 gate / up, one row: 63 us, 3.9 TB/s, where HBM would take 38). Tried and not kept: the codes as
+// subnormal operands of the products without a multiply-add, with scaled rows of x and their sums for the zeros (63 us, but 232 against 139 for 13 rows
+// of 152064 x 3584); two strips per warp (62 and 182); a ring in shared memory filled with cp.async (72 and 148).
 #include "int4.cuh"
 #include "launch.cuh"
 

@@ -247,7 +247,7 @@ def _dense(what, x, w, out, residual, out_f32, cfg):
 
 def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None, out=None, rows_hint=None, _cfg=None):
     """Per-expert linear over expert-sorted rows. counts / offsets are int32 device tensors of E (offsets may have E + 1) entries: rows of expert e are
-    offsets[e] : offsets[e] + counts[e] of the result. They read the same rows of x, or with src_row (int32, one entry per row of the result) rows
+    offsets[e] : offsets[e] + counts[e] of the result, no row belongs to two. They read the same rows of x, or with src_row (int32, one entry per row of the result) rows
     src_row[r]: the tokens themselves, without a sorted copy. Rows not covered by any expert are left untouched (uninitialised in a result that the call
     makes). rows_hint: rows expected over all experts, of which the choice of kernel depends (default: all of the result's)."""
     what = "int4 grouped_linear"

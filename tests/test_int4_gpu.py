@@ -195,6 +195,94 @@ def test_same_bits_twice_and_on_two_streams():
         assert all(torch.equal(y, z) for g in got for z in g)
 
 
+@pytest.mark.parametrize("cfg, rows, features, K, group", [((16, 1), 16, 128 * 301, 256, 64), ((32, 1), 40, 128 * 150, 128, 32), ((64, 1), 129, 128 * 101, 384, 128),
+                                                           ((128, 1), 400, 128 * 41, 128, 64), ((128, 1), 300, 128 * 60, 256, 32), (None, 500, 9000, 192, 64), (None, 17, 40000, 128, 128)])
+def test_more_tiles_than_places(cfg, rows, features, K, group):
+    """Every CTA walks several tiles: what one leaves (accumulators, slots, stages) the next finds in order."""
+    w, full = weight((), features, K, group, True, torch.float16, False)
+    x = acts(rows, K)
+    within(int4.linear(x, w, out_f32=True, _cfg=cfg), x, full, half_step=2.0 ** -24)
+    w, full = weight((), 2 * (features // 3), K, group, False, torch.bfloat16, True)
+    within(int4.swiglu_linear(x, w, _cfg=cfg), x, full, True)
+    ops.workspace().check_status()
+
+
+@pytest.mark.parametrize("cfg", [None, (16, 1), (128, 1), (0, 0)])
+def test_many_uneven_experts(cfg):
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    counts = torch.randint(0, 40, (90,), generator=gen, device=DEV, dtype=torch.int32)
+    counts[::7] = 0
+    off = torch.cat((counts.new_zeros(1), counts.cumsum(0))).to(torch.int32)
+    n = int(off[-1])
+    w, full = weight((90,), 300, 160, 32, True, torch.bfloat16, False)
+    x, src = acts(64, 160), torch.randint(0, 64, (n,), generator=gen, device=DEV, dtype=torch.int32)
+    y = int4.grouped_linear(x, w, counts, off, src_row=src, _cfg=cfg)
+    expert = torch.repeat_interleave(torch.arange(90, device=DEV), counts.long())
+    for e in range(90):
+        mine = expert == e
+        if bool(mine.any()):
+            within(y[mine], x[src[mine].long()], full[e])
+    ops.workspace().check_status()
+
+
+@pytest.mark.parametrize("cfg", [(0, 0), (16, 1), (64, 1)])
+def test_experts_beyond_31_bits(cfg):
+    """The last expert's codes lie more than 2^31 bytes into the weight."""
+    one, full = weight((1,), 512, 8192, 128, False, torch.bfloat16, False)
+    E = (1 << 31) // one.data[0].numel() + 2
+    if E > int4.MAX_EXPERTS:
+        E = int4.MAX_EXPERTS
+    data = torch.zeros(E, *one.data.shape[1:], dtype=torch.uint8, device=DEV)
+    data[-1].copy_(one.data[0])
+    assert (E - 1) * one.data[0].numel() >= 1 << 31
+    w = int4.Int4Weight(data, (E, 512, 8192), 128, False, torch.bfloat16, False)
+    x = acts(20, 8192)
+    counts = torch.zeros(E, dtype=torch.int32, device=DEV)
+    counts[-1] = 20
+    y = int4.grouped_linear(x, w, counts, torch.zeros_like(counts), _cfg=cfg)
+    within(y, x, full[0])
+
+
+def test_two_graphs_at_once():
+    """Captured products and routers share nothing: replayed at once on two streams they give what they give one after another."""
+    x = [acts(48, 512, seed=s) for s in (1, 2)]
+    w, _ = weight((16,), 2 * 192, 512, 64, True, torch.bfloat16, True)
+    d, _ = weight((), 4096, 2048, 128, False, torch.bfloat16, False)
+    wide = [acts(30, 2048, seed=s) for s in (3, 4)]
+    wg = torch.randn(16, 512, device=DEV).bfloat16()
+    graphs, outs = [], []
+    for i in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            def step():
+                logits = x[i].float() @ wg.float().t()
+                ids, rw, counts, offsets, row_of, src = experts.route_balanced(logits, 2)
+                return int4.grouped_linear(x[i], w, counts, offsets, swiglu=True, src_row=src), int4.linear(wide[i], d, out_f32=True), ids, row_of
+            step()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(step())
+        graphs.append((g, side))
+        torch.cuda.synchronize()
+    for g, _ in graphs:
+        g.replay()
+        torch.cuda.synchronize()
+    want = [[t.clone() for t in o] for o in outs]
+    for o in outs:
+        for t in o:
+            t.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, side in graphs:
+            with torch.cuda.stream(side):
+                g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(want, outs):
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)
+
+
 # ---- choice of experts ------------------------------------------------------------------------------------------------
 ROUTES = [  # tokens, experts, top, groups, keep, group_best, score, renorm
     (1, 1, 1, 1, 1, 2, "softmax", True), (1, 128, 8, 1, 1, 2, "softmax", True), (5, 33, 4, 1, 1, 1, "sigmoid", False), (64, 64, 6, 8, 4, 2, "sigmoid", True),

@@ -44,20 +44,20 @@ def route_balanced(logits, top, bias=None, groups=1, keep=1, score="sigmoid", gr
         raise ValueError("route_balanced: bias must be fp32 [experts] on the logits' device")
     if not logits.is_cuda:
         return ri.route_balanced(logits, top, bias, groups, keep, score, group_best, renorm, scale, e_first, e_count)
+    dev, n = logits.device, T * top
     with _lib.on_device(logits):
-        L, dev, n = _lib.lib(), logits.device, T * top
+        L = _lib.lib()
         need = L.skein_route_balanced_scratch(T, E) if T > ONE_LAUNCH else 0
         if need < 0:
             raise ValueError(f"route_balanced: {T} tokens are more than one call takes")
-        ids = torch.empty((T, top), dtype=torch.int32, device=dev)
-        w = torch.empty((T, top), dtype=torch.float32, device=dev)
-        meta = torch.empty(2 * E + 1 + 2 * n, dtype=torch.int32, device=dev)
         scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        at = meta.data_ptr()
+        buf = torch.empty(4 * n + 2 * E + 1, dtype=torch.int32, device=dev)      # all results: an allocation costs more than a view
+        at = buf.data_ptr()
         rc = L.skein_route_balanced(
             logits.data_ptr(), logits.stride(0), dtype == torch.bfloat16, None if bias is None else bias.data_ptr(), T, E, top, groups, keep, group_best,
-            renorm, score == "sigmoid", scale, e_first, e_count, ids.data_ptr(), w.data_ptr(), at, at + 4 * E, at + 4 * (2 * E + 1),
-            at + 4 * (2 * E + 1 + n), scratch.data_ptr() if need else None, _lib.stream_on(dev))
-        _lib.check(rc, "route_balanced")
-        _lib.count_launch(2 if need else 1)
-    return (ids, w, *meta.split_with_sizes((E, E + 1, n, n)))
+            renorm, score == "sigmoid", scale, e_first, e_count, at, at + 4 * n, at + 8 * n, at + 8 * n + 4 * E, at + 8 * n + 8 * E + 4,
+            at + 12 * n + 8 * E + 4, scratch.data_ptr() if need else None, _lib.stream_on(dev))
+    _lib.check(rc, "route_balanced")
+    _lib.count_launch(2 if need else 1)
+    ids, w, counts, offsets, row_of, src_token = buf.split_with_sizes((n, n, E, E + 1, n, n))
+    return ids.view(T, top), w.view(torch.float32).view(T, top), counts, offsets, row_of, src_token

@@ -174,12 +174,9 @@ def _check(what, x, w: Int4Weight, pair, dims):
         raise ValueError(f"{what}: x is on {x.device}, the weight on {w.device}")
 
 
-def _out(what, out, rows, w, dtype, device):
-    if out is None:
-        return torch.empty((rows, w.features), dtype=dtype, device=device)
-    if out.shape != (rows, w.features) or out.dtype != dtype or out.device != device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
+def _check_out(what, out, rows, w, dtype):
+    if out.shape != (rows, w.features) or out.dtype != dtype or out.device != w.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
         raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
-    return out
 
 
 def _few_rows(hint: int, K: int) -> bool:
@@ -232,7 +229,11 @@ def swiglu_linear(x, w: Int4Weight, out=None, _cfg=None):
 
 def _dense(what, x, w, out, residual, out_f32, cfg):
     T = x.shape[0]
-    out = _out(what, out, T, w, torch.float32 if out_f32 else torch.bfloat16, x.device)
+    dtype = torch.float32 if out_f32 else torch.bfloat16
+    if out is None:
+        out = torch.empty((T, w.features), dtype=dtype, device=w.device)
+    else:
+        _check_out(what, out, T, w, dtype)
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
                                  or residual.stride(1) != 1 or (T > 1 and residual.stride(0) != out.stride(0))):
         raise ValueError(f"{what}: the residual must have the result's shape, type and strides")
@@ -259,7 +260,10 @@ def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None
     if src_row is not None and (src_row.dtype != torch.int32 or src_row.dim() != 1 or not src_row.is_contiguous() or src_row.device != x.device):
         raise ValueError(f"{what}: src_row must be int32 [rows] on x's device")
     rows = x.shape[0] if src_row is None else src_row.shape[0]
-    out = _out(what, out, rows, w, torch.bfloat16, x.device)
+    if out is None:
+        out = torch.empty((rows, w.features), dtype=torch.bfloat16, device=w.device)
+    else:
+        _check_out(what, out, rows, w, torch.bfloat16)
     if rows == 0:
         return out
     if x.shape[0] == 0:

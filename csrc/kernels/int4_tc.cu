@@ -2,8 +2,10 @@
 //
 // Weights are the M side (128 rows of a tile), NT rows of x the N side. A CTA walks tiles, or with few of them owns a piece of the K of one (the CTAs of
 // a cluster share the tile). Roles, one pipeline:
-//   producer    one bulk copy per step (codes, scales and zeros of 128 rows x 128 of K are one run) and TMA tiles of x, or of the rows that
-//               src_row names (tile::gather4), into a ring of shared-memory stages
+//   producer    one bulk copy per step (codes, scales and zeros of 128 rows x 128 of K are one run) and TMA tiles of x into a ring of shared-memory
+//               stages
+//   gatherers   two warps that copy the rows of x which src_row names, 16 bytes a lane (tile::gather4 takes 55 to 80 cycles for four rows of 128 bytes:
+//               it bounded experts at 250 us where these take 170)
 //   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (exact), 64 of K a slot, written to tensor
 //               memory as the A operand
 //   MMA         one thread; every group of K has an accumulator of its own (a ring of them)
@@ -12,9 +14,10 @@
 // but double the error of a product, and more for a gate / up pair.)
 // What bounds it: the handing over between the roles. A step (128 rows x 128 of K) takes a CTA about 1050 cycles whatever it holds; with the
 // conversion, the drains and seven of eight MMAs left out it still took 870. The MMAs of a step are 280 cycles with up to 64 rows of x and 512 with 128, the
-// weights' share of HBM is 365 cycles per SM. So with up to 64 rows two CTAs share an SM, handovers are whole steps, and tests of barriers are
-// issued before their answers are needed. Measured: 1000 rows of gate / up 37888 x 3584 248 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 478 us
-// (1.0 PFLOP/s), 13 rows of 152064 x 3584 100 us (3.1 TB/s).
+// weights' share of HBM is 365 cycles per SM. So with up to 64 rows two CTAs share an SM, with 16 rows two tiles of weights a step, handovers are whole
+// steps, and tests of barriers are issued before their answers are needed. Gathered rows are bounded by the two warps that copy them. Measured: 1000 rows of
+// gate / up 37888 x 3584 243 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 468 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 96 us (3.2 TB/s),
+// 128 rows over 8 experts of 28672 x 4096, gathered, 169 us (2.9 TB/s).
 // Pieces of a tile meet in distributed shared memory in rank order: the result does not depend on timing, and no memory outlives the call.
 #include "int4.cuh"
 #include "launch.cuh"
@@ -30,22 +33,25 @@ constexpr int IT_SCALES = 8;             // steps of the ring of scales
 constexpr int IT_BAND = 12;              // feature tiles of a band in which the row tiles run (L2 keeps a band's weights)
 
 struct Int4Tc {
+  const __nv_bfloat16* x;
   const int* src_row;
   const uint8_t* w;
   const void* residual;
   void* out;
   const int *counts, *offsets;
   int* status;
-  long long out_ld;
-  int rows, x_rows, E, F, K, strips, steps, m_tiles, split, stages, flags;   // flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros
+  long long x_ld, out_ld;
+  int rows, x_rows, E, F, K, strips, steps, w_tiles, m_tiles, split, stages, flags;   // flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros
   uint64_t budget_ns;
 };
 
-__device__ __forceinline__ void it_gather4(uint32_t dst, const void* tmap, uint32_t bar, int x, int r0, int r1, int r2, int r3) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+// 16 bytes of a gathered row; bytes = 0: zeros
+__device__ __forceinline__ void it_copy16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// The barrier hears of this thread's copies when they are complete: one arrival of its count.
+__device__ __forceinline__ void it_copy_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void it_copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // Bounded wait of a thread.
 __device__ __forceinline__ bool it_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t budget_ns) {
@@ -83,43 +89,44 @@ __device__ __forceinline__ float2 it_unpack(uint64_t a) {
   return r;
 }
 
-// shape of a launch
-template <int NT>
+// Shape of a launch. SUB: tiles of 128 weight rows that a CTA takes at a time.
+template <int NT, int SUB>
 struct ItShape {
-  static constexpr bool WIDE = NT == 128;                  // one CTA per SM, 512 columns; else two with 256 each
+  static constexpr bool ONE = NT == 128;                   // one CTA per SM, 512 columns; else two with 256 each
   static constexpr int CONV_WARPS = NT == 64 ? 4 : 8, EPI_WARPS = NT >= 64 ? 8 : 4;
-  static constexpr int THREADS = 32 * (4 + CONV_WARPS + EPI_WARPS);       // warps 0 and 1 produce and issue, 2 and 3 only align the quadrants
+  static constexpr int GROUPS = CONV_WARPS / 4 / SUB;      // of converters that take the steps in turn
+  static constexpr int THREADS = 32 * (4 + CONV_WARPS + EPI_WARPS);       // warp 0 produces, 1 issues, 2 and 3 gather
   static constexpr int ACC = NT;                           // columns of an accumulator
-  static constexpr int BUFS = WIDE ? 3 : NT == 16 ? 4 : 2;
-  static constexpr int SLOTS = NT == 16 || NT == 32 ? 3 : 2;       // of a converted step, 64 columns each
-  static constexpr int COLS = WIDE ? 512 : 256;
-  static constexpr int EPI_COLS = NT / (EPI_WARPS / 4);    // columns of an epilogue warp
+  static constexpr int BUFS = NT == 16 ? 4 : ONE ? 3 : 2;
+  static constexpr int SLOTS = SUB == 2 ? 1 : NT <= 32 ? 3 : 2;           // of a converted step, 64 columns for each tile
+  static constexpr int COLS = ONE ? 512 : 256;
+  static constexpr int EPI_COLS = NT / (EPI_WARPS / 4);    // columns that an epilogue warp takes, of every tile
   // Scales of the steps that are converted and not drained: a converter that writes those of step s + IT_SCALES has seen the MMAs of step s + IT_SCALES
   // - SLOTS done, which began after the epilogue had freed the accumulators of step s + IT_SCALES - SLOTS - BUFS, and had read their scales before
   static_assert(SLOTS + BUFS < IT_SCALES, "the ring of scales");
-  static_assert(BUFS * ACC + SLOTS * 64 <= COLS, "tensor memory");
+  static_assert(SUB * (BUFS * ACC + SLOTS * 64) <= COLS && GROUPS * 4 * SUB == CONV_WARPS, "tensor memory");
 };
 
-template <int NT, int GP>
-__global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Int4Tc p) {
+template <int NT, int GP, int SUB>
+__global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::ONE ? 1 : 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Int4Tc p) {
   namespace cg = cooperative_groups;
-  using S = ItShape<NT>;
+  using S = ItShape<NT, SUB>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[IT_MAX_STAGES], bar_empty[IT_MAX_STAGES], bar_cfull[S::SLOTS], bar_cempty[S::SLOTS], bar_dfull[S::BUFS], bar_dempty[S::BUFS];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
-  __shared__ float scales[IT_SCALES][GP][128];
+  __shared__ float scales[IT_SCALES][GP][SUB * 128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const bool zeros = p.flags & 8;
   const int rec = i4_record(GP, zeros);
   constexpr int X_BYTES = NT * 256;
-  const int stage_bytes = X_BYTES + ((rec + 1023) & ~1023);
+  const int w_bytes = (rec + 1023) & ~1023, stage_bytes = X_BYTES + SUB * w_bytes;
 
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int s = 0; s < p.stages; ++s) { mbar_init(smem_u32(&bar_full[s]), 1); mbar_init(smem_u32(&bar_empty[s]), 1); }
-    for (int s = 0; s < S::SLOTS; ++s) { mbar_init(smem_u32(&bar_cfull[s]), 4); mbar_init(smem_u32(&bar_cempty[s]), 1); }
+    for (int s = 0; s < p.stages; ++s) { mbar_init(smem_u32(&bar_full[s]), p.src_row != nullptr ? 65 : 1); mbar_init(smem_u32(&bar_empty[s]), 1); }
+    for (int s = 0; s < S::SLOTS; ++s) { mbar_init(smem_u32(&bar_cfull[s]), 4 * SUB); mbar_init(smem_u32(&bar_cempty[s]), 1); }
     for (int b = 0; b < S::BUFS; ++b) { mbar_init(smem_u32(&bar_dfull[b]), 1); mbar_init(smem_u32(&bar_dempty[b]), S::EPI_WARPS); }
     fence_mbar_init();
   }
@@ -170,7 +177,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
     return Tile{e, band * IT_BAND + rb - n * bm, off[e] + n * NT, min(NT, cnt[e] - n * NT)};
   };
   const bool live = first < total;           // the same for every CTA of a cluster
-  uint64_t acc[S::EPI_COLS / 2];             // two columns each
+  uint64_t acc[SUB][S::EPI_COLS / 2];        // two columns each
   const bool pair = p.flags & 1, f32 = p.flags & 4;
   auto store = [&](size_t at, float y) {
     if (f32) ((float*)p.out)[at] = p.residual ? y + ((const float*)p.residual)[at] : y;
@@ -186,57 +193,37 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   if (live) {
     if (warp == 0) {
       // ================= producer =================
-      if (lane == 0) tma_prefetch_desc(&tmX);
-      const uint64_t keep = l2_policy_evict_last();
-      int st = 0, e = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int u = first; u < total && ok; u += hop) {
-        const Tile tl = tile_at(u, e);
-        const uint8_t* w = p.w + ((size_t)tl.e * p.m_tiles + tl.m) * p.steps * rec;
-        // a lane's part of a gathered tile: four rows of a half, twice with 128 rows
-        constexpr int PARTS = NT == 128 ? 2 : 1;
-        int from[PARTS][4];
-        if (p.src_row != nullptr) {
-#pragma unroll
-          for (int i = 0; i < PARTS; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int at = ((lane + 32 * i) >> 1) * 4 + k;
-              int row = 0;
-              if (at < tl.valid) {
-                row = p.src_row[tl.row0 + at];
-                if (row < 0 || row >= p.x_rows) { report_status(p.status, ST_BAD_INDEX, row); row = 0; }
-              }
-              from[i][k] = row;
+      if (elect_one()) {
+        if (p.src_row == nullptr) tma_prefetch_desc(&tmX);
+        const uint64_t keep = l2_policy_evict_last();
+        int st = 0, e = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int u = first; u < total && ok; u += hop) {
+          const Tile tl = tile_at(u, e);
+          // (behind the last tile that one again, for nothing)
+          const uint8_t* w = p.w + ((size_t)tl.e * p.w_tiles + tl.m * SUB) * p.steps * rec;
+          const size_t second = tl.m * SUB + 1 < p.w_tiles ? (size_t)p.steps * rec : 0;
+          for (int s = s0; s < s1; ++s) {
+            if (!it_wait(smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
+              report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x);
+              abort_flag = 1;
+              ok = false;
+              break;
             }
-        }
-        for (int s = s0; s < s1; ++s) {
-          if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
-            if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
-            ok = false;
-            break;
-          }
-          const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
-          if (lane == 0) {
-            mbar_expect_tx(full, X_BYTES + rec);
+            const uint32_t full = smem_u32(&bar_full[st]), at = smem_base + st * stage_bytes;
+            mbar_expect_tx(full, (p.src_row == nullptr ? X_BYTES : 0) + SUB * rec);
             bulk_load_1d(at + X_BYTES, w + (size_t)s * rec, rec, full);
+            if (SUB == 2) bulk_load_1d(at + X_BYTES + w_bytes, w + second + (size_t)s * rec, rec, full);
             if (p.src_row == nullptr) {
               tma_load_2d(at, &tmX, full, s * I4_STEP, tl.row0, keep);
               tma_load_2d(at + NT * 128, &tmX, full, s * I4_STEP + 64, tl.row0, keep);
             }
+            if (++st == p.stages) { st = 0; ph ^= 1; }
           }
-          __syncwarp();
-          if (p.src_row != nullptr) {
-            // a half that lies behind K as a whole has scales of zero: any columns do
-            const int x = lane & 1 ? (s * I4_STEP + 64 < p.K ? s * I4_STEP + 64 : 0) : s * I4_STEP;
-#pragma unroll
-            for (int i = 0; i < PARTS; ++i)
-              if (lane + 32 * i < NT / 2) it_gather4(at + (lane & 1) * NT * 128 + ((lane + 32 * i) >> 1) * 512, &tmX, full, x, from[i][0], from[i][1], from[i][2], from[i][3]);
-          }
-          if (++st == p.stages) { st = 0; ph ^= 1; }
         }
       }
+      __syncwarp();
     } else if (warp == 1) {
       // ================= MMA =================
       if (elect_one()) {
@@ -250,7 +237,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
           if (!seen_c && !it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; ok = false; break; }
           const uint32_t at = smem_base + st * stage_bytes;
           const uint64_t dx0 = umma_desc_sw128(at), dx1 = umma_desc_sw128(at + NT * 128);
-          const uint32_t a_tmem = tmem_base + S::BUFS * S::ACC + slot * 64;
+          const uint32_t a_tmem = tmem_base + SUB * (S::BUFS * S::ACC + slot * 64);
           const uint32_t cempty = smem_u32(&bar_cempty[slot]), empty = smem_u32(&bar_empty[st]);
           if (++slot == S::SLOTS) { slot = 0; sph ^= 1; }
           if (++st == p.stages) st = 0;
@@ -264,10 +251,12 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             tc_fence_after();
             constexpr int PER = 8 / GP;              // MMAs of a group
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const int k = g * PER + i;
-              mma_f16_ts(tmem_base + buf * S::ACC, a_tmem + 8 * k, (k < 4 ? dx0 : dx1) + 2 * (k & 3), idesc, i > 0 ? 1u : 0u);
-            }
+            for (int sub = 0; sub < SUB; ++sub)
+#pragma unroll
+              for (int i = 0; i < PER; ++i) {
+                const int k = g * PER + i;
+                mma_f16_ts(tmem_base + (buf * SUB + sub) * S::ACC, a_tmem + sub * 64 + 8 * k, (k < 4 ? dx0 : dx1) + 2 * (k & 3), idesc, i > 0 ? 1u : 0u);
+              }
             tc_commit(smem_u32(&bar_dfull[buf]));
             if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
             seen_d = it_peek(smem_u32(&bar_dempty[buf]), bph ^ 1);
@@ -279,13 +268,58 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
         }
       }
       __syncwarp();
+    } else if (warp < 4) {
+      // ================= rows that src_row names: 16 lanes copy one, two warps four at a time, swizzled as TMA would =================
+      if (NT < 128 && p.src_row != nullptr) {
+        const int half = lane >> 4, c = lane & 15, first_row = 2 * (warp - 2) + half;
+        int st = 0, e = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int u = first; u < total && ok; u += hop) {
+          const Tile tl = tile_at(u, e);
+          const int mine = 4 * (lane >> 1) + 2 * (warp - 2) + (lane & 1);       // a lane keeps the number of one of its warp's rows
+          int from = 0;
+          if (mine < tl.valid) {
+            const int row = p.src_row[tl.row0 + mine];
+            if (row < 0 || row >= p.x_rows) report_status(p.status, ST_BAD_INDEX, row);
+            else from = row;
+          }
+          for (int s = s0; s < s1; ++s) {
+            if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
+              if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
+              ok = false;
+              break;
+            }
+            const int k = s * I4_STEP + c * 8;             // (behind K zeros, as their scales are)
+            const __nv_bfloat16* x = p.x + (k < p.K ? k : 0);
+            const uint32_t bytes = k < p.K ? 16 : 0, to = smem_base + st * stage_bytes + (c >> 3) * NT * 128 + first_row * 128;
+            constexpr int PASSES = NT / 4, BATCH = PASSES < 8 ? PASSES : 8;       // addresses first: a chain from shuffle to copy is 70 cycles
+#pragma unroll
+            for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
+              if (4 * i0 >= tl.valid) break;
+              const __nv_bfloat16* src[BATCH];
+#pragma unroll
+              for (int i = 0; i < BATCH; ++i) src[i] = x + (size_t)__shfl_sync(0xffffffffu, from, 2 * (i0 + i) + half) * p.x_ld;
+#pragma unroll
+              for (int i = 0; i < BATCH; ++i) {
+                const int at = 4 * (i0 + i);
+                // (rows of the stage behind the tile's last stay what they were: no result has them)
+                if (at + first_row < tl.valid) it_copy16(to + at * 128 + (((c & 7) ^ ((at + first_row) & 7)) << 4), src[i], bytes);
+              }
+            }
+            it_copy_arrive(smem_u32(&bar_full[st]));
+            if (++st == p.stages) { st = 0; ph ^= 1; }
+          }
+        }
+        it_copy_wait_all();
+      }
     } else if (warp >= 4 && warp < 4 + S::CONV_WARPS) {
-      // ================= converters: row r of the tile; with eight warps the two groups take the steps in turn =================
-      constexpr int GROUPS = S::CONV_WARPS / 4;
-      const int r = (warp & 3) * 32 + lane, group = (warp - 4) >> 2;
+      // ================= converters: row r of the tile; of eight warps four take a tile each, or the two groups the steps in turn =================
+      constexpr int GROUPS = S::GROUPS;
+      const int r = (warp & 3) * 32 + lane, sub = (warp - 4) / 4 % SUB, group = (warp - 4) / (4 * SUB);
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
-      const int in_stage = X_BYTES + (r >> 4) * I4_CODES + (r & 7) * 16 + ((r >> 3) & 1) * 8, row_at = (r >> 4) * 8 + (r & 7), odd = (r >> 3) & 1;
-      const int zero_at = X_BYTES + i4_zeros(GP) + row_at * GP * 2 + odd, scale_at = X_BYTES + I4_SCALES + row_at * GP * 4 + odd * 2;
+      const int in_stage = X_BYTES + sub * w_bytes + (r >> 4) * I4_CODES + (r & 7) * 16 + ((r >> 3) & 1) * 8, row_at = (r >> 4) * 8 + (r & 7), odd = (r >> 3) & 1;
+      const int zero_at = X_BYTES + sub * w_bytes + i4_zeros(GP) + row_at * GP * 2 + odd, scale_at = X_BYTES + sub * w_bytes + I4_SCALES + row_at * GP * 4 + odd * 2;
       int st = group, slot = group;
       uint32_t ph = 0, sph = 0, seen = 0;
       // (a step is a step here, whatever tile it belongs to)
@@ -296,15 +330,15 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
           break;
         }
         const uint8_t* at = smem_raw + (smem_base - smem_u32(smem_raw)) + st * stage_bytes;
-        const uint32_t to = tmem_base + S::BUFS * S::ACC + slot * 64 + lane_tmem, cfull = smem_u32(&bar_cfull[slot]), cempty = smem_u32(&bar_cempty[slot]);
+        const uint32_t to = tmem_base + SUB * (S::BUFS * S::ACC + slot * 64) + sub * 64 + lane_tmem, cfull = smem_u32(&bar_cfull[slot]), cempty = smem_u32(&bar_cempty[slot]);
         uint32_t free_slot = it_peek(cempty, sph ^ 1);
         const uint32_t sph_now = sph;
         slot += GROUPS;
         if (slot >= S::SLOTS) { slot -= S::SLOTS; sph ^= 1; }
-        st += GROUPS;                         // (an even number of stages: a group sees every phase of its own)
+        st += GROUPS;                         // (two groups, an even number of stages: a group sees every phase of its own)
         if (st >= p.stages) { st -= p.stages; ph ^= 1; }
         // With registers for it the whole step is ready before the slot is asked for: what follows the wait is in the chain slot - MMAs - slot.
-        constexpr int READY = S::WIDE ? 2 : 1;       // halves of a step
+        constexpr int READY = S::ONE ? 2 : 1;       // halves of a step
         bool ok = true;
 #pragma unroll
         for (int j0 = 0; j0 < 2; j0 += READY) {
@@ -337,7 +371,7 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
             }
             tc_fence_after();
 #pragma unroll
-            for (int g = 0; g < GP; ++g) scales[s & (IT_SCALES - 1)][g][r] = sc[g];
+            for (int g = 0; g < GP; ++g) scales[s & (IT_SCALES - 1)][g][sub * 128 + r] = sc[g];
           }
 #pragma unroll
           for (int i = 0; i < READY; ++i) {
@@ -347,6 +381,9 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
         }
         if (!ok) break;
         seen = it_peek(smem_u32(&bar_full[st]), ph);
+        // gathered rows are ordinary writes, which this thread has seen complete: from here on the MMAs see them too. (The gatherers would wait in the
+        // fence for the copies that they have only begun.)
+        if (p.src_row != nullptr) fence_proxy_async_smem();
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -354,14 +391,16 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
       }
     } else if (warp >= 4) {
       // ================= epilogue: row r, columns col0 .. + EPI_COLS =================
-      const int r = (warp & 3) * 32 + lane, col0 = ((warp - 4 - S::CONV_WARPS) >> 2) * S::EPI_COLS;
+      const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS;
       const uint32_t lane_tmem = (uint32_t)((warp & 3) * 32) << 16;
       int buf = 0, it = 0, e = 0;
       uint32_t bph = 0, seen = 0;
       bool ok = true;
       for (int u = first; u < total; u += hop) {
 #pragma unroll
-        for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[c] = 0ull;
+        for (int h = 0; h < SUB; ++h)
+#pragma unroll
+          for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[h][c] = 0ull;
         for (int s = s0; s < s1 && ok; ++s, ++it) {
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
@@ -371,60 +410,67 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
               break;
             }
             tc_fence_after();
-            const uint32_t from = tmem_base + buf * S::ACC + col0 + lane_tmem, dempty = smem_u32(&bar_dempty[buf]);
-            // (written before the arrival that let the step's MMAs begin)
-            const float sc = *reinterpret_cast<volatile float*>(&scales[it & (IT_SCALES - 1)][g][r]);
-            const uint64_t s2 = it_pack(sc, sc);
+            const uint32_t from = tmem_base + buf * SUB * S::ACC + col0 + lane_tmem, dempty = smem_u32(&bar_dempty[buf]);
             if (++buf == S::BUFS) { buf = 0; bph ^= 1; }
-            constexpr int STEP = S::EPI_COLS < 32 ? 16 : 32;
+            // (written before the arrival that let the step's MMAs begin)
+            uint64_t s2[SUB];
 #pragma unroll
-            for (int c0 = 0; c0 < S::EPI_COLS; c0 += STEP) {
-              uint32_t v[STEP];
-              tmem_ld16(from + c0, v);
-              if constexpr (STEP == 32) tmem_ld16(from + c0 + 16, v + 16);
+            for (int h = 0; h < SUB; ++h) {
+              const float sc = *reinterpret_cast<volatile float*>(&scales[it & (IT_SCALES - 1)][g][h * 128 + r]);
+              s2[h] = it_pack(sc, sc);
+            }
+            constexpr int COLS_ALL = SUB * S::EPI_COLS, AT_ONCE = S::EPI_COLS < 32 ? 16 : 32;
+#pragma unroll
+            for (int c0 = 0; c0 < COLS_ALL; c0 += AT_ONCE) {
+              uint32_t v[AT_ONCE];
+#pragma unroll
+              for (int c = 0; c < AT_ONCE; c += 16) tmem_ld16(from + c0 + c, v + c);
               tmem_ld_wait();
-              if (c0 + STEP == S::EPI_COLS) {
+              if (c0 + AT_ONCE == COLS_ALL) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(dempty);
                 seen = it_peek(smem_u32(&bar_dfull[buf]), bph);
               }
 #pragma unroll
-              for (int c = 0; c < STEP; c += 2) it_fma2(acc[(c0 + c) / 2], v[c], v[c + 1], s2);
+              for (int c = 0; c < AT_ONCE; c += 2) it_fma2(acc[(c0 + c) / S::EPI_COLS][(c0 + c) % S::EPI_COLS / 2], v[c], v[c + 1], s2[(c0 + c) / S::EPI_COLS]);
             }
           }
         }
         if (!ok || p.split > 1) break;
         const Tile tl = tile_at(u, e);
         // (MMAs of the next tile wait for these warps once the accumulators are full: what is the same for all columns stays out of the loops)
-        const int f = pair ? (tl.m * 8 + (r >> 4)) * 8 + (r & 7) : tl.m * 128 + r, mine = pair ? (lane >> 3) & 1 : 0;
-        const int left = f < p.F ? tl.valid - col0 - mine : 0;
-        const size_t at = (size_t)(tl.row0 + col0 + mine) * p.out_ld + f;
-        if (pair) {
-          __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
 #pragma unroll
-          for (int c = 0; c < S::EPI_COLS; c += 2) {
-            const float2 v = it_unpack(acc[c / 2]);
-            const float y = of_pair(v.x, v.y);
-            if (c < left) *to = __float2bfloat16(y);
-            to += 2 * p.out_ld;
-          }
-        } else if (!f32 && p.residual == nullptr) {
-          __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
+        for (int h = 0; h < SUB; ++h) {
+          const int m = tl.m * SUB + h, f = pair ? (m * 8 + (r >> 4)) * 8 + (r & 7) : m * 128 + r, mine = pair ? (lane >> 3) & 1 : 0;
+          const int left = f < p.F ? tl.valid - col0 - mine : 0;
+          const size_t at = (size_t)(tl.row0 + col0 + mine) * p.out_ld + f;
+          if (pair) {
+            __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
 #pragma unroll
-          for (int c = 0; c < S::EPI_COLS; c += 2) {
-            const float2 v = it_unpack(acc[c / 2]);
-            if (c < left) *to = __float2bfloat16(v.x);
-            to += p.out_ld;
-            if (c + 1 < left) *to = __float2bfloat16(v.y);
-            to += p.out_ld;
-          }
-        } else {
+            for (int c = 0; c < S::EPI_COLS; c += 2) {
+              const float2 v = it_unpack(acc[h][c / 2]);
+              const float y = of_pair(v.x, v.y);
+              if (c < left) *to = __float2bfloat16(y);
+              to += 2 * p.out_ld;
+            }
+          } else if (!f32 && p.residual == nullptr) {
+            __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
 #pragma unroll
-          for (int c = 0; c < S::EPI_COLS; c += 2) {
-            const float2 v = it_unpack(acc[c / 2]);
-            if (c < left) store(at + (size_t)c * p.out_ld, v.x);
-            if (c + 1 < left) store(at + (size_t)(c + 1) * p.out_ld, v.y);
+            for (int c = 0; c < S::EPI_COLS; c += 2) {
+              const float2 v = it_unpack(acc[h][c / 2]);
+              if (c < left) *to = __float2bfloat16(v.x);
+              to += p.out_ld;
+              if (c + 1 < left) *to = __float2bfloat16(v.y);
+              to += p.out_ld;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < S::EPI_COLS; c += 2) {
+              const float2 v = it_unpack(acc[h][c / 2]);
+              if (c < left) store(at + (size_t)c * p.out_ld, v.x);
+              if (c + 1 < left) store(at + (size_t)(c + 1) * p.out_ld, v.y);
+            }
           }
         }
       }
@@ -434,38 +480,44 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   // ---- the pieces of a tile: every CTA finishes NT / split columns, summed in rank order
   if (p.split > 1 && live) {
     const bool epi = warp >= 4 + S::CONV_WARPS;
-    const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS, slice = NT / p.split;
-    float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));      // [rank][slice][128], on stages that nothing reads any more
+    const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS;
+    const int slice = NT / p.split;
+    float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));      // [rank][tile][slice][128], on stages that nothing reads any more
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     if (epi) {
 #pragma unroll
-      for (int c = 0; c < S::EPI_COLS; c += 2) {       // (a slice is an even number of columns)
-        const float2 v = it_unpack(acc[c / 2]);
-        float* to = cluster.map_shared_rank(recv, (col0 + c) / slice) + (rank * slice + (col0 + c) % slice) * 128 + r;
-        to[0] = v.x;
-        to[128] = v.y;
-      }
+      for (int h = 0; h < SUB; ++h)
+#pragma unroll
+        for (int c = 0; c < S::EPI_COLS; c += 2) {       // (a slice is an even number of columns)
+          const float2 v = it_unpack(acc[h][c / 2]);
+          float* to = cluster.map_shared_rank(recv, (col0 + c) / slice) + ((rank * SUB + h) * slice + (col0 + c) % slice) * 128 + r;
+          to[0] = v.x;
+          to[128] = v.y;
+        }
     }
     cluster.sync();
     if (epi && abort_flag == 0) {
       int e = 0;
       const Tile tl = tile_at(first, e);
-      for (int c = part * 2; c < slice; c += 2 * (S::EPI_WARPS / 4)) {
-        if (rank * slice + c >= tl.valid) break;
-        float a = 0.f, b = 0.f;
-        for (int q = 0; q < p.split; ++q) {
-          a += recv[(q * slice + c) * 128 + r];
-          b += recv[(q * slice + c + 1) * 128 + r];
-        }
-        const int col = rank * slice + c, f = pair ? (tl.m * 8 + (r >> 4)) * 8 + (r & 7) : tl.m * 128 + r;
-        if (pair) {
-          const float y = of_pair(a, b);
-          const int own = col + ((lane >> 3) & 1);
-          if (f < p.F && own < tl.valid) store((size_t)(tl.row0 + own) * p.out_ld + f, y);
-        } else if (f < p.F) {
-          store((size_t)(tl.row0 + col) * p.out_ld + f, a);
-          if (col + 1 < tl.valid) store((size_t)(tl.row0 + col + 1) * p.out_ld + f, b);
+      for (int h = 0; h < SUB; ++h) {
+        const int m = tl.m * SUB + h, f = pair ? (m * 8 + (r >> 4)) * 8 + (r & 7) : m * 128 + r;
+        for (int c = part * 2; c < slice; c += S::EPI_WARPS / 2) {
+          const int col = rank * slice + c;
+          if (col >= tl.valid) break;
+          float a = 0.f, b = 0.f;
+          for (int q = 0; q < p.split; ++q) {
+            a += recv[((q * SUB + h) * slice + c) * 128 + r];
+            b += recv[((q * SUB + h) * slice + c + 1) * 128 + r];
+          }
+          if (pair) {
+            const float y = of_pair(a, b);
+            const int own = col + ((lane >> 3) & 1);
+            if (f < p.F && own < tl.valid) store((size_t)(tl.row0 + own) * p.out_ld + f, y);
+          } else if (f < p.F) {
+            store((size_t)(tl.row0 + col) * p.out_ld + f, a);
+            if (col + 1 < tl.valid) store((size_t)(tl.row0 + col + 1) * p.out_ld + f, b);
+          }
         }
       }
     }
@@ -479,21 +531,21 @@ __global__ void __launch_bounds__(ItShape<NT>::THREADS, ItShape<NT>::WIDE ? 1 : 
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, S::COLS); }
 }
 
-template <int NT, int GP>
+template <int NT, int GP, int SUB>
 static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s) {
-  using S = ItShape<NT>;
+  using S = ItShape<NT, SUB>;
   static PerDevice allowed;
-  const int list = 4 * (3 * p.E + 1), room = (S::WIDE ? 224 : 112) * 1024 - IT_SCALES * GP * 512 - 2048;     // (beside the static part)
-  const int stage = NT * 256 + ((i4_record(GP, p.flags & 8) + 1023) & ~1023);
+  const int list = 4 * (3 * p.E + 1), room = (S::ONE ? 224 : 112) * 1024 - IT_SCALES * GP * 512 * SUB - 2048;     // (beside the static part)
+  const int stage = NT * 256 + SUB * ((i4_record(GP, p.flags & 8) + 1023) & ~1023);
   p.stages = (room - 1024 - list) / stage;
   if (p.stages > IT_MAX_STAGES) p.stages = IT_MAX_STAGES;
-  p.stages &= ~1;        // every stage belongs to one group of converters
+  if (S::GROUPS == 2) p.stages &= ~1;        // every stage belongs to one group of converters
   if (p.stages < 2) return -1;
-  const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP>, room);
+  const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP, SUB>, room);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};
   // a cluster has one tile, else a CTA per place on the GPU walks them
-  cfg.gridDim = dim3(p.split > 1 ? (unsigned)tiles * p.split : (unsigned)min(tiles, S::WIDE ? 148 : 296));
+  cfg.gridDim = dim3(p.split > 1 ? (unsigned)tiles * p.split : (unsigned)min(tiles, S::ONE ? 148 : 296));
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = (size_t)p.stages * stage + 1024 + list;
   cfg.stream = s;
@@ -506,11 +558,11 @@ static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return (int)cudaLaunchKernelEx(&cfg, int4_tc_kernel<NT, GP>, tmX, p);
+  return (int)cudaLaunchKernelEx(&cfg, int4_tc_kernel<NT, GP, SUB>, tmX, p);
 }
-template <int NT>
+template <int NT, int SUB>
 static int launch_tc_group(const CUtensorMap& tmX, const Int4Tc& p, int group, int tiles, cudaStream_t s) {
-  return group == 128 ? launch_tc<NT, 1>(tmX, p, tiles, s) : group == 64 ? launch_tc<NT, 2>(tmX, p, tiles, s) : launch_tc<NT, 4>(tmX, p, tiles, s);
+  return group == 128 ? launch_tc<NT, 1, SUB>(tmX, p, tiles, s) : group == 64 ? launch_tc<NT, 2, SUB>(tmX, p, tiles, s) : launch_tc<NT, 4, SUB>(tmX, p, tiles, s);
 }
 
 }  // namespace skein
@@ -525,41 +577,52 @@ extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, 
   if (rows < 0 || x_rows < 1 || E < 1 || E > 1024 || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
   if (x_ld % 8 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0) return -1;
   if (n_tile == 0) {
-    // experts' rows differ: room for a quarter more than their mean, as a second tile of an expert converts its weights again (28672 x 4096, 8 experts:
-    // mean 16 301 us with tiles of 16 rows, 251 with 32; 2048 x 1408, 64 experts: mean 12 60 and 69, mean 37 111 with 32, 123 with 64)
+    // experts' rows differ: room for a quarter more than their mean, as a second tile of an expert converts its weights again. Measured, us, tiles of
+    // 16 / 32 / 64 rows: 28672 x 4096, 8 experts, mean 8 125 / 168 / 199, mean 16 181 / 170 / 199, mean 32 282 / 247 / 226; 2048 x 1408, 64 experts, mean 4.5
+    // 31 / 38 / 46, mean 12 45 / 42 / 51, mean 37 81 / 70 / 65.
     const int want = counts == nullptr ? rows_hint : rows_hint + rows_hint / 4;
     n_tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
   }
   if (n_tile != 16 && n_tile != 32 && n_tile != 64 && n_tile != 128) return -1;
+  // Gathered rows take two warps of a CTA as long as the MMAs of 128: two CTAs with 64 are as quick (28672 x 4096, 8 experts, mean 64 353 us and 413, mean 250
+  // 1031 and 1066).
+  if (src_row != nullptr && n_tile == 128) n_tile = 64;
   Int4Tc p;
-  p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts; p.offsets = offsets; p.status = status;
+  p.x = (const __nv_bfloat16*)x; p.x_ld = x_ld; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts; p.offsets = offsets; p.status = status;
   p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.E = E; p.F = F; p.K = K; p.flags = flags;
   p.strips = flags & 1 ? (F + 7) / 8 : (F + 15) / 16;
   p.steps = (K + I4_STEP - 1) / I4_STEP;
-  p.m_tiles = (p.strips + 7) / 8;
+  p.w_tiles = (p.strips + 7) / 8;
   p.budget_ns = (uint64_t)gemm_wait_budget_ms() * 1000000ull;
-  // row tiles at most: an expert's last one may be part empty
+  // row tiles at most (an expert's last one may be part empty), and those to expect
   const long long row_tiles = counts == nullptr ? (rows + n_tile - 1) / n_tile : (rows + (long long)(n_tile - 1) * (E < rows ? E : rows)) / n_tile;
+  const long long expect_rows = counts == nullptr ? row_tiles : rows < E ? (long long)rows : (long long)E * ((rows_hint + n_tile - 1) / n_tile);
+  // Two tiles of 16 rows at a time from where one each fills the GPU (1408 x 2048 pairs, 64 experts, mean 4.5: 79 us one at a time, 65 two; 152064 x 3584 100
+  // and 96; but 18944 x 2048, 148 tiles, 12.1 and 16.2).
+  const bool two = n_tile == 16 && split <= 1 && p.w_tiles * expect_rows >= 296;
+  p.m_tiles = two ? (p.w_tiles + 1) / 2 : p.w_tiles;
   const long long tiles = row_tiles * p.m_tiles;
   if (split == 0) {
     // Pieces until every place on the GPU has a CTA, while they keep eight steps, or four where there is less than one CTA per SM (16 rows of 4096 x 4096:
     // 12.7 us in two pieces, 10.1 in four of eight steps, 10.7 in eight; 1024 x 4096 11.9 in four, 9.3 in eight; 4096 x 14336 18.6 and 17.6).
-    const long long expect = counts == nullptr ? tiles : p.m_tiles * (rows < E ? (long long)rows : (long long)E * ((rows_hint + n_tile - 1) / n_tile));
+    const long long expect = p.m_tiles * expect_rows;
     const int slots = 148 * (n_tile == 128 ? 1 : 2);
     split = 1;
-    while (split < 8 && expect * split * 2 <= slots && p.steps / (split * 2) >= (expect * split * 2 <= 148 ? 4 : 8)) split *= 2;
+    while (!two && split < 8 && expect * split * 2 <= slots && p.steps / (split * 2) >= (expect * split * 2 <= 148 ? 4 : 8)) split *= 2;
   }
   if (split != 1 && split != 2 && split != 4 && split != 8) return -1;
   if (tiles * split > 0x7fffffffll) return -1;
   p.split = split;
-  CUtensorMap tmX;
-  const int rc = make_tmap_2d(&tmX, x, (uint64_t)x_rows, (uint64_t)K, (uint64_t)x_ld, 2, src_row != nullptr ? 1 : n_tile);
-  if (rc) return rc;
+  CUtensorMap tmX{};
+  if (src_row == nullptr) {
+    const int rc = make_tmap_2d(&tmX, x, (uint64_t)x_rows, (uint64_t)K, (uint64_t)x_ld, 2, n_tile);
+    if (rc) return rc;
+  }
   cudaStream_t s = (cudaStream_t)stream;
   switch (n_tile) {
-    case 16: return launch_tc_group<16>(tmX, p, group, (int)tiles, s);
-    case 32: return launch_tc_group<32>(tmX, p, group, (int)tiles, s);
-    case 64: return launch_tc_group<64>(tmX, p, group, (int)tiles, s);
-    default: return launch_tc_group<128>(tmX, p, group, (int)tiles, s);
+    case 16: return two ? launch_tc_group<16, 2>(tmX, p, group, (int)tiles, s) : launch_tc_group<16, 1>(tmX, p, group, (int)tiles, s);
+    case 32: return launch_tc_group<32, 1>(tmX, p, group, (int)tiles, s);
+    case 64: return launch_tc_group<64, 1>(tmX, p, group, (int)tiles, s);
+    default: return launch_tc_group<128, 1>(tmX, p, group, (int)tiles, s);
   }
 }

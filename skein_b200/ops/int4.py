@@ -179,12 +179,17 @@ def _check_out(what, out, rows, w, dtype):
         raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
 
 
-def _few_rows(hint: int, K: int) -> bool:
+def _few_rows(hint: int, K: int, grouped: bool) -> bool:
     """Whether a product with `hint` rows per matrix runs on the kernel of few rows (csrc/kernels/int4_rows.cu) instead of the one on tensor memory
     (int4_tc.cu), which has more to set up and is the quicker one from where a warp's share of the rows of x costs more than the conversion. Measured, few
-    rows / tensor memory, us: 4096 x 4096 7.3 / 9.7 at 1 row, 9.8 / 10.1 at 8, 11.7 / 10.1 at 12; 4096 x 14336 13.9 / 17.4 at 1, 17.1 / 17.6 at 4, 19.0 / 17.6
-    at 6; gate / up 14336 x 4096 25.2 / 30.3 at 1, 29.1 / 30.9 at 8, 37.0 / 31.1 at 12; 8 experts of it 35.5 / 65.5 at 1 token, 156 / 188 at a mean of 8
-    rows, 277 / 251 at 16; 64 experts 2048 x 1408 32.7 / 33.4 at a mean of 1.5, 48.4 / 45.7 at 4.5."""
+    rows / tensor memory, us: 4096 x 4096 7.4 / 9.6 at 1 row, 9.8 / 9.9 at 8, 12.7 / 10.0 at 16; 4096 x 14336 13.9 / 17.4 at 1, 16.9 / 17.6 at 4, 25.5 / 17.6
+    at 7; gate / up 14336 x 4096 25.3 / 29.8 at 1, 29.1 / 29.8 at 8, 37.8 / 29.8 at 16.
+    With experts the tensor-memory kernel takes two tiles at a time, and the mean of unequal rows is asked. 8 experts, gate / up 14336 x 4096: 35.4 / 43.6 at 1
+    token, 90 / 92 at a mean of 2 rows, 117 / 124 at 3, 130 / 125 at 4; 4096 x 14336 61 / 75 at 2, 66 / 75 at 3, 79 / 75 at 4. 64 experts, gate / up 1408 x
+    2048: 26.9 / 31 at 0.4, 41.9 / 41.9 at 0.75, 53 / 54 at 1.5, 61 / 55 at 2.3; 2048 x 1408 26 / 24 at 0.75, 35 / 25 at 1.5. 128 experts, 2048 x 768: 21 / 20
+    at 0.25, 32 / 25 at 1."""
+    if grouped:
+        return hint << 10 < min(K, 1 << 12)
     return hint <= 8 and hint * K <= 1 << 16
 
 
@@ -202,7 +207,7 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
     """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, (0, team) of the kernel of few rows."""
     L, dev = _lib.lib(), w.device
     xp, x_ld = x.data_ptr(), x.stride(0)
-    few = _few_rows(hint, w.K) if cfg is None else cfg[0] == 0
+    few = _few_rows(hint, w.K, counts is not None) if cfg is None else cfg[0] == 0
     args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.ptr, None if residual is None else residual.data_ptr(), out.data_ptr(),
             out.stride(0), None if counts is None else counts.data_ptr(), None if counts is None else offsets.data_ptr(), rows, x.shape[0], w.matrices,
             w.features, w.K, w.group, hint, flags)

@@ -225,6 +225,34 @@ def test_many_uneven_experts(cfg):
     ops.workspace().check_status()
 
 
+@pytest.mark.parametrize("tile", [16, 32, 64, 128])
+@pytest.mark.parametrize("E, features, K, group, zeros, pair", [(60, 650, 1024, 128, False, False), (100, 392, 416, 32, True, True), (1024, 130, 192, 64, True, False),
+                                                                (7, 5400, 320, 64, False, True), (40, 1030, 2176, 128, True, False)])
+def test_gathered_rows_of_many_tiles(E, features, K, group, zeros, pair, tile):
+    """An odd number of weight tiles per expert, experts that are empty, of one row and of several row tiles, rows named twice, rows of x that lie apart; a row
+    that is no number stays alone, though its place in shared memory is used again."""
+    gen = torch.Generator(device=DEV).manual_seed(E)
+    counts = torch.randint(0, 30, (E,), generator=gen, device=DEV, dtype=torch.int32)
+    counts[::5], counts[1], counts[-1] = 0, 1, 150
+    off = torch.cat((counts.new_zeros(1), counts.cumsum(0))).to(torch.int32)
+    n = int(off[-1])
+    w, full = weight((E,), features * (2 if pair else 1), K, group, zeros, torch.bfloat16, pair)
+    x = acts(50, K + 24)[:, 8:8 + K]
+    x[7] = float("nan")
+    src = torch.randint(0, 50, (n,), generator=gen, device=DEV, dtype=torch.int32)
+    src[torch.randint(0, n, (n // 3,), generator=gen, device=DEV)] = 5
+    y = int4.grouped_linear(x, w, counts, off, swiglu=pair, src_row=src, _cfg=(tile, 1))
+    expert = torch.repeat_interleave(torch.arange(E, device=DEV), counts.long())
+    lost = src == 7
+    assert bool(lost.any()) and bool(y[lost].isnan().all())
+    for e in list(range(0, E, max(1, E // 40))) + [E - 1]:
+        mine = (expert == e) & ~lost
+        if bool(mine.any()):
+            within(y[mine], x[src[mine].long()], full[e], pair)
+    assert bool(y[~lost].isfinite().all())
+    ops.workspace().check_status()
+
+
 @pytest.mark.parametrize("cfg", [(0, 0), (16, 1), (64, 1)])
 def test_experts_beyond_31_bits(cfg):
     """The last expert's codes lie more than 2^31 bytes into the weight."""

@@ -17,6 +17,7 @@ GROUPS = (32, 64, 128)
 STEP = 128                 # elements of K of a packed block (16 rows)
 CODES = 16 * STEP // 2     # its bytes of codes
 MAX_EXPERTS = 1024
+MAX_ROW = 1 << 16       # of K in the kernel of few rows, which keeps whole rows of x in shared memory
 
 
 class Int4Weight:
@@ -189,8 +190,8 @@ def _few_rows(hint: int, K: int, grouped: bool) -> bool:
     2048: 26.9 / 31 at 0.4, 41.9 / 41.9 at 0.75, 53 / 54 at 1.5, 61 / 55 at 2.3; 2048 x 1408 26 / 24 at 0.75, 35 / 25 at 1.5. 128 experts, 2048 x 768: 21 / 20
     at 0.25, 32 / 25 at 1."""
     if grouped:
-        return hint << 10 < min(K, 1 << 12)
-    return hint <= 8 and hint * K <= 1 << 16
+        return hint << 10 < min(K, 1 << 12) and K <= MAX_ROW
+    return hint <= 8 and hint * K <= MAX_ROW
 
 
 _STATUS: dict = {}      # device -> address of the status word of its workspace, which is made once
@@ -211,7 +212,10 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
     args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.ptr, None if residual is None else residual.data_ptr(), out.data_ptr(),
             out.stride(0), None if counts is None else counts.data_ptr(), None if counts is None else offsets.data_ptr(), rows, x.shape[0], w.matrices,
             w.features, w.K, w.group, hint, flags)
-    if few or xp % 16 or x_ld % 8:
+    aside = xp % 16 != 0 or x_ld % 8 != 0
+    if aside and w.K > MAX_ROW:
+        raise ValueError(f"{what}: rows of x off 16-byte boundaries have at most {MAX_ROW} elements, not {w.K}")
+    if few or aside:
         rc = L.skein_int4_rows(*args, cfg[1] if cfg and few else 0, _status(dev), _lib.stream_on(dev))
     else:
         rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), _status(dev), _lib.stream_on(dev))

@@ -104,6 +104,23 @@ def test_strides_and_alignment(rows):
     within(int4.linear(wide[:1, :256].expand(rows, 256), w), wide[:1, :256].expand(rows, 256), full)
 
 
+def test_long_rows():
+    """Rows that the kernel of few rows has no place for go to the other one, or are refused where that cannot read them."""
+    K = int4.MAX_ROW + 32768
+    w, full = weight((2,), 48, K, 128, True, torch.bfloat16, False)
+    wide = acts(3, K + 8)
+    x = wide[:, :K]
+    cnt, off = torch.tensor([1, 2], dtype=torch.int32, device=DEV), torch.tensor([0, 1, 3], dtype=torch.int32, device=DEV)
+    y = int4.grouped_linear(x, w, cnt, off)
+    within(y[:1], x[:1], full[0])
+    within(y[1:], x[1:], full[1])
+    with pytest.raises(ValueError, match="16-byte"):
+        int4.grouped_linear(wide[:, 1:K + 1], w, cnt, off)
+    w, full = weight((), 48, int4.MAX_ROW, 128, True, torch.bfloat16, False)
+    within(int4.linear(wide[:, 1:int4.MAX_ROW + 1], w), wide[:, 1:int4.MAX_ROW + 1], full)
+    ops.workspace().check_status()
+
+
 @pytest.mark.parametrize("rows", [4, 40])
 def test_a_row_that_is_no_number_stays_alone(rows):
     w, full = weight((), 64, 256, 128, False, torch.bfloat16, False)

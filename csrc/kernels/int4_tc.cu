@@ -16,7 +16,7 @@
 // conversion, the drains and seven of eight MMAs left out it still took 870. The MMAs of a step are 280 cycles with up to 64 rows of x and 512 with 128, the
 // weights' share of HBM is 365 cycles per SM. So with up to 64 rows two CTAs share an SM, with 16 rows two tiles of weights a step, handovers are whole
 // steps, and tests of barriers are issued before their answers are needed. Gathered rows are bounded by the two warps that copy them. Measured: 1000 rows of
-// gate / up 37888 x 3584 243 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 468 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 96 us (3.2 TB/s),
+// gate / up 37888 x 3584 250 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 480 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 84 us (3.7 TB/s),
 // 128 rows over 8 experts of 28672 x 4096, gathered, 169 us (2.9 TB/s).
 // Pieces of a tile meet in distributed shared memory in rank order: the result does not depend on timing, and no memory outlives the call.
 #include "int4.cuh"
@@ -41,7 +41,7 @@ struct Int4Tc {
   const int *counts, *offsets;
   int* status;
   long long x_ld, out_ld;
-  int rows, x_rows, E, F, K, strips, steps, w_tiles, m_tiles, split, stages, flags;   // flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros
+  int rows, x_rows, E, F, K, strips, steps, w_tiles, m_tiles, split, least, stages, flags;   // split: CTAs of a cluster, least: steps of a piece; flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros
   uint64_t budget_ns;
 };
 
@@ -107,6 +107,9 @@ struct ItShape {
   static_assert(SUB * (BUFS * ACC + SLOTS * 64) <= COLS && GROUPS * 4 * SUB == CONV_WARPS, "tensor memory");
 };
 
+// What a CTA does: `items` tiles, `hop` apart; of the last one steps s0 .. s1 (of the others all), with `share` CTAs of a cluster on it
+struct ItPlan { int items, hop, last, s0, s1, share, mine, n_steps; };
+
 template <int NT, int GP, int SUB>
 __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::ONE ? 1 : 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Int4Tc p) {
   namespace cg = cooperative_groups;
@@ -115,6 +118,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
   __shared__ __align__(8) uint64_t bar_full[IT_MAX_STAGES], bar_empty[IT_MAX_STAGES], bar_cfull[S::SLOTS], bar_cempty[S::SLOTS], bar_dfull[S::BUFS], bar_dempty[S::BUFS];
   __shared__ uint32_t tmem_base_smem;
   __shared__ int abort_flag;
+  __shared__ ItPlan plan;
   __shared__ float scales[IT_SCALES][GP][SUB * 128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -163,20 +167,42 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       run += __shfl_sync(0xffffffffu, inc, 31);
     }
     if (lane == 0) pre[p.E] = run;
+    // A CTA walks whole tiles, every role at its own pace: the next tile's steps begin while the last one's results are stored. With two tiles a step
+    // what does not fill a round is shared: `share` CTAs of a cluster take a piece of K each.
+    if (SUB == 2 && lane == 0) {
+      const int grid = (int)gridDim.x, me = (int)blockIdx.x, rounds = run / grid, left = run - rounds * grid;
+      int share = 1;
+      while (share < p.split && left * share * 2 <= grid && p.steps >= p.least * share * 2) share *= 2;
+      const int rank = me % share;
+      const bool more = me / share < left;
+      plan.hop = grid;
+      plan.items = rounds + more;
+      plan.last = more ? rounds * grid + me / share : me + (rounds - 1) * grid;
+      plan.s0 = more ? (int)((long long)p.steps * rank / share) : 0;
+      plan.s1 = more ? (int)((long long)p.steps * (rank + 1) / share) : p.steps;
+      plan.share = share;
+      plan.mine = more && share > 1;
+      plan.n_steps = (plan.items - 1) * p.steps + plan.s1 - plan.s0;
+    }
   }
   __syncthreads();
-  const int total = pre[p.E];
-  // A CTA walks tiles `first`, first + hop, ..., every role at its own pace: the next tile's steps begin while the last one's results are stored. The
-  // CTAs of a cluster share one tile.
-  const int rank = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, hop = (int)gridDim.x / p.split;
-  const int s0 = (int)((long long)p.steps * rank / p.split), s1 = (int)((long long)p.steps * (rank + 1) / p.split);
+  // The other shapes, which the plan costs registers in their loops (3 to 8 %), take tiles `hop` apart from `first`, the same steps of each; the CTAs of a
+  // cluster share all of theirs (one).
+  const int rank_of = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, hop = (int)gridDim.x / p.split, total = pre[p.E];
+  const int s0 = (int)((long long)p.steps * rank_of / p.split), s1 = (int)((long long)p.steps * (rank_of + 1) / p.split);
+  const int items = SUB == 2 ? plan.items : first < total ? (total - first + hop - 1) / hop : 0;
+  struct Item { int u, s0, s1; };
+  auto item_at = [&](int n) {
+    if (SUB == 1) return Item{first + n * hop, s0, s1};
+    if (n + 1 < plan.items) return Item{(int)blockIdx.x + n * plan.hop, 0, p.steps};
+    return Item{plan.last, plan.s0, plan.s1};
+  };
   struct Tile { int e, m, row0, valid; };
   auto tile_at = [&](int u, int& e) {        // e: the expert of the role's tile before
     while (u >= pre[e + 1]) ++e;
     const int r = u - pre[e], nt = (cnt[e] + NT - 1) / NT, band = r / (IT_BAND * nt), rb = r - band * IT_BAND * nt, bm = min(IT_BAND, p.m_tiles - band * IT_BAND), n = rb / bm;
     return Tile{e, band * IT_BAND + rb - n * bm, off[e] + n * NT, min(NT, cnt[e] - n * NT)};
   };
-  const bool live = first < total;           // the same for every CTA of a cluster
   uint64_t acc[SUB][S::EPI_COLS / 2];        // two columns each
   const bool pair = p.flags & 1, f32 = p.flags & 4;
   auto store = [&](size_t at, float y) {
@@ -190,7 +216,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
     return silu(g) * u;
   };
 
-  if (live) {
+  if (items > 0) {
     if (warp == 0) {
       // ================= producer =================
       if (elect_one()) {
@@ -199,12 +225,13 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         int st = 0, e = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int u = first; u < total && ok; u += hop) {
-          const Tile tl = tile_at(u, e);
+        for (int n = 0; n < items && ok; ++n) {
+          const Item it = item_at(n);
+          const Tile tl = tile_at(it.u, e);
           // (behind the last tile that one again, for nothing)
           const uint8_t* w = p.w + ((size_t)tl.e * p.w_tiles + tl.m * SUB) * p.steps * rec;
           const size_t second = tl.m * SUB + 1 < p.w_tiles ? (size_t)p.steps * rec : 0;
-          for (int s = s0; s < s1; ++s) {
+          for (int s = it.s0; s < it.s1; ++s) {
             if (!it_wait(smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
               report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x);
               abort_flag = 1;
@@ -231,8 +258,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         int st = 0, slot = 0, buf = 0;
         uint32_t sph = 0, bph = 0, seen_c = 0, seen_d = 0;
         bool ok = true;
-        for (int u = first; u < total && ok; u += hop)
-        for (int s = s0; s < s1; ++s) {
+        for (int n = SUB == 2 ? items - 1 : 0; n < items && ok; ++n)
+        for (int s = 0, n_steps = SUB == 2 ? plan.n_steps : s1 - s0; s < n_steps; ++s) {
           // (the converters have seen the stage arrive, x included)
           if (!seen_c && !it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; ok = false; break; }
           const uint32_t at = smem_base + st * stage_bytes;
@@ -275,8 +302,9 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         int st = 0, e = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int u = first; u < total && ok; u += hop) {
-          const Tile tl = tile_at(u, e);
+        for (int n = 0; n < items && ok; ++n) {
+          const Item it = item_at(n);
+          const Tile tl = tile_at(it.u, e);
           const int mine = 4 * (lane >> 1) + 2 * (warp - 2) + (lane & 1);       // a lane keeps the number of one of its warp's rows
           int from = 0;
           if (mine < tl.valid) {
@@ -284,7 +312,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
             if (row < 0 || row >= p.x_rows) report_status(p.status, ST_BAD_INDEX, row);
             else from = row;
           }
-          for (int s = s0; s < s1; ++s) {
+          for (int s = it.s0; s < it.s1; ++s) {
             if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
               if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
               ok = false;
@@ -323,7 +351,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       int st = group, slot = group;
       uint32_t ph = 0, sph = 0, seen = 0;
       // (a step is a step here, whatever tile it belongs to)
-      const int n_steps = (total - first + hop - 1) / hop * (s1 - s0);
+      const int n_steps = SUB == 2 ? plan.n_steps : items * (s1 - s0);
       for (int s = group; s < n_steps; s += GROUPS) {
         if (!it_warp_wait(seen, smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
@@ -396,12 +424,13 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       int buf = 0, it = 0, e = 0;
       uint32_t bph = 0, seen = 0;
       bool ok = true;
-      for (int u = first; u < total; u += hop) {
+      for (int n = 0; n < items; ++n) {
+        const Item now = item_at(n);
 #pragma unroll
         for (int h = 0; h < SUB; ++h)
 #pragma unroll
           for (int c = 0; c < S::EPI_COLS / 2; ++c) acc[h][c] = 0ull;
-        for (int s = s0; s < s1 && ok; ++s, ++it) {
+        for (int s = now.s0; s < now.s1 && ok; ++s, ++it) {
 #pragma unroll
           for (int g = 0; g < GP; ++g) {
             if (!it_warp_wait(seen, smem_u32(&bar_dfull[buf]), bph, &abort_flag, p.budget_ns)) {
@@ -437,8 +466,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
             }
           }
         }
-        if (!ok || p.split > 1) break;
-        const Tile tl = tile_at(u, e);
+        if (!ok || (SUB == 2 ? plan.mine && n + 1 == items : p.split > 1)) break;
+        const Tile tl = tile_at(now.u, e);
         // (MMAs of the next tile wait for these warps once the accumulators are full: what is the same for all columns stays out of the loops)
 #pragma unroll
         for (int h = 0; h < SUB; ++h) {
@@ -453,6 +482,16 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
               const float y = of_pair(v.x, v.y);
               if (c < left) *to = __float2bfloat16(y);
               to += 2 * p.out_ld;
+            }
+          } else if (NT <= 32 && f32 && p.residual == nullptr) {        // (logits of a step)
+            float* to = (float*)p.out + at;
+#pragma unroll
+            for (int c = 0; c < S::EPI_COLS; c += 2) {
+              const float2 v = it_unpack(acc[h][c / 2]);
+              if (c < left) *to = v.x;
+              to += p.out_ld;
+              if (c + 1 < left) *to = v.y;
+              to += p.out_ld;
             }
           } else if (!f32 && p.residual == nullptr) {
             __nv_bfloat16* to = (__nv_bfloat16*)p.out + at;
@@ -477,11 +516,13 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
     }
   }
 
-  // ---- the pieces of a tile: every CTA finishes NT / split columns, summed in rank order
-  if (p.split > 1 && live) {
-    const bool epi = warp >= 4 + S::CONV_WARPS;
+  // ---- the pieces of a tile: every CTA finishes NT / share columns, summed in rank order
+  const int share = SUB == 2 ? plan.share : p.split;
+  if (share > 1) {        // (of every CTA or none)
+    const bool epi = (SUB == 2 ? plan.mine : items > 0) && warp >= 4 + S::CONV_WARPS;
+    const int rank = SUB == 2 ? (int)blockIdx.x % share : rank_of;
     const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS;
-    const int slice = NT / p.split;
+    const int slice = NT / share, base = (int)blockIdx.x % p.split - rank;      // base: the group's first CTA in the cluster
     float* recv = reinterpret_cast<float*>(smem_raw + (smem_base - smem_u32(smem_raw)));      // [rank][tile][slice][128], on stages that nothing reads any more
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
@@ -491,7 +532,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
 #pragma unroll
         for (int c = 0; c < S::EPI_COLS; c += 2) {       // (a slice is an even number of columns)
           const float2 v = it_unpack(acc[h][c / 2]);
-          float* to = cluster.map_shared_rank(recv, (col0 + c) / slice) + ((rank * SUB + h) * slice + (col0 + c) % slice) * 128 + r;
+          float* to = cluster.map_shared_rank(recv, base + (col0 + c) / slice) + ((rank * SUB + h) * slice + (col0 + c) % slice) * 128 + r;
           to[0] = v.x;
           to[128] = v.y;
         }
@@ -499,14 +540,14 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
     cluster.sync();
     if (epi && abort_flag == 0) {
       int e = 0;
-      const Tile tl = tile_at(first, e);
+      const Tile tl = tile_at(SUB == 2 ? plan.last : first, e);
       for (int h = 0; h < SUB; ++h) {
         const int m = tl.m * SUB + h, f = pair ? (m * 8 + (r >> 4)) * 8 + (r & 7) : m * 128 + r;
         for (int c = part * 2; c < slice; c += S::EPI_WARPS / 2) {
           const int col = rank * slice + c;
           if (col >= tl.valid) break;
           float a = 0.f, b = 0.f;
-          for (int q = 0; q < p.split; ++q) {
+          for (int q = 0; q < share; ++q) {
             a += recv[((q * SUB + h) * slice + c) * 128 + r];
             b += recv[((q * SUB + h) * slice + c + 1) * 128 + r];
           }
@@ -544,8 +585,14 @@ static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s
   const cudaError_t e = allow_smem(allowed, (const void*)int4_tc_kernel<NT, GP, SUB>, room);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg{};
-  // a cluster has one tile, else a CTA per place on the GPU walks them
-  cfg.gridDim = dim3(p.split > 1 ? (unsigned)tiles * p.split : (unsigned)min(tiles, S::ONE ? 148 : 296));
+  const int places = S::ONE ? 148 : 296;
+  const bool walk = p.split == 1;
+  // CTAs that stay. Of a dense product whose last round would leave half of them idle they come in pairs, which share its tiles (13 rows of 152064 x 3584: 84
+  // us, 93 without; not experts, whose tiles the host cannot count and whose unequal CTAs pairs slow down: 48 tokens of 64 experts 37 us, 31 without).
+  if (SUB == 2 && p.counts == nullptr && tiles > places && tiles % places != 0 && tiles % places <= places / 2) {
+    p.split = 2;
+    p.least = 4;
+  }
   cfg.blockDim = dim3(S::THREADS);
   cfg.dynamicSmemBytes = (size_t)p.stages * stage + 1024 + list;
   cfg.stream = s;
@@ -558,6 +605,7 @@ static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
+  cfg.gridDim = dim3((unsigned)(walk ? min(tiles, places) : tiles * p.split));
   return (int)cudaLaunchKernelEx(&cfg, int4_tc_kernel<NT, GP, SUB>, tmX, p);
 }
 template <int NT, int SUB>
@@ -598,7 +646,7 @@ extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, 
   const long long row_tiles = counts == nullptr ? (rows + n_tile - 1) / n_tile : (rows + (long long)(n_tile - 1) * (E < rows ? E : rows)) / n_tile;
   const long long expect_rows = counts == nullptr ? row_tiles : rows < E ? (long long)rows : (long long)E * ((rows_hint + n_tile - 1) / n_tile);
   // Two tiles of 16 rows at a time from where one each fills the GPU (1408 x 2048 pairs, 64 experts, mean 4.5: 79 us one at a time, 65 two; 152064 x 3584 100
-  // and 96; but 18944 x 2048, 148 tiles, 12.1 and 16.2).
+  // and 84; but 18944 x 2048, 148 tiles, 12.1 and 16.2).
   const bool two = n_tile == 16 && split <= 1 && p.w_tiles * expect_rows >= 296;
   p.m_tiles = two ? (p.w_tiles + 1) / 2 : p.w_tiles;
   const long long tiles = row_tiles * p.m_tiles;
@@ -613,6 +661,7 @@ extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, 
   if (split != 1 && split != 2 && split != 4 && split != 8) return -1;
   if (tiles * split > 0x7fffffffll) return -1;
   p.split = split;
+  p.least = 0;
   CUtensorMap tmX{};
   if (src_row == nullptr) {
     const int rc = make_tmap_2d(&tmX, x, (uint64_t)x_rows, (uint64_t)K, (uint64_t)x_ld, 2, n_tile);

@@ -242,6 +242,23 @@ def test_many_uneven_experts(cfg):
     ops.workspace().check_status()
 
 
+@pytest.mark.parametrize("tiles, last", [(2 * 296 + 1, 5), (2 * 296 + 4, 128), (2 * 296 + 296, 77), (4 * 296 + 40, 1), (2 * 296 + 300, 128)])
+def test_a_last_round_is_shared(tiles, last):
+    """Tiles that do not fill a round of the GPU's places, with and without CTAs that share them, an odd one and one of few rows among them."""
+    features, K = 128 * (tiles - 1) + last, 1088
+    w, full = weight((), features, K, 64, True, torch.bfloat16, False)
+    x = acts(14, K)
+    y = int4.linear(x, w, out_f32=True, _cfg=(16, 0))
+    within(y, x, full, half_step=2.0 ** -24)
+    assert torch.equal(y, int4.linear(x, w, out_f32=True, _cfg=(16, 0)))
+    r = torch.randn(14, features, device=DEV).bfloat16()
+    within(int4.linear(x, w, residual=r, _cfg=(16, 0)), x, full, residual=r)
+    del w, full
+    w, full = weight((), 2 * (features // 2), K, 32, False, torch.float16, True)
+    within(int4.swiglu_linear(x, w, _cfg=(16, 0)), x, full, True)
+    ops.workspace().check_status()
+
+
 @pytest.mark.parametrize("tile", [16, 32, 64, 128])
 @pytest.mark.parametrize("E, features, K, group, zeros, pair", [(60, 650, 1024, 128, False, False), (100, 392, 416, 32, True, True), (1024, 130, 192, 64, True, False),
                                                                 (7, 5400, 320, 64, False, True), (40, 1030, 2176, 128, True, False)])

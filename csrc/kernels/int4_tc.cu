@@ -16,7 +16,7 @@
 // conversion, the drains and seven of eight MMAs left out it still took 870. The MMAs of a step are 280 cycles with up to 64 rows of x and 512 with 128, the
 // weights' share of HBM is 365 cycles per SM. So with up to 64 rows two CTAs share an SM, with 16 rows two tiles of weights a step, handovers are whole
 // steps, and tests of barriers are issued before their answers are needed. Gathered rows are bounded by the two warps that copy them. Measured: 1000 rows of
-// gate / up 37888 x 3584 250 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 480 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 84 us (3.7 TB/s),
+// gate / up 37888 x 3584 243 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 467 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 83 us (3.7 TB/s),
 // 128 rows over 8 experts of 28672 x 4096, gathered, 169 us (2.9 TB/s).
 // Pieces of a tile meet in distributed shared memory in rank order: the result does not depend on timing, and no memory outlives the call.
 #include "int4.cuh"
@@ -107,8 +107,8 @@ struct ItShape {
   static_assert(SUB * (BUFS * ACC + SLOTS * 64) <= COLS && GROUPS * 4 * SUB == CONV_WARPS, "tensor memory");
 };
 
-// What a CTA does: `items` tiles, `hop` apart; of the last one steps s0 .. s1 (of the others all), with `share` CTAs of a cluster on it
-struct ItPlan { int items, hop, last, s0, s1, share, mine, n_steps; };
+// What a CTA does: `items` tiles, the last of them `last` with steps s0 .. s1 of it (of the others all) and `share` CTAs of a cluster on it
+struct ItPlan { int items, last, s0, s1, share, mine, n_steps; };
 
 template <int NT, int GP, int SUB>
 __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::ONE ? 1 : 2) int4_tc_kernel(const __grid_constant__ CUtensorMap tmX, const Int4Tc p) {
@@ -175,7 +175,6 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       while (share < p.split && left * share * 2 <= grid && p.steps >= p.least * share * 2) share *= 2;
       const int rank = me % share;
       const bool more = me / share < left;
-      plan.hop = grid;
       plan.items = rounds + more;
       plan.last = more ? rounds * grid + me / share : me + (rounds - 1) * grid;
       plan.s0 = more ? (int)((long long)p.steps * rank / share) : 0;
@@ -186,16 +185,15 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
     }
   }
   __syncthreads();
-  // The other shapes, which the plan costs registers in their loops (3 to 8 %), take tiles `hop` apart from `first`, the same steps of each; the CTAs of a
-  // cluster share all of theirs (one).
-  const int rank_of = (int)blockIdx.x % p.split, first = (int)blockIdx.x / p.split, hop = (int)gridDim.x / p.split, total = pre[p.E];
-  const int s0 = (int)((long long)p.steps * rank_of / p.split), s1 = (int)((long long)p.steps * (rank_of + 1) / p.split);
-  const int items = SUB == 2 ? plan.items : first < total ? (total - first + hop - 1) / hop : 0;
+  // The other shapes, which the plan would cost registers in their loops (3 to 8 %), take tiles `hop` apart from `first`, the same steps of each; the CTAs
+  // of a cluster share all of theirs (one).
+  const int total = pre[p.E], rank_of = SUB == 2 ? 0 : (int)blockIdx.x % p.split, first = SUB == 2 ? (int)blockIdx.x : (int)blockIdx.x / p.split;
+  const int hop = SUB == 2 ? (int)gridDim.x : (int)gridDim.x / p.split, end = SUB == 2 ? first + plan.items * hop : total;
+  const int s0 = SUB == 2 ? 0 : (int)((long long)p.steps * rank_of / p.split), s1 = SUB == 2 ? p.steps : (int)((long long)p.steps * (rank_of + 1) / p.split);
   struct Item { int u, s0, s1; };
-  auto item_at = [&](int n) {
-    if (SUB == 1) return Item{first + n * hop, s0, s1};
-    if (n + 1 < plan.items) return Item{(int)blockIdx.x + n * plan.hop, 0, p.steps};
-    return Item{plan.last, plan.s0, plan.s1};
+  auto item_at = [&](int u) {
+    if (SUB == 2 && u + hop >= end) return Item{plan.last, plan.s0, plan.s1};
+    return Item{u, s0, s1};
   };
   struct Tile { int e, m, row0, valid; };
   auto tile_at = [&](int u, int& e) {        // e: the expert of the role's tile before
@@ -216,7 +214,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
     return silu(g) * u;
   };
 
-  if (items > 0) {
+  if (first < end) {
     if (warp == 0) {
       // ================= producer =================
       if (elect_one()) {
@@ -225,8 +223,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         int st = 0, e = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int n = 0; n < items && ok; ++n) {
-          const Item it = item_at(n);
+        for (int u = first; u < end && ok; u += hop) {
+          const Item it = item_at(u);
           const Tile tl = tile_at(it.u, e);
           // (behind the last tile that one again, for nothing)
           const uint8_t* w = p.w + ((size_t)tl.e * p.w_tiles + tl.m * SUB) * p.steps * rec;
@@ -258,8 +256,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         int st = 0, slot = 0, buf = 0;
         uint32_t sph = 0, bph = 0, seen_c = 0, seen_d = 0;
         bool ok = true;
-        for (int n = SUB == 2 ? items - 1 : 0; n < items && ok; ++n)
-        for (int s = 0, n_steps = SUB == 2 ? plan.n_steps : s1 - s0; s < n_steps; ++s) {
+        for (int u = first; u < end && ok; u += hop)
+        for (int s = item_at(u).s0, to = item_at(u).s1; s < to; ++s) {
           // (the converters have seen the stage arrive, x included)
           if (!seen_c && !it_wait(smem_u32(&bar_cfull[slot]), sph, &abort_flag, p.budget_ns)) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; ok = false; break; }
           const uint32_t at = smem_base + st * stage_bytes;
@@ -302,8 +300,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         int st = 0, e = 0;
         uint32_t ph = 0;
         bool ok = true;
-        for (int n = 0; n < items && ok; ++n) {
-          const Item it = item_at(n);
+        for (int u = first; u < end && ok; u += hop) {
+          const Item it = item_at(u);
           const Tile tl = tile_at(it.u, e);
           const int mine = 4 * (lane >> 1) + 2 * (warp - 2) + (lane & 1);       // a lane keeps the number of one of its warp's rows
           int from = 0;
@@ -351,7 +349,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       int st = group, slot = group;
       uint32_t ph = 0, sph = 0, seen = 0;
       // (a step is a step here, whatever tile it belongs to)
-      const int n_steps = SUB == 2 ? plan.n_steps : items * (s1 - s0);
+      const int n_steps = SUB == 2 ? plan.n_steps : (total - first + hop - 1) / hop * (s1 - s0);
       for (int s = group; s < n_steps; s += GROUPS) {
         if (!it_warp_wait(seen, smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }
@@ -424,8 +422,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       int buf = 0, it = 0, e = 0;
       uint32_t bph = 0, seen = 0;
       bool ok = true;
-      for (int n = 0; n < items; ++n) {
-        const Item now = item_at(n);
+      for (int u = first; u < end; u += hop) {
+        const Item now = item_at(u);
 #pragma unroll
         for (int h = 0; h < SUB; ++h)
 #pragma unroll
@@ -466,7 +464,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
             }
           }
         }
-        if (!ok || (SUB == 2 ? plan.mine && n + 1 == items : p.split > 1)) break;
+        if (!ok || (SUB == 2 ? plan.mine && u + hop >= end : p.split > 1)) break;
         const Tile tl = tile_at(now.u, e);
         // (MMAs of the next tile wait for these warps once the accumulators are full: what is the same for all columns stays out of the loops)
 #pragma unroll
@@ -519,7 +517,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
   // ---- the pieces of a tile: every CTA finishes NT / share columns, summed in rank order
   const int share = SUB == 2 ? plan.share : p.split;
   if (share > 1) {        // (of every CTA or none)
-    const bool epi = (SUB == 2 ? plan.mine : items > 0) && warp >= 4 + S::CONV_WARPS;
+    const bool epi = (SUB == 2 ? plan.mine : first < end) && warp >= 4 + S::CONV_WARPS;
     const int rank = SUB == 2 ? (int)blockIdx.x % share : rank_of;
     const int r = (warp & 3) * 32 + lane, part = (warp - 4 - S::CONV_WARPS) >> 2, col0 = part * S::EPI_COLS;
     const int slice = NT / share, base = (int)blockIdx.x % p.split - rank;      // base: the group's first CTA in the cluster
@@ -587,7 +585,7 @@ static int launch_tc(const CUtensorMap& tmX, Int4Tc p, int tiles, cudaStream_t s
   cudaLaunchConfig_t cfg{};
   const int places = S::ONE ? 148 : 296;
   const bool walk = p.split == 1;
-  // CTAs that stay. Of a dense product whose last round would leave half of them idle they come in pairs, which share its tiles (13 rows of 152064 x 3584: 84
+  // CTAs that stay. Of a dense product whose last round would leave half of them idle they come in pairs, which share its tiles (13 rows of 152064 x 3584: 83
   // us, 93 without; not experts, whose tiles the host cannot count and whose unequal CTAs pairs slow down: 48 tokens of 64 experts 37 us, 31 without).
   if (SUB == 2 && p.counts == nullptr && tiles > places && tiles % places != 0 && tiles % places <= places / 2) {
     p.split = 2;
@@ -646,7 +644,7 @@ extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, 
   const long long row_tiles = counts == nullptr ? (rows + n_tile - 1) / n_tile : (rows + (long long)(n_tile - 1) * (E < rows ? E : rows)) / n_tile;
   const long long expect_rows = counts == nullptr ? row_tiles : rows < E ? (long long)rows : (long long)E * ((rows_hint + n_tile - 1) / n_tile);
   // Two tiles of 16 rows at a time from where one each fills the GPU (1408 x 2048 pairs, 64 experts, mean 4.5: 79 us one at a time, 65 two; 152064 x 3584 100
-  // and 84; but 18944 x 2048, 148 tiles, 12.1 and 16.2).
+  // and 83; but 18944 x 2048, 148 tiles, 12.1 and 16.2).
   const bool two = n_tile == 16 && split <= 1 && p.w_tiles * expect_rows >= 296;
   p.m_tiles = two ? (p.w_tiles + 1) / 2 : p.w_tiles;
   const long long tiles = row_tiles * p.m_tiles;

@@ -175,9 +175,11 @@ def _check(what, x, w: Int4Weight, pair, dims):
         raise ValueError(f"{what}: x is on {x.device}, the weight on {w.device}")
 
 
-def _check_out(what, out, rows, w, dtype):
+def _check_out(what, out, x, rows, w, dtype):
     if out.shape != (rows, w.features) or out.dtype != dtype or out.device != w.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
         raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
+    if rows and out.data_ptr() == x.data_ptr():
+        raise ValueError(f"{what}: out lies on x, which is read until the end")
 
 
 def _few_rows(hint: int, K: int, grouped: bool) -> bool:
@@ -207,7 +209,7 @@ def _status(device) -> int:
 def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags, cfg=None):
     """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, (0, team) of the kernel of few rows."""
     L, dev = _lib.lib(), w.device
-    xp, x_ld = x.data_ptr(), x.stride(0)
+    xp, x_ld = x.data_ptr(), x.stride(0) if x.shape[0] > 1 else w.K
     few = _few_rows(hint, w.K, counts is not None) if cfg is None else cfg[0] == 0
     args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.ptr, None if residual is None else residual.data_ptr(), out.data_ptr(),
             out.stride(0), None if counts is None else counts.data_ptr(), None if counts is None else offsets.data_ptr(), rows, x.shape[0], w.matrices,
@@ -225,7 +227,7 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
 
 def linear(x, w: Int4Weight, out=None, residual=None, out_f32=False, _cfg=None):
     """y[t, f] = sum_k x[t, k] W[f, k] (+ residual[t, f]) for bf16 x [T, K] (rows may be strided). out_f32: y and the residual are fp32, else both are
-    bf16. out may be the residual, or a run of columns of a wider matrix."""
+    bf16. out may be the residual, or a run of columns of a wider matrix, but not x."""
     _check("int4 linear", x, w, False, 2)
     return _dense("int4 linear", x, w, out, residual, out_f32, _cfg)
 
@@ -242,7 +244,7 @@ def _dense(what, x, w, out, residual, out_f32, cfg):
     if out is None:
         out = torch.empty((T, w.features), dtype=dtype, device=w.device)
     else:
-        _check_out(what, out, T, w, dtype)
+        _check_out(what, out, x, T, w, dtype)
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
                                  or residual.stride(1) != 1 or (T > 1 and residual.stride(0) != out.stride(0))):
         raise ValueError(f"{what}: the residual must have the result's shape, type and strides")
@@ -272,7 +274,7 @@ def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None
     if out is None:
         out = torch.empty((rows, w.features), dtype=torch.bfloat16, device=w.device)
     else:
-        _check_out(what, out, rows, w, torch.bfloat16)
+        _check_out(what, out, x, rows, w, torch.bfloat16)
     if rows == 0:
         return out
     if x.shape[0] == 0:

@@ -104,6 +104,7 @@ def test_product_refusals():
            lambda: int4.linear(x, one, residual=torch.zeros(4, 8)), lambda: int4.linear(x, one, residual=torch.zeros(8, 4, dtype=torch.bfloat16).t()),
            lambda: int4.grouped_linear(x, one, n, n), lambda: int4.grouped_linear(x, many, n.long(), n), lambda: int4.grouped_linear(x, many, n[:1], n),
            lambda: int4.grouped_linear(x, many, n, n, swiglu=True), lambda: int4.grouped_linear(x, many, n, n, src_row=n.long())]
+    bad += [lambda: int4.linear(x, one, out=x[:, :8]), lambda: int4.grouped_linear(x, many, n, n, out=x[:, :8])]
     for call in bad:
         with pytest.raises(ValueError):
             call()

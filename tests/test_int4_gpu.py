@@ -118,6 +118,9 @@ def test_long_rows():
         int4.grouped_linear(wide[:, 1:K + 1], w, cnt, off)
     w, full = weight((), 48, int4.MAX_ROW, 128, True, torch.bfloat16, False)
     within(int4.linear(wide[:, 1:int4.MAX_ROW + 1], w), wide[:, 1:int4.MAX_ROW + 1], full)
+    w, full = weight((), 16, K, 128, True, torch.bfloat16, False)
+    odd = wide.view(-1)[:2 * K + 1].as_strided((1, K), (K + 1, 1))      # the stride of one row says nothing
+    within(int4.linear(odd, w), odd, full)
     ops.workspace().check_status()
 
 

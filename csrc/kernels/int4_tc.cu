@@ -5,7 +5,7 @@
 //   producer    one bulk copy per step (codes, scales and zeros of 128 rows x 128 of K are one run) and TMA tiles of x into a ring of shared-memory
 //               stages
 //   gatherers   two warps that copy the rows of x which src_row names, 16 bytes a lane (tile::gather4 takes 55 to 80 cycles for four rows of 128 bytes:
-//               it bounded experts at 250 us where these take 170)
+//               it bounded experts at 250 us where these take 160)
 //   converters  a thread owns a row: eight codes of a word become four bf16 pairs code - zero (exact), 64 of K a slot, written to tensor
 //               memory as the A operand
 //   MMA         one thread; every group of K has an accumulator of its own (a ring of them)
@@ -17,7 +17,7 @@
 // weights' share of HBM is 365 cycles per SM. So with up to 64 rows two CTAs share an SM, with 16 rows two tiles of weights a step, handovers are whole
 // steps, and tests of barriers are issued before their answers are needed. Gathered rows are bounded by the two warps that copy them. Measured: 1000 rows of
 // gate / up 37888 x 3584 243 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 467 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 83 us (3.7 TB/s),
-// 128 rows over 8 experts of 28672 x 4096, gathered, 169 us (2.9 TB/s).
+// 128 rows over 8 experts of 28672 x 4096, gathered, 160 us (3.0 TB/s).
 // Pieces of a tile meet in distributed shared memory in rank order: the result does not depend on timing, and no memory outlives the call.
 #include "int4.cuh"
 #include "launch.cuh"
@@ -303,13 +303,19 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
         for (int u = first; u < end && ok; u += hop) {
           const Item it = item_at(u);
           const Tile tl = tile_at(it.u, e);
-          const int mine = 4 * (lane >> 1) + 2 * (warp - 2) + (lane & 1);       // a lane keeps the number of one of its warp's rows
+          // A lane looks one of its warp's rows up. Where the rows begin is kept for the tile; of tiles of 64, which have no registers for it, computed
+          // for eight copies at a time (one chain from shuffle to copy is 70 cycles).
+          const int mine = 4 * (lane >> 1) + 2 * (warp - 2) + (lane & 1);
           int from = 0;
           if (mine < tl.valid) {
             const int row = p.src_row[tl.row0 + mine];
             if (row < 0 || row >= p.x_rows) report_status(p.status, ST_BAD_INDEX, row);
             else from = row;
           }
+          constexpr int PASSES = NT < 128 ? NT / 4 : 1, KEPT = PASSES < 8 ? PASSES : 8;
+          const __nv_bfloat16* src[KEPT];
+#pragma unroll
+          for (int i = 0; i < KEPT && PASSES == KEPT; ++i) src[i] = p.x + (size_t)__shfl_sync(0xffffffffu, from, 2 * i + half) * p.x_ld;
           for (int s = it.s0; s < it.s1; ++s) {
             if (!it_warp_wait(0, smem_u32(&bar_empty[st]), ph ^ 1, &abort_flag, p.budget_ns)) {
               if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_EMPTY, blockIdx.x); abort_flag = 1; }
@@ -317,20 +323,21 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
               break;
             }
             const int k = s * I4_STEP + c * 8;             // (behind K zeros, as their scales are)
-            const __nv_bfloat16* x = p.x + (k < p.K ? k : 0);
+            const int at_k = k < p.K ? k : 0;
+            const __nv_bfloat16* x = p.x + at_k;
             const uint32_t bytes = k < p.K ? 16 : 0, to = smem_base + st * stage_bytes + (c >> 3) * NT * 128 + first_row * 128;
-            constexpr int PASSES = NT / 4, BATCH = PASSES < 8 ? PASSES : 8;       // addresses first: a chain from shuffle to copy is 70 cycles
 #pragma unroll
-            for (int i0 = 0; i0 < PASSES; i0 += BATCH) {
-              if (4 * i0 >= tl.valid) break;
-              const __nv_bfloat16* src[BATCH];
+            for (int i0 = 0; i0 < PASSES; i0 += KEPT) {
+              if (PASSES > KEPT) {
+                if (4 * i0 >= tl.valid) break;
 #pragma unroll
-              for (int i = 0; i < BATCH; ++i) src[i] = x + (size_t)__shfl_sync(0xffffffffu, from, 2 * (i0 + i) + half) * p.x_ld;
+                for (int i = 0; i < KEPT; ++i) src[i] = x + (size_t)__shfl_sync(0xffffffffu, from, 2 * (i0 + i) + half) * p.x_ld;
+              }
 #pragma unroll
-              for (int i = 0; i < BATCH; ++i) {
+              for (int i = 0; i < KEPT; ++i) {
                 const int at = 4 * (i0 + i);
                 // (rows of the stage behind the tile's last stay what they were: no result has them)
-                if (at + first_row < tl.valid) it_copy16(to + at * 128 + (((c & 7) ^ ((at + first_row) & 7)) << 4), src[i], bytes);
+                if (at + first_row < tl.valid) it_copy16(to + at * 128 + (((c & 7) ^ ((at + first_row) & 7)) << 4), PASSES > KEPT ? src[i] : src[i] + at_k, bytes);
               }
             }
             it_copy_arrive(smem_u32(&bar_full[st]));
@@ -624,8 +631,8 @@ extern "C" int skein_int4_tc(const void* x, long long x_ld, const int* src_row, 
   if (x_ld % 8 != 0 || (uintptr_t)x % 16 != 0 || (uintptr_t)w % 16 != 0) return -1;
   if (n_tile == 0) {
     // experts' rows differ: room for a quarter more than their mean, as a second tile of an expert converts its weights again. Measured, us, tiles of
-    // 16 / 32 / 64 rows: 28672 x 4096, 8 experts, mean 8 125 / 168 / 199, mean 16 181 / 170 / 199, mean 32 282 / 247 / 226; 2048 x 1408, 64 experts, mean 4.5
-    // 31 / 38 / 46, mean 12 45 / 42 / 51, mean 37 81 / 70 / 65.
+    // 16 / 32 / 64 rows: 28672 x 4096, 8 experts, mean 8 125 / 157 / 199, mean 16 179 / 160 / 199, mean 24 223 / 208 / 226; 2048 x 1408, 64 experts, mean
+    // 4.5 31 / 38 / 46, mean 12 45 / 42 / 51, mean 37 81 / 70 / 65.
     const int want = counts == nullptr ? rows_hint : rows_hint + rows_hint / 4;
     n_tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
   }

@@ -175,10 +175,35 @@ def _check(what, x, w: Int4Weight, pair, dims):
         raise ValueError(f"{what}: x is on {x.device}, the weight on {w.device}")
 
 
+def _meet(a, b) -> bool:
+    """Whether two matrices with contiguous rows share a byte. Rows of the same distance (columns of one buffer, every other row of it) are compared at once,
+    others row by row, and only where the spans meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    if a.shape[0] > b.shape[0]:
+        a, b = b, a
+    p, n, step, size = a.data_ptr(), a.shape[0], a.stride(0) * a.element_size(), a.shape[1] * a.element_size()
+    q, m, other, wide = b.data_ptr(), b.shape[0], b.stride(0) * b.element_size(), b.shape[1] * b.element_size()
+    if p + (n - 1) * step + size <= q or q + (m - 1) * other + wide <= p:
+        return False
+    if m == 1 or other == 0:        # (a row that repeats is one row)
+        m = other = 1
+    if n == 1 or step == 0:
+        n, step = 1, other
+    if step == other:               # rows i and j meet where (i - j) step lies between q - p - size and q - p + wide: the first that does
+        d = max((q - p - size) // step + 1, 1 - m)
+        return d < n and d * step < q - p + wide
+    for at in range(p, p + n * step, step):
+        j = max((at - wide - q) // other + 1, 0)
+        if j < m and q + j * other < at + size:
+            return True
+    return False
+
+
 def _check_out(what, out, x, rows, w, dtype):
     if out.shape != (rows, w.features) or out.dtype != dtype or out.device != w.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
         raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
-    if rows and out.data_ptr() == x.data_ptr():
+    if _meet(out, x):
         raise ValueError(f"{what}: out lies on x, which is read until the end")
 
 
@@ -227,13 +252,13 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
 
 def linear(x, w: Int4Weight, out=None, residual=None, out_f32=False, _cfg=None):
     """y[t, f] = sum_k x[t, k] W[f, k] (+ residual[t, f]) for bf16 x [T, K] (rows may be strided). out_f32: y and the residual are fp32, else both are
-    bf16. out may be the residual, or a run of columns of a wider matrix, but not x."""
+    bf16. out may be the residual, or a run of columns of a wider matrix, but shares no memory with x."""
     _check("int4 linear", x, w, False, 2)
     return _dense("int4 linear", x, w, out, residual, out_f32, _cfg)
 
 
 def swiglu_linear(x, w: Int4Weight, out=None, _cfg=None):
-    """silu(x Wg^T) * (x Wu^T) with both products from one pass over x; w is packed as a pair."""
+    """silu(x Wg^T) * (x Wu^T) with both products from one pass over x; w is packed as a pair; out as in `linear`."""
     _check("int4 swiglu_linear", x, w, True, 2)
     return _dense("int4 swiglu_linear", x, w, out, None, False, _cfg)
 

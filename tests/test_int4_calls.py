@@ -1,0 +1,63 @@
+"""Calls of the 4-bit products and of the balanced router that share memory, are copied or name rows that are not there, on the CPU."""
+import random
+
+import pytest
+import torch
+
+from skein_b200.ops import int4
+
+
+def small(lead=(), rows=16, K=64, pair=False, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (*lead, rows, K // 2), generator=gen, dtype=torch.uint8)
+    return int4.pack_weight(codes, torch.rand(*lead, rows, K // 64, generator=gen).bfloat16(), pair=pair)
+
+
+def test_meeting_matrices_are_found():
+    """Against the bytes themselves, over every kind of pair: columns and rows of one buffer, single and repeated rows, rows of other distances, two types."""
+    rng, found = random.Random(3), [0, 0]
+    buf = torch.zeros(400, dtype=torch.bfloat16)
+
+    def matrix():
+        rows, wide = rng.choice((1, 2, 3, 7)), rng.randint(1, 12)
+        step = rng.choice((0, 12, 12, 24, 24, 31)) if rng.random() < 0.8 else rng.randint(wide, 40)
+        t, first = (buf, rng.randint(0, 60)) if rng.random() < 0.7 else (buf.view(torch.float32), rng.randint(0, 30))
+        step = step if t is buf else step // 2
+        return t.as_strided((rows, wide), (step, 1), first + (rng.randint(0, 60) if t is buf else 0))
+
+    def bytes_of(t):
+        size = t.element_size()
+        return {t.data_ptr() + (r * t.stride(0) + c) * size + i for r in range(t.shape[0]) for c in range(t.shape[1]) for i in range(size)}
+    for _ in range(4000):
+        a, b = matrix(), matrix()
+        want = bool(bytes_of(a) & bytes_of(b))
+        assert int4._meet(a, b) == int4._meet(b, a) == want, (a.shape, a.stride(), a.storage_offset(), a.dtype, b.shape, b.stride(), b.storage_offset(), b.dtype)
+        found[want] += 1
+    assert min(found) > 500
+    assert not int4._meet(buf[:0].view(0, 4), buf[:8].view(2, 4)) and not int4._meet(buf[:8].view(2, 4), buf[:0].view(2, 0))
+
+
+def test_out_on_rows_of_x_is_refused():
+    one, many, pair = small(rows=16), small((2,), rows=16), small(rows=32, pair=True)
+    n, first = torch.tensor([2, 2], dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32)
+    buf = torch.zeros(6, 200, dtype=torch.bfloat16)
+    flat = torch.zeros(8, 64, dtype=torch.bfloat16)
+    for x, out in ((buf[:4, :64], buf[:4, 8:24]), (buf[:4, :64], buf[1:5, :16]), (buf[:4, 60:124], buf[2:, 50:66]), (buf[1:5, 40:104], buf[:4, 30:46]),
+                   (flat[:4], flat.view(-1)[192 + 63:].as_strided((4, 16), (16, 1))), (flat[::2], flat.view(16, 32)[1::4, 16:])):
+        for call in (lambda: int4.linear(x, one, out=out), lambda: int4.swiglu_linear(x, pair, out=out), lambda: int4.grouped_linear(x, many, n, first, out=out)):
+            with pytest.raises(ValueError, match="lies on x"):
+                call()
+    # as a result of other rows, with the rows named
+    with pytest.raises(ValueError, match="lies on x"):
+        int4.grouped_linear(flat[:1], many, n, first, src_row=torch.zeros(4, dtype=torch.int32), out=flat.view(-1)[32:].as_strided((4, 16), (16, 1)))
+
+
+def test_out_beside_x_is_taken():
+    one = small(rows=16)
+    buf = torch.randn(9, 200, generator=torch.Generator().manual_seed(1)).bfloat16()
+    want = int4.linear(buf[:4, :64].clone(), one)
+    for x, out in ((buf[:4, :64], buf[:4, 64:80]), (buf[:4, :64], buf[4:8, :16]), (buf[:4, :64], buf.view(-1)[800:].as_strided((4, 16), (16, 1))), (buf[:4, :64], buf[:4, 184:])):
+        assert torch.equal(int4.linear(x, one, out=out), want) and torch.equal(out, want)
+    rows = torch.zeros(8, 64, dtype=torch.bfloat16)
+    rows[::2] = buf[:4, :64]
+    assert torch.equal(int4.linear(rows[::2], one, out=rows[1::2, 5:21]), want)

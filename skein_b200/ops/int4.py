@@ -252,7 +252,7 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
 
 def linear(x, w: Int4Weight, out=None, residual=None, out_f32=False, _cfg=None):
     """y[t, f] = sum_k x[t, k] W[f, k] (+ residual[t, f]) for bf16 x [T, K] (rows may be strided). out_f32: y and the residual are fp32, else both are
-    bf16. out may be the residual, or a run of columns of a wider matrix, but shares no memory with x."""
+    bf16. out may be a run of columns of a wider matrix; it shares no memory with x, nor with the residual unless it is the residual."""
     _check("int4 linear", x, w, False, 2)
     return _dense("int4 linear", x, w, out, residual, out_f32, _cfg)
 
@@ -273,6 +273,8 @@ def _dense(what, x, w, out, residual, out_f32, cfg):
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
                                  or residual.stride(1) != 1 or (T > 1 and residual.stride(0) != out.stride(0))):
         raise ValueError(f"{what}: the residual must have the result's shape, type and strides")
+    if residual is not None and residual.data_ptr() != out.data_ptr() and _meet(residual, out):
+        raise ValueError(f"{what}: the residual is out itself or lies beside it")
     if T == 0:
         return out
     if not x.is_cuda:

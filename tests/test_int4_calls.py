@@ -61,3 +61,20 @@ def test_out_beside_x_is_taken():
     rows = torch.zeros(8, 64, dtype=torch.bfloat16)
     rows[::2] = buf[:4, :64]
     assert torch.equal(int4.linear(rows[::2], one, out=rows[1::2, 5:21]), want)
+
+
+def test_a_residual_is_out_or_beside_it():
+    one = small(rows=16)
+    x = torch.randn(4, 64, generator=torch.Generator().manual_seed(2)).bfloat16()
+    buf = torch.randn(9, 40, generator=torch.Generator().manual_seed(3)).bfloat16()
+    for r, out in ((buf[1:5, :16], buf[:4, :16]), (buf[:4, 5:21], buf[:4, :16]), (buf[:4, 30:].as_strided((4, 16), (40, 1)), buf[1:5, :16])):
+        with pytest.raises(ValueError, match="residual"):
+            int4.linear(x, one, out=out, residual=r)
+    with pytest.raises(ValueError, match="residual"):      # one row
+        int4.linear(x[:1], one, out=buf[:1, :16], residual=buf[:1, 15:31])
+    keep = buf.clone()
+    want = int4.linear(x, one, residual=keep[:4, 16:32].contiguous())
+    assert torch.equal(int4.linear(x, one, out=buf[:4, :16], residual=buf[:4, 16:32]), want)
+    assert torch.equal(int4.linear(x, one, out=buf[:4, 16:32], residual=buf[:4, 16:32]), want)
+    wide = torch.randn(4, 16)
+    assert torch.equal(int4.linear(x[:1], one, out=wide[:1], residual=wide[:1].as_strided((1, 16), (3, 1)), out_f32=True), wide[:1])

@@ -9,14 +9,13 @@
 // this kind has the 64-bit rate for it. A logit that is not a number counts as the lowest; logits and biases are clamped to +-3e38, so that no
 // input makes an index invalid.
 //
-// A warp owns a token. Choices are kept as ordered 64-bit integers, whose last four bits give way to the expert's place in its lane (two choices within 16
-// units in the last place count as equal); a lane sorts its own, and a round of the choice is a maximum over the lanes' heads: one instruction on
-// the upper halves, two more where several lanes have the largest. Without the order a round compared all of them again (4096 tokens, 256 experts:
+// A warp owns a token. Choices are kept as ordered 64-bit integers, all bits of them; a lane sorts its own with their places beside them, and a round of the
+// choice is a maximum over the lanes' heads: one instruction on the upper halves, two more where several lanes have the largest, and a minimum of the
+// places where they are equal. Without the order a round compared all of them again (4096 tokens, 256 experts:
 // 3250 instructions per token, 35 us). The layout is a counting sort that keeps the tokens' order: for every expert a CTA has one bit per token of its
 // tile, so that a pair's place among the tile's is a count of bits, whatever order the warps came in. Up to 256 tokens the tiles are the CTAs of one
 // cluster, which add their counts up in distributed shared memory; beyond, the first kernel leaves the tiles' counts in memory and a second one
-// finishes the places. One token takes 6.6 us with 128 experts, 64 tokens 7.1 with 64 and 12.0 with 256, 4096 tokens 27.4: a token is about 2200
-// instructions, 230 of them 64-bit ones.
+// finishes the places. One token takes 6.7 us with 128 experts, 64 tokens 7.2 with 64, 12.6 with 256 and 19.3 with 512, 4096 tokens of 256 26.1.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include <cooperative_groups.h>
@@ -54,31 +53,40 @@ __device__ __forceinline__ float rb_clamp(float v) { return fminf(fmaxf(v, -3e38
 __device__ __forceinline__ double rb_max(double a, double b) { return a > b ? a : b; }
 __device__ __forceinline__ double rb_min(double a, double b) { return a > b ? b : a; }
 
-// The lane whose key is the largest, the lowest of several.
-__device__ __forceinline__ int rb_first(unsigned long long key) {
+// The lane whose key is the largest; of several the one with the lowest place, of those the lowest lane.
+__device__ __forceinline__ int rb_first(unsigned long long key, unsigned place) {
   const unsigned hi = (unsigned)(key >> 32), mh = __reduce_max_sync(0xffffffffu, hi);
   unsigned who = __ballot_sync(0xffffffffu, hi == mh);
   if (who & (who - 1)) {
     const unsigned lo = hi == mh ? (unsigned)key : 0u, ml = __reduce_max_sync(0xffffffffu, lo);
-    who = __ballot_sync(0xffffffffu, hi == mh && lo == ml);
+    const bool in = hi == mh && lo == ml;
+    who = __ballot_sync(0xffffffffu, in);
+    if (who & (who - 1)) {
+      const unsigned at = in ? place : ~0u, first = __reduce_min_sync(0xffffffffu, at);
+      who = __ballot_sync(0xffffffffu, in && at == first);
+    }
   }
   return __ffs(who) - 1;
 }
-// Descending order of N (a power of two) keys: merges of ever longer runs, the second of two turned round.
+// Descending order of N (a power of two) keys, equal ones by their places: Batcher's odd-even merges, which have fewer exchanges than bitonic ones (19 for 24
+// with 8 keys, 63 for 80 with 16).
 template <int N>
-__device__ __forceinline__ void rb_sort(unsigned long long (&k)[N]) {
+__device__ __forceinline__ void rb_sort(unsigned long long (&k)[N], unsigned (&place)[N]) {
 #pragma unroll
-  for (int run = 2; run <= N; run *= 2)
+  for (int run = 1; run < N; run *= 2)
 #pragma unroll
-    for (int hop = run / 2; hop > 0; hop /= 2)
+    for (int hop = run; hop > 0; hop /= 2)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int j = hop == run / 2 ? (i & ~(run - 1)) + run - 1 - (i & (run - 1)) : i ^ hop;
-        if (j <= i) continue;
-        const bool turn = k[j] > k[i];
+        const int j = i + hop;
+        if (i < hop % run || ((i - hop % run) & hop) || j >= N || i / (2 * run) != j / (2 * run)) continue;
+        const bool turn = k[j] > k[i] || (k[j] == k[i] && place[j] < place[i]);
         const unsigned long long a = turn ? k[j] : k[i], b = turn ? k[i] : k[j];
+        const unsigned c = turn ? place[j] : place[i], d = turn ? place[i] : place[j];
         k[i] = a;
         k[j] = b;
+        place[i] = c;
+        place[j] = d;
       }
 }
 
@@ -120,7 +128,7 @@ __device__ __forceinline__ void rb_token(const RouteBalanced& p, int t, int slot
     key[q] = 0ull;
     if (e < p.E) {
       const double c = p.bias != nullptr ? s[q] + (double)rb_clamp(p.bias[e]) : s[q];
-      key[q] = (rb_key(c) & ~15ull) | (unsigned)(15 - q);
+      key[q] = rb_key(c);
       if (p.keep < p.groups) pool[e] = c;
     }
   }
@@ -163,7 +171,7 @@ __device__ __forceinline__ void rb_token(const RouteBalanced& p, int t, int slot
     for (int k = 0; k < p.keep; ++k) {
       // the lower group where two are equal: of a lane's two the first, of several lanes' first ones the lowest before any second one
       const unsigned long long first = worth[0], second = p.groups > 32 ? worth[1] : 0ull;
-      const int l = rb_first(first > second ? first : second);
+      const int l = rb_first(first > second ? first : second, 0u);
       const bool up = __shfl_sync(0xffffffffu, first >= second ? 0 : 1, l);
       int got = l + (up ? 32 : 0);
       if (p.groups > 32) {
@@ -182,7 +190,13 @@ __device__ __forceinline__ void rb_token(const RouteBalanced& p, int t, int slot
       if (e < p.E && !((kept >> of) & 1ull)) key[q] = 0ull;
     }
   }
-  rb_sort<PER>(key);
+  unsigned place[PER];
+#pragma unroll
+  for (int q = 0; q < PER; ++q) place[q] = q;
+  rb_sort<PER>(key, place);
+  unsigned long long places = 0;       // four bits each, in order
+#pragma unroll
+  for (int q = 0; q < PER; ++q) places |= (unsigned long long)place[q] << (4 * q);
   __syncwarp();                // the pool's choices are read
   unsigned long long* list = reinterpret_cast<unsigned long long*>(pool);
 #pragma unroll
@@ -190,10 +204,12 @@ __device__ __forceinline__ void rb_token(const RouteBalanced& p, int t, int slot
   unsigned long long head = key[0];
   int next = 1, my_id = 0;
   for (int j = 0; j < p.top; ++j) {
-    const int l = rb_first(head);
-    const int e = (15 - (int)(__shfl_sync(0xffffffffu, (unsigned)head, l) & 15u)) * 32 + l;
+    const unsigned at = (unsigned)places & 15u;
+    const int l = rb_first(head, at);
+    const int e = (int)__shfl_sync(0xffffffffu, at, l) * 32 + l;
     if (lane == l) {
       head = next < PER ? list[next * 32 + lane] : 0ull;
+      places >>= 4;
       ++next;
     }
     if (lane == j) my_id = e;

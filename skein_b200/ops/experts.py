@@ -20,9 +20,8 @@ def route_balanced(logits, top, bias=None, groups=1, keep=1, score="sigmoid", gr
 
     s is the sigmoid or the softmax of the logits, c = s + bias (fp32 [E]). With groups > keep, the experts are `groups` equal groups of neighbours, a
     group is worth the sum of its `group_best` (1 or 2) largest c, and the `keep` best groups are eligible. The `top` largest c are chosen in descending
-    order, ties to the lower index; their weights are scale * s, divided by the sum of the chosen s (+ 1e-20) with renorm. Scores and choices are 64-bit
-    (choices within 16 units in the last place of each other count as equal); logits and biases that are not numbers count as the lowest, infinite ones as
-    +-3e38.
+    order, ties to the lower index; their weights are scale * s, divided by the sum of the chosen s (+ 1e-20) with renorm. Scores and choices are 64-bit;
+    logits and biases that are not numbers count as the lowest, infinite ones as +-3e38.
 
     Returns (ids int32 [T, top], weights fp32 [T, top], counts [E], offsets [E + 1], row_of [T * top], src_token [T * top]) as `ops.route` does: pair
     (t, j) sits at row_of[t * top + j] of the expert-sorted rows (-1: an expert outside e_first .. + e_count), src_token is its inverse; rows of

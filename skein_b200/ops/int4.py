@@ -27,14 +27,26 @@ class Int4Weight:
     def __init__(self, data, shape, group, pair, scales, zeros):
         self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
         self.scales, self.zeros = scales, zeros
-        self.device, self.K = data.device, shape[-1]
-        self.ptr, self.matrices = data.data_ptr(), data.shape[0]
+        self.K = shape[-1]
         self.features = shape[-2] // 2 if pair else shape[-2]
         self.flags = int(pair) | (2 if scales == torch.float16 else 0) | (8 if zeros else 0)
 
+    # (asked of the storage each time: a copied, pickled or moved weight has another one)
     @property
     def is_cuda(self):
         return self.data.is_cuda
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def ptr(self):
+        return self.data.data_ptr()
+
+    @property
+    def matrices(self):
+        return self.data.shape[0]
 
     def nbytes(self) -> int:
         return self.data.numel()

@@ -1,4 +1,6 @@
 """Calls of the 4-bit products and of the balanced router that share memory, are copied or name rows that are not there, on the CPU."""
+import copy
+import io
 import random
 
 import pytest
@@ -78,3 +80,16 @@ def test_a_residual_is_out_or_beside_it():
     assert torch.equal(int4.linear(x, one, out=buf[:4, 16:32], residual=buf[:4, 16:32]), want)
     wide = torch.randn(4, 16)
     assert torch.equal(int4.linear(x[:1], one, out=wide[:1], residual=wide[:1].as_strided((1, 16), (3, 1)), out_f32=True), wide[:1])
+
+
+def test_a_copied_or_pickled_weight_has_its_own_address():
+    w = small((2,), 16, 128)
+    file = io.BytesIO()
+    torch.save(w, file)
+    file.seek(0)
+    for other in (copy.deepcopy(w), torch.load(file, weights_only=False)):
+        assert other.data.data_ptr() != w.data.data_ptr() and other.ptr == other.data.data_ptr()
+        assert torch.equal(other.dequant(), w.dequant()) and other.device == w.device and other.matrices == 2
+    moved = copy.copy(w)
+    moved.data = w.data.to("meta")
+    assert moved.device.type == "meta" and not moved.is_cuda and w.device.type == "cpu"

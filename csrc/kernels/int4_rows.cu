@@ -338,13 +338,15 @@ static int pick_group(const Int4Rows& p, int group, bool zero, bool half, int te
 
 // x [x_rows, x_ld] bf16 (row r of the product reads row src_row[r], or r); w as in int4.cuh; out and residual [rows, out_ld] bf16
 // or fp32. counts / offsets null: one matrix for all rows. rows_hint: rows expected of an expert. flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
-// team: warps that share a strip (1, 4, 8 or 16, at most its steps), 0: by the rule above. Returns -1 for what it does not take (more than IR_MAX_E experts, or a row of x past the shared memory: K of 94,000).
+// team: warps that share a strip (1, 4, 8 or 16, at most its steps), 0: by the rule above. Returns -1 for what it does not take (more than IR_MAX_E experts,
+// a weight off 16-byte boundaries, or a row of x past the shared memory: K of 94,000).
 extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld,
                                const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int rows_hint, int flags, int team,
                                int* status, void* stream) {
   using namespace skein;
   if (rows == 0) return 0;
   if (rows < 0 || E < 1 || E > IR_MAX_E || F < 1 || K < 32 || K % group != 0 || (group != 32 && group != 64 && group != 128)) return -1;
+  if ((uintptr_t)w % 16 != 0) return -1;
   Int4Rows p;
   p.x = (const __nv_bfloat16*)x; p.src_row = src_row; p.w = (const uint8_t*)w; p.residual = residual; p.out = out; p.counts = counts;
   p.offsets = offsets; p.status = status; p.x_ld = x_ld; p.out_ld = out_ld; p.rows = rows; p.x_rows = x_rows; p.E = E; p.F = F; p.K = K;

@@ -20,11 +20,29 @@ MAX_EXPERTS = 1024
 MAX_ROW = 1 << 16       # of K in the kernel of few rows, which keeps whole rows of x in shared memory
 
 
+def _data_shape(shape, group, pair, scales, zeros):
+    """Of the packed weight [rows, K] or [experts, rows, K]."""
+    if len(shape) not in (2, 3) or min(shape) < 1 or group not in GROUPS or shape[-1] % group:
+        raise ValueError(f"int4 weight: [rows, K] or [experts, rows, K] with K a multiple of the group ({GROUPS}), not {tuple(shape)} in groups of {group}")
+    n, rows = shape[0] if len(shape) == 3 else 1, shape[-2]
+    if n > MAX_EXPERTS:
+        raise ValueError(f"int4 weight: at most {MAX_EXPERTS} experts")
+    if pair and rows % 2:
+        raise ValueError("int4 weight: a pair has as many up rows as gate rows")
+    if scales not in (torch.bfloat16, torch.float16):
+        raise ValueError("int4 weight: scales are bf16 or fp16")
+    tiles = -(-rows // 2 // 64) if pair else -(-rows // 128)
+    return (n, tiles, -(-shape[-1] // STEP), 8 * (CODES + STEP // group * (48 if zeros else 32)))
+
+
 class Int4Weight:
     """data uint8 [matrices, tiles, steps, bytes]: codes, scales and zeros of 128 rows x 128 of K (csrc/kernels/int4.cuh). `shape` is the logical [rows, K]
     or [experts, rows, K]; `pair`: gate rows, then up rows, packed side by side for the SwiGLU product."""
 
     def __init__(self, data, shape, group, pair, scales, zeros):
+        want = _data_shape(shape, group, pair, scales, zeros)
+        if data.dtype != torch.uint8 or data.shape != want or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"int4 weight: data must be contiguous uint8 {want} on a 16-byte boundary")
         self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
         self.scales, self.zeros = scales, zeros
         self.K = shape[-1]
@@ -130,18 +148,14 @@ def pack_weight(codes, scale, zero=None, pair=False) -> Int4Weight:
             raise ValueError("int4 weight: zero must be uint8 of scale's shape")
         if int(zero.max()) > 15:
             raise ValueError("int4 weight: zeros are 0 .. 15")
-    if pair and rows % 2:
-        raise ValueError("int4 weight: a pair has as many up rows as gate rows")
     if any(t is not None and t.device != codes.device for t in (scale, zero)):
         raise ValueError("int4 weight: codes, scale and zero lie on different devices")
-    n = lead[0] if lead else 1
-    if n > MAX_EXPERTS:
-        raise ValueError(f"int4 weight: at most {MAX_EXPERTS} experts")
-    S, B = -(-rows // 128) * 8 if not pair else -(-rows // 2 // 64) * 8, -(-K // STEP)
+    n, tiles, B, _ = size = _data_shape((*lead, rows, K), group, pair, scale.dtype, zero is not None)
+    S = 8 * tiles
     w = _rows_in(_deinterleave(codes.reshape(n, rows, half).contiguous().view(torch.int32)), pair, S)        # [n, S, half, g, K / 8]
     w = torch.nn.functional.pad(w, (0, B * 16 - w.shape[-1])) if w.shape[-1] < B * 16 else w
     per = STEP // group
-    data = codes.new_empty(n, S // 8, B, 8 * (CODES + per * (48 if zero is not None else 32)))
+    data = codes.new_empty(size)
     to = data[..., :8 * CODES].view(torch.int32).view(n, S // 8, B, 8, 2, 4, 8, 2, 2)                        # [n, tile, B, strip, j, t, g, half, h]
     to.copy_(w.reshape(n, S // 8, 8, 2, 8, B, 2, 2, 4).permute(0, 1, 5, 2, 6, 8, 4, 3, 7))
 

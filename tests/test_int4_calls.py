@@ -93,3 +93,19 @@ def test_a_copied_or_pickled_weight_has_its_own_address():
     moved = copy.copy(w)
     moved.data = w.data.to("meta")
     assert moved.device.type == "meta" and not moved.is_cuda and w.device.type == "cpu"
+
+
+def test_a_weight_made_from_other_storage_is_checked():
+    w = small((3,), 32, 128, pair=True)
+    make = lambda data, shape=w.shape, group=64, pair=True, scales=torch.bfloat16, zeros=False: int4.Int4Weight(data, shape, group, pair, scales, zeros)      # noqa: E731
+    buf = torch.zeros(w.nbytes() + 64, dtype=torch.uint8)
+    first = -buf.data_ptr() % 16
+    at = buf[first + 16:first + 16 + w.nbytes()].view(w.data.shape)
+    at.copy_(w.data)
+    assert torch.equal(make(at).dequant(), w.dequant())
+    bad = [dict(data=buf[first + 8:first + 8 + w.nbytes()].view(w.data.shape)), dict(data=w.data[:2]), dict(data=w.data.to(torch.int8)), dict(data=w.data, shape=(3, 32, 256)),
+           dict(data=w.data, shape=(3, 200, 128)), dict(data=w.data, group=32), dict(data=w.data, group=48), dict(data=w.data, zeros=True), dict(data=w.data, shape=(3, 31, 128)),
+           dict(data=w.data.expand(3, 1, 1, -1)[:1].expand(3, 1, 1, w.data.shape[-1])), dict(data=w.data, scales=torch.float32), dict(data=w.data, shape=(32, 128))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            make(**kw)

@@ -152,7 +152,10 @@ def pack_weight(codes, scale, zero=None, pair=False) -> Int4Weight:
         raise ValueError("int4 weight: codes, scale and zero lie on different devices")
     n, tiles, B, _ = size = _data_shape((*lead, rows, K), group, pair, scale.dtype, zero is not None)
     S = 8 * tiles
-    w = _rows_in(_deinterleave(codes.reshape(n, rows, half).contiguous().view(torch.int32)), pair, S)        # [n, S, half, g, K / 8]
+    codes = codes.reshape(n, rows, half).contiguous()
+    if codes.storage_offset() % 4:           # (a part of a buffer of bytes)
+        codes = codes.clone()
+    w = _rows_in(_deinterleave(codes.view(torch.int32)), pair, S)                                            # [n, S, half, g, K / 8]
     w = torch.nn.functional.pad(w, (0, B * 16 - w.shape[-1])) if w.shape[-1] < B * 16 else w
     per = STEP // group
     data = codes.new_empty(size)

@@ -109,3 +109,14 @@ def test_a_weight_made_from_other_storage_is_checked():
     for kw in bad:
         with pytest.raises(ValueError):
             make(**kw)
+
+
+@pytest.mark.parametrize("first", [0, 1, 2, 4, 7])
+def test_codes_may_begin_at_any_byte(first):
+    gen = torch.Generator().manual_seed(9)
+    codes, scale = torch.randint(0, 256, (2, 6, 48), generator=gen, dtype=torch.uint8), torch.rand(2, 6, 3, generator=gen).bfloat16()
+    buf = torch.empty(first + codes.numel(), dtype=torch.uint8)
+    part = buf[first:].view(codes.shape)
+    part.copy_(codes)
+    assert torch.equal(int4.pack_weight(part, scale).data, int4.pack_weight(codes, scale).data)
+    assert torch.equal(int4.pack_weight(part[1], scale[1]).dequant(), int4.pack_weight(codes, scale).dequant()[1])

@@ -26,10 +26,14 @@ def product(x, w, residual=None, out_f32=False, swiglu=False):
 
 def grouped_product(x, w, counts, offsets, swiglu, src_row, out):
     """Rows offsets[e] .. + counts[e] of `out` from rows of x (by src_row, or the same ones); the others stay."""
-    for e, (c, o) in enumerate(zip(counts.tolist(), offsets.tolist())):
-        if c:
-            rows = x[o:o + c] if src_row is None else x[src_row[o:o + c].long()]
-            out[o:o + c] = product(rows, w[e], swiglu=swiglu)
+    ends = [(e, o, o + c) for e, (c, o) in enumerate(zip(counts.tolist(), offsets.tolist())) if c]
+    for e, a, b in ends:
+        named = src_row[max(a, 0):max(b, 0)] if src_row is not None else None
+        if a < 0 or b < a or b > out.shape[0] or (named is not None and bool(((named < 0) | (named >= x.shape[0])).any())):
+            raise ValueError(f"int4 grouped_linear: index out of range at expert {e}")
+    for e, a, b in ends:
+        rows = x[a:b] if src_row is None else x[src_row[a:b].long()]
+        out[a:b] = product(rows, w[e], swiglu=swiglu)
     return out
 
 

@@ -120,3 +120,18 @@ def test_codes_may_begin_at_any_byte(first):
     part.copy_(codes)
     assert torch.equal(int4.pack_weight(part, scale).data, int4.pack_weight(codes, scale).data)
     assert torch.equal(int4.pack_weight(part[1], scale[1]).dequant(), int4.pack_weight(codes, scale).dequant()[1])
+
+
+def test_rows_outside_are_refused():
+    """What a GPU call reports in the workspace's status."""
+    w = small((2,), 16, 64)
+    x, out = torch.ones(4, 64, dtype=torch.bfloat16), torch.full((4, 16), 3.0, dtype=torch.bfloat16)
+    n, first = torch.tensor([2, 2], dtype=torch.int32), torch.tensor([0, 2], dtype=torch.int32)
+    src = torch.tensor([0, 3, 1, 2], dtype=torch.int32)
+    for counts, offsets, rows in ((n, first, src - 1), (n, first, src + 1), (n + 1, first, None), (n, first - 1, None), (n, first + 1, src), (n - 3, first, None)):
+        with pytest.raises(ValueError, match="out of range"):
+            int4.grouped_linear(x, w, counts, offsets, src_row=rows, out=out)
+    assert bool((out == 3).all())
+    unset = torch.tensor([1, 2, -7, 90], dtype=torch.int32)              # rows that no expert covers
+    int4.grouped_linear(x, w, torch.tensor([2, 0], dtype=torch.int32), torch.tensor([0, -5], dtype=torch.int32), src_row=unset, out=out)
+    assert bool((out[2:] == 3).all()) and not bool((out[:2] == 3).any())

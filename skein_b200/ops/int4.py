@@ -265,14 +265,17 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
     L, dev = _lib.lib(), w.device
     xp, x_ld = x.data_ptr(), x.stride(0) if x.shape[0] > 1 else w.K
     few = _few_rows(hint, w.K, counts is not None) if cfg is None else cfg[0] == 0
+    if xp % 16 or x_ld % 8:
+        if w.K > MAX_ROW:
+            raise ValueError(f"{what}: rows of x off 16-byte boundaries have at most {MAX_ROW} elements, not {w.K}")
+        if not few:     # (few rows are read two bytes at a time; 1000 rows of gate / up 18944 x 3584 so took 1770 us, laid out anew 253)
+            x = x.clone(memory_format=torch.contiguous_format)
+            xp, x_ld = x.data_ptr(), w.K
     args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.ptr, None if residual is None else residual.data_ptr(), out.data_ptr(),
             out.stride(0), None if counts is None else counts.data_ptr(), None if counts is None else offsets.data_ptr(), rows, x.shape[0], w.matrices,
             w.features, w.K, w.group, hint, flags)
-    aside = xp % 16 != 0 or x_ld % 8 != 0
-    if aside and w.K > MAX_ROW:
-        raise ValueError(f"{what}: rows of x off 16-byte boundaries have at most {MAX_ROW} elements, not {w.K}")
-    if few or aside:
-        rc = L.skein_int4_rows(*args, cfg[1] if cfg and few else 0, _status(dev), _lib.stream_on(dev))
+    if few:
+        rc = L.skein_int4_rows(*args, cfg[1] if cfg else 0, _status(dev), _lib.stream_on(dev))
     else:
         rc = L.skein_int4_tc(*args, *(cfg or (0, 0)), _status(dev), _lib.stream_on(dev))
     _lib.check(rc, what)

@@ -32,7 +32,7 @@ struct Int4Rows {
   int* status;
   long long x_ld, out_ld;
   uint64_t budget_ns;
-  int rows, x_rows, E, F, K, tiles, strips, steps, out_f32, vec, pair, x_stage;   // x_stage: rows of a tile (8 NT, or as many as fit a team's shared memory)
+  int rows, x_rows, E, F, K, strips, steps, out_f32, vec, pair, x_stage;   // x_stage: rows of a tile (8, or as many as fit a team's shared memory)
 };
 
 // bytes of a row of x in shared memory: 64 past a multiple of 128, so that eight rows x 64 bytes lie in different banks
@@ -82,11 +82,11 @@ struct Int4Step {       // a lane's part of a step of one strip
   }
 };
 
-template <int NT, int GP, bool ZERO, bool HALF, int WK>
+template <int GP, bool ZERO, bool HALF, int WK>
 __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_constant__ Int4Rows p) {
   constexpr int TEAMS = IR_WARPS / WK, REC = i4_record(GP, ZERO);
   extern __shared__ __align__(16) uint8_t x_smem[];
-  __shared__ float4 sums[2][IR_WARPS][NT][32];
+  __shared__ float4 sums[2][IR_WARPS][32];
   __shared__ int pre[IR_MAX_E + 1], cnt[IR_MAX_E];      // row tiles before an expert, its rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   __shared__ __align__(8) uint64_t bar[TEAMS];          // a team's sums of a strip are parked
@@ -161,36 +161,33 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_c
   uint8_t* x_team = x_smem + (size_t)team * p.x_stage * x_row;
   int e = 0, i = 0, n_done = 0, valid = 0, row0 = 0, old_valid = 0, old_row0 = 0, old_strip = 0;
   int left = u1 - u0, tile = u0 / p.strips, staged = -1, strip = u0 - tile * p.strips;
-  const uint8_t* xb[NT];
-  float acc[NT][4];
+  const uint8_t* xb = nullptr;
+  float acc[4];
   // adds up the team's sums of the strip before (its turn goes round the warps) and stores them
   auto finish = [&]() {
+    if ((n_done - 1) % WK != part) return;
+    float4 (*parked)[32] = sums[(n_done - 1) & 1] + team * WK;
+    float4 v = parked[0][lane];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if ((n_done - 1 + n) % WK != part) continue;
-      float4 (*parked)[NT][32] = sums[(n_done - 1) & 1] + team * WK;
-      float4 v = parked[0][n][lane];
+    for (int w = 1; w < WK; ++w) {
+      const float4 o = parked[w][lane];
+      v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+    }
+    // v: (row g, x rows 2t and 2t + 1), (row g + 8, the same)
 #pragma unroll
-      for (int w = 1; w < WK; ++w) {
-        const float4 o = parked[w][n][lane];
-        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-      }
-      // v: (row g, x rows 2t and 2t + 1), (row g + 8, the same)
+    for (int j = 0; j < 2; ++j) {
+      const int r = 2 * t + j;
+      if (r >= old_valid) continue;
+      const float a = 64.f * (j ? v.y : v.x), b = 64.f * (j ? v.w : v.z);       // (the codes were 64ths)
+      const size_t to = (size_t)(old_row0 + r) * p.out_ld;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = n * 8 + 2 * t + j;
-        if (r >= old_valid) continue;
-        const float a = 64.f * (j ? v.y : v.x), b = 64.f * (j ? v.w : v.z);       // (the codes were 64ths)
-        const size_t to = (size_t)(old_row0 + r) * p.out_ld;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (p.pair && h) continue;
-          const int f = p.pair ? old_strip * 8 + g : old_strip * 16 + g + 8 * h;
-          if (f >= p.F) continue;
-          const float y = p.pair ? silu(a) * b : h ? b : a;
-          if (p.out_f32) ((float*)p.out)[to + f] = p.residual ? y + ((const float*)p.residual)[to + f] : y;
-          else ((__nv_bfloat16*)p.out)[to + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[to + f]) : y);
-        }
+      for (int h = 0; h < 2; ++h) {
+        if (p.pair && h) continue;
+        const int f = p.pair ? old_strip * 8 + g : old_strip * 16 + g + 8 * h;
+        if (f >= p.F) continue;
+        const float y = p.pair ? silu(a) * b : h ? b : a;
+        if (p.out_f32) ((float*)p.out)[to + f] = p.residual ? y + ((const float*)p.residual)[to + f] : y;
+        else ((__nv_bfloat16*)p.out)[to + f] = __float2bfloat16(p.residual ? y + __bfloat162float(((const __nv_bfloat16*)p.residual)[to + f]) : y);
       }
     }
   };
@@ -200,9 +197,7 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_c
       if (left <= 0) break;
       if (i == 0) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[n][k] = 0.f;
+        for (int k = 0; k < 4; ++k) acc[k] = 0.f;
         if (staged != tile) {      // the rows of x of this tile
           while (tile >= pre[e + 1]) ++e;
           const int first = (tile - pre[e]) * p.x_stage, base = p.counts != nullptr ? p.offsets[e] : 0;
@@ -230,14 +225,13 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_c
             }
           }
           staged = tile;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) xb[n] = x_team + (size_t)min(n * 8 + g, valid - 1) * x_row + t * 16 + part * I4_STEP * 2;
+          xb = x_team + (size_t)min(g, valid - 1) * x_row + t * 16 + part * I4_STEP * 2;
           ir_team_sync<WK * 32>(team);
         }
       }
       const int at = i * (WK * I4_STEP * 2);
       constexpr int per = 4 / GP;               // quarters of a step in a group
-      float part_sum[NT][4];
+      float part_sum[4];
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {             // 32 of K each
@@ -245,22 +239,16 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_c
         const uint4 c = buf[d].c[q >> 1];
         i4_expand(q & 1 ? c.y : c.x, ZERO ? i4_zero(buf[d].z[ZERO ? grp : 0] & 0xff) : I4_EIGHT, lo);
         i4_expand(q & 1 ? c.w : c.z, ZERO ? i4_zero(buf[d].z[ZERO ? grp : 0] >> 8) : I4_EIGHT, hi);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4 b = *reinterpret_cast<const uint4*>(xb[n] + at + q * 64);
-          if (q % per == 0) ir_mma0(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-          else ir_mma(part_sum[n], lo[0], hi[0], lo[1], hi[1], b.x, b.y);
-          ir_mma(part_sum[n], lo[2], hi[2], lo[3], hi[3], b.z, b.w);
-        }
+        const uint4 b = *reinterpret_cast<const uint4*>(xb + at + q * 64);
+        if (q % per == 0) ir_mma0(part_sum, lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+        else ir_mma(part_sum, lo[0], hi[0], lo[1], hi[1], b.x, b.y);
+        ir_mma(part_sum, lo[2], hi[2], lo[3], hi[3], b.z, b.w);
         if (q % per == per - 1) {
           float sl, sh;
           if constexpr (HALF) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&buf[d].s[grp])); sl = f.x; sh = f.y; }
           else { sl = __uint_as_float(buf[d].s[grp] << 16); sh = __uint_as_float(buf[d].s[grp] & 0xffff0000u); }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[n][0] += sl * part_sum[n][0]; acc[n][1] += sl * part_sum[n][1];
-            acc[n][2] += sh * part_sum[n][2]; acc[n][3] += sh * part_sum[n][3];
-          }
+          acc[0] += sl * part_sum[0]; acc[1] += sl * part_sum[1];
+          acc[2] += sh * part_sum[2]; acc[3] += sh * part_sum[3];
         }
       }
       load(buf[d]);
@@ -274,8 +262,7 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_c
         __syncwarp();
         finish();
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) sums[n_done & 1][warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+      sums[n_done & 1][warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
       __syncwarp();
       if (WK > 1 && lane == 0) mbar_arrive(smem_u32(&bar[team]));
       ++n_done;
@@ -292,23 +279,23 @@ __global__ void __launch_bounds__(IR_THREADS, 1) int4_rows_kernel(const __grid_c
   }
 }
 
-template <int NT, int GP, bool ZERO, bool HALF, int WK>
+template <int GP, bool ZERO, bool HALF, int WK>
 static int launch_rows(Int4Rows p, cudaStream_t s) {
   static PerDevice allowed;
   constexpr int TEAMS = IR_WARPS / WK;
-  p.x_stage = min(8 * NT, p.rows);
+  p.x_stage = min(8, p.rows);
   while (p.x_stage > 0 && TEAMS * (p.x_stage * ir_x_row(p.steps)) > IR_SMEM) --p.x_stage;
   if (p.x_stage < 1 || ((long long)p.rows / p.x_stage + min(p.E, p.rows)) * p.strips > 0x7fffffffll) return -1;
-  const cudaError_t e = allow_smem(allowed, (const void*)int4_rows_kernel<NT, GP, ZERO, HALF, WK>, IR_SMEM);
+  const cudaError_t e = allow_smem(allowed, (const void*)int4_rows_kernel<GP, ZERO, HALF, WK>, IR_SMEM);
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(int4_rows_kernel<NT, GP, ZERO, HALF, WK>, dim3(148), dim3(IR_THREADS), (size_t)TEAMS * (p.x_stage * ir_x_row(p.steps)), s, p);
+  return (int)launch_pdl(int4_rows_kernel<GP, ZERO, HALF, WK>, dim3(148), dim3(IR_THREADS), (size_t)TEAMS * (p.x_stage * ir_x_row(p.steps)), s, p);
 }
 // Warps of a team: as many as leave each three steps or more of a strip, and more where its rows of x do not fit a smaller team's shared memory or the
 // strips are few (one row of 4096 x 4096, 256 strips: 7.3 us with 8 warps, 7.7 with 16, but four rows 8.9 and 8.8, and 1024 x 4096 5.9 and 5.3;
 // 28672 x 4096 25.2 and 27.7; 2048 x 1408 over experts 32.7 with 4, 34.8 with 8).
-template <int NT, int GP, bool ZERO, bool HALF>
+template <int GP, bool ZERO, bool HALF>
 static int pick_team(const Int4Rows& p, int team, cudaStream_t s) {
-  const int x = min(8 * NT, p.rows) * ir_x_row(p.steps);
+  const int x = min(8, p.rows) * ir_x_row(p.steps);
   const long long strips = (long long)p.strips * min(p.E, p.rows);
   if (team == 0)
     team = p.steps >= 48 || (p.steps >= 24 && strips <= 296 && (p.rows > 2 || strips <= 148)) || (p.steps >= 16 && x > IR_SMEM / 2)  ? 16
@@ -317,31 +304,30 @@ static int pick_team(const Int4Rows& p, int team, cudaStream_t s) {
                                                                 : 1;
   if (team > p.steps) return -1;
   switch (team) {
-    case 16: return launch_rows<NT, GP, ZERO, HALF, 16>(p, s);
-    case 8: return launch_rows<NT, GP, ZERO, HALF, 8>(p, s);
-    case 4: return launch_rows<NT, GP, ZERO, HALF, 4>(p, s);
-    case 1: return launch_rows<NT, GP, ZERO, HALF, 1>(p, s);
+    case 16: return launch_rows<GP, ZERO, HALF, 16>(p, s);
+    case 8: return launch_rows<GP, ZERO, HALF, 8>(p, s);
+    case 4: return launch_rows<GP, ZERO, HALF, 4>(p, s);
+    case 1: return launch_rows<GP, ZERO, HALF, 1>(p, s);
     default: return -1;
   }
 }
-template <int NT, int GP>
+template <int GP>
 static int pick_form(const Int4Rows& p, bool zero, bool half, int team, cudaStream_t s) {
-  if (zero) return half ? pick_team<NT, GP, true, true>(p, team, s) : pick_team<NT, GP, true, false>(p, team, s);
-  return half ? pick_team<NT, GP, false, true>(p, team, s) : pick_team<NT, GP, false, false>(p, team, s);
+  if (zero) return half ? pick_team<GP, true, true>(p, team, s) : pick_team<GP, true, false>(p, team, s);
+  return half ? pick_team<GP, false, true>(p, team, s) : pick_team<GP, false, false>(p, team, s);
 }
-template <int NT>
 static int pick_group(const Int4Rows& p, int group, bool zero, bool half, int team, cudaStream_t s) {
-  return group == 128 ? pick_form<NT, 1>(p, zero, half, team, s) : group == 64 ? pick_form<NT, 2>(p, zero, half, team, s) : pick_form<NT, 4>(p, zero, half, team, s);
+  return group == 128 ? pick_form<1>(p, zero, half, team, s) : group == 64 ? pick_form<2>(p, zero, half, team, s) : pick_form<4>(p, zero, half, team, s);
 }
 
 }  // namespace skein
 
 // x [x_rows, x_ld] bf16 (row r of the product reads row src_row[r], or r); w as in int4.cuh; out and residual [rows, out_ld] bf16
-// or fp32. counts / offsets null: one matrix for all rows. rows_hint: rows expected of an expert. flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
+// or fp32. counts / offsets null: one matrix for all rows. rows_hint is for the other kernel. flags: 1 pair, 2 fp16 scales, 4 fp32 output, 8 zeros.
 // team: warps that share a strip (1, 4, 8 or 16, at most its steps), 0: by the rule above. Returns -1 for what it does not take (more than IR_MAX_E experts,
 // a weight off 16-byte boundaries, or a row of x past the shared memory: K of 94,000).
 extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row, const void* w, const void* residual, void* out, long long out_ld,
-                               const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int rows_hint, int flags, int team,
+                               const int* counts, const int* offsets, int rows, int x_rows, int E, int F, int K, int group, int /*rows_hint*/, int flags, int team,
                                int* status, void* stream) {
   using namespace skein;
   if (rows == 0) return 0;
@@ -353,10 +339,9 @@ extern "C" int skein_int4_rows(const void* x, long long x_ld, const int* src_row
   p.budget_ns = (uint64_t)gemm_wait_budget_ms() * 1000000ull;
   p.pair = flags & 1;
   p.strips = p.pair ? (F + 7) / 8 : (F + 15) / 16;
-  p.tiles = (p.strips + 7) / 8;
   p.steps = (K + I4_STEP - 1) / I4_STEP;
   p.out_f32 = (flags >> 2) & 1;
   p.vec = x_ld % 8 == 0 && (uintptr_t)x % 16 == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  return rows_hint > 8 ? pick_group<2>(p, group, flags & 8, flags & 2, team, s) : pick_group<1>(p, group, flags & 8, flags & 2, team, s);
+  return pick_group(p, group, flags & 8, flags & 2, team, s);
 }

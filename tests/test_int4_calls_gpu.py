@@ -67,3 +67,54 @@ def test_captured_rows_off_16_bytes_follow_their_input():
         wide.copy_(acts(50, 400, seed=20 + seed))
         graph.replay()
         assert float(unit(y, x, full, 128).max()) <= 1
+
+
+ORDERS = [  # rows, features, K, group: long sums, where an allowance for a chain over all of K would let whole groups go missing
+    (1, 40, 98304, 128), (2, 33, 65536, 64), (3, 64, 14336, 128), (5, 70, 28672, 32), (8, 130, 8192, 128), (13, 300, 14336, 64), (40, 129, 16384, 128), (100, 64, 32768, 128),
+    (130, 200, 14336, 32)]
+
+
+@pytest.mark.parametrize("rows, features, K, group", ORDERS)
+def test_long_sums(rows, features, K, group):
+    w, full = weight((), features, K, group)
+    x = acts(rows, K)
+    y = int4.linear(x, w, out_f32=True)
+    assert float(unit(y, x, full, group).max()) <= 1
+    # what the bound is worth: without the last group most results are out of it
+    short = x.clone()
+    short[:, K - group:] = 0
+    assert float((unit(int4.linear(short, w, out_f32=True), x, full, group) > 1).float().mean()) > 0.5
+    w, full = weight((2,), features, K, group, zeros=False, scales=torch.float16)
+    cnt, off = torch.tensor([rows - rows // 3, rows // 3], dtype=torch.int32, device=DEV), torch.tensor([0, rows - rows // 3, rows], dtype=torch.int32, device=DEV)
+    y = int4.grouped_linear(x, w, cnt, off)
+    for e, part in ((0, slice(0, rows - rows // 3)), (1, slice(rows - rows // 3, rows))):
+        if part.start < part.stop:
+            assert float(unit(y[part], x[part], full[e], group, 2.0 ** -8).max()) <= 1
+    ops.workspace().check_status()
+
+
+@pytest.mark.parametrize("team", [1, 4, 8, 16])
+@pytest.mark.parametrize("rows, features, K, group", [(1, 16, 2048, 64), (7, 200, 2176, 128), (8, 1000, 2048, 32), (11, 150, 384, 128), (11, 96, 2176, 64), (19, 40, 640, 32), (30, 300, 1408, 128),
+                                                      (13, 70, 8192, 128), (29, 33, 16384, 64)])
+def test_teams_of_few_rows(rows, features, K, group, team):
+    """Every size of a team, with tiles of fewer than eight rows where a team's shared memory holds no more (K of 1408 with one warp, 8192 with four,
+    16384 with eight and sixteen), a last tile that is not full, and experts of unequal rows."""
+    steps = -(-K // 128)
+    row = steps * 256 + 64
+    if team > steps or 16 // team * row > 184 * 1024:
+        pytest.skip("a team of more warps than steps, or without room for a row")
+    w, full = weight((), features, K, group)
+    x = acts(rows, K)
+    y = int4.linear(x, w, out_f32=True, _cfg=(0, team))
+    assert float(unit(y, x, full, group).max()) <= 1
+    w, full = weight((4,), features, K, group, scales=torch.float16)
+    counts = [rows // 2, 0, 1, rows]
+    cnt = torch.tensor(counts, dtype=torch.int32, device=DEV)
+    off = torch.cat((cnt.new_zeros(1), cnt.cumsum(0))).to(torch.int32)
+    src = torch.randint(0, rows, (sum(counts),), generator=torch.Generator(device=DEV).manual_seed(4), device=DEV, dtype=torch.int32)
+    y = int4.grouped_linear(x, w, cnt, off, src_row=src, _cfg=(0, team))
+    for e in range(4):
+        part = slice(int(off[e]), int(off[e + 1]))
+        if counts[e]:
+            assert float(unit(y[part], x[src[part].long()], full[e], group, 2.0 ** -8).max()) <= 1
+    ops.workspace().check_status()

@@ -7,7 +7,7 @@
 // The bias steers the choice only. Scores are 64-bit: the choices of a step decide which rows meet which weights, and experts whose scores differ by
 // less than the error of a 32-bit exponential would be chosen by the build that computes them (with 256 experts one token in about 3000). A GPU of
 // this kind has the 64-bit rate for it. A logit that is not a number counts as the lowest; logits and biases are clamped to +-3e38, so that no
-// input makes an index invalid.
+// input makes an index invalid. (Compiled without fast-math, which would take subnormal biases and weights for zero.)
 //
 // A warp owns a token. Choices are kept as ordered 64-bit integers, all bits of them; a lane sorts its own with their places beside them, and a round of the
 // choice is a maximum over the lanes' heads: one instruction on the upper halves, two more where several lanes have the largest, and a minimum of the

@@ -39,8 +39,8 @@ ARCH_SOURCES = {
     "Derusun": ("attn_decode", "attn_decode_mma", "attn_latent_decode", "attn_latent_prefill", "attn_prefill_tc", "attn_window", "gemm_pair", "gemm_simt", "gemm_small",
                 "gemm_ws", "latent", "parallel_layer", "postnorm", "prenorm", "recurrent", "recurrent_channel_tc", "recurrent_tc", "rope_kv", "sample"),
 }
-# Sources compiled without fast-math: their exponentials, logarithms and tanh keep the accuracy of 32-bit.
-EXACT_SOURCES = ("attn_window", "parallel_layer", "prenorm", "recurrent", "recurrent_channel_tc", "recurrent_tc", "selective")
+# Sources compiled without fast-math: their exponentials, logarithms and tanh keep the accuracy of 32-bit (of route_balanced: subnormal numbers stay).
+EXACT_SOURCES = ("attn_window", "parallel_layer", "prenorm", "recurrent", "recurrent_channel_tc", "recurrent_tc", "route_balanced", "selective")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -61,3 +61,22 @@ def test_equal_scores_go_to_the_lower_index(E, top, dtype):
         got = experts.route_balanced(z.to(DEV, dtype), top, score=score)
         want = [sorted(range(E), key=lambda e: (-row[e], e))[:top] for row in z.tolist()]
         assert got[0].cpu().tolist() == want
+
+
+@pytest.mark.parametrize("T", [2, 300])
+def test_subnormal_numbers_count(T):
+    """Weights, biases and logits below the smallest normal number of 32 bits."""
+    z = torch.zeros(T, 24)
+    z[:, 1:] = -86.0 - torch.arange(23) * 0.75
+    ids, w, *_ = experts.route_balanced(z.to(DEV), 16, score="softmax", renorm=False)
+    want = ri.select_balanced(z, 16, None, 1, 1, "softmax", 2, False, 1.0)
+    assert torch.equal(ids.cpu(), want[0]) and bool((want[1][:, 4:] < 2.0 ** -126).all()) and bool((want[1] > 0).all())
+    # (a rounding of 64 bits on either side: a step of the value, or of the subnormal numbers)
+    assert torch.allclose(w.cpu().double(), want[1].double(), rtol=2.0 ** -23, atol=2.0 ** -149)
+    z = torch.full((T, 24), -800.0)              # scores of 0: the bias alone decides
+    bias = (torch.arange(24) % 7) * 2.0 ** -140
+    ids = experts.route_balanced(z.to(DEV), 9, bias=bias.to(DEV))[0]
+    assert torch.equal(ids.cpu(), ri.select_balanced(z, 9, bias, 1, 1, "sigmoid", 2, True, 1.0)[0])
+    z = (torch.arange(24) % 5).float().repeat(T, 1) * 2.0 ** -140       # (sigmoids of 1/2, softmaxes of 1/24, whatever the logits)
+    for score in experts.SCORES:
+        assert experts.route_balanced(z.to(DEV), 9, score=score)[0].cpu().tolist() == [list(range(9))] * T

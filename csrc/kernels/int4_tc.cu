@@ -167,6 +167,8 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       run += __shfl_sync(0xffffffffu, inc, 31);
     }
     if (lane == 0) pre[p.E] = run;
+    // (tiles that share their K have a place each; more of them are rows that belong to several experts)
+    if (SUB == 1 && p.split > 1 && lane == 0 && run > (int)gridDim.x / p.split) report_status(p.status, ST_BAD_INDEX, p.E);
     // A CTA walks whole tiles, every role at its own pace: the next tile's steps begin while the last one's results are stored. With two tiles a step
     // what does not fill a round is shared: `share` CTAs of a cluster take a piece of K each.
     if (SUB == 2 && lane == 0) {
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
   // The other shapes, which the plan would cost registers in their loops (3 to 8 %), take tiles `hop` apart from `first`, the same steps of each; the CTAs
   // of a cluster share all of theirs (one).
   const int total = pre[p.E], rank_of = SUB == 2 ? 0 : (int)blockIdx.x % p.split, first = SUB == 2 ? (int)blockIdx.x : (int)blockIdx.x / p.split;
-  const int hop = SUB == 2 ? (int)gridDim.x : (int)gridDim.x / p.split, end = SUB == 2 ? first + plan.items * hop : total;
+  const int hop = SUB == 2 ? (int)gridDim.x : (int)gridDim.x / p.split, end = SUB == 2 ? first + plan.items * hop : p.split > 1 ? min(total, hop) : total;
   const int s0 = SUB == 2 ? 0 : (int)((long long)p.steps * rank_of / p.split), s1 = SUB == 2 ? p.steps : (int)((long long)p.steps * (rank_of + 1) / p.split);
   struct Item { int u, s0, s1; };
   auto item_at = [&](int u) {
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(ItShape<NT, SUB>::THREADS, ItShape<NT, SUB>::O
       int st = group, slot = group;
       uint32_t ph = 0, sph = 0, seen = 0;
       // (a step is a step here, whatever tile it belongs to)
-      const int n_steps = SUB == 2 ? plan.n_steps : (total - first + hop - 1) / hop * (s1 - s0);
+      const int n_steps = SUB == 2 ? plan.n_steps : (end - first + hop - 1) / hop * (s1 - s0);
       for (int s = group; s < n_steps; s += GROUPS) {
         if (!it_warp_wait(seen, smem_u32(&bar_full[st]), ph, &abort_flag, p.budget_ns)) {
           if (lane == 0) { report_status(p.status, ST_TIMEOUT_SMEM_FULL, blockIdx.x); abort_flag = 1; }

@@ -118,3 +118,21 @@ def test_teams_of_few_rows(rows, features, K, group, team):
         if counts[e]:
             assert float(unit(y[part], x[src[part].long()], full[e], group, 2.0 ** -8).max()) <= 1
     ops.workspace().check_status()
+
+
+@pytest.mark.parametrize("cfg", [(16, 8), (32, 2), (64, 4), (128, 2)])
+def test_rows_of_several_experts_are_reported(cfg):
+    """Tiles that share their K have one place each: experts that claim the same rows make more tiles than places, which is told at once, not waited for."""
+    w, full = weight((4,), 200, 2048, 128)
+    x = acts(260, 2048)
+    cnt, off = torch.full((4,), 260, dtype=torch.int32, device=DEV), torch.zeros(4, dtype=torch.int32, device=DEV)
+    src = torch.arange(260, dtype=torch.int32, device=DEV)
+    for named in (None, src):
+        int4.grouped_linear(x, w, cnt, off, src_row=named, _cfg=cfg)
+        with pytest.raises(RuntimeError, match="out of range"):
+            ops.workspace().check_status()
+    cnt = torch.tensor([200, 0, 60, 0], dtype=torch.int32, device=DEV)
+    off = torch.tensor([0, 7, 200, 0], dtype=torch.int32, device=DEV)
+    y = int4.grouped_linear(x, w, cnt, off, _cfg=cfg)
+    assert float(unit(y[:200], x[:200], full[0], 128, 2.0 ** -8).max()) <= 1 and float(unit(y[200:], x[200:], full[2], 128, 2.0 ** -8).max()) <= 1
+    ops.workspace().check_status()

@@ -45,7 +45,7 @@ class Int4Weight:
             raise ValueError(f"int4 weight: data must be contiguous uint8 {want} on a 16-byte boundary")
         self.data, self.shape, self.group, self.pair = data, tuple(shape), group, pair
         self.scales, self.zeros = scales, zeros
-        self.K = shape[-1]
+        self.K, self.matrices = shape[-1], want[0]
         self.features = shape[-2] // 2 if pair else shape[-2]
         self.flags = int(pair) | (2 if scales == torch.float16 else 0) | (8 if zeros else 0)
 
@@ -61,10 +61,6 @@ class Int4Weight:
     @property
     def ptr(self):
         return self.data.data_ptr()
-
-    @property
-    def matrices(self):
-        return self.data.shape[0]
 
     def nbytes(self) -> int:
         return self.data.numel()
@@ -200,7 +196,7 @@ def _check(what, x, w: Int4Weight, pair, dims):
         raise ValueError(f"{what}: the weight is {'' if w.pair else 'not '}packed as a gate / up pair")
     if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != w.K or x.stride(1) != 1:
         raise ValueError(f"{what}: x must be bf16 [rows, {w.K}] with contiguous rows")
-    if x.device != w.device:
+    if x.device != w.data.device:
         raise ValueError(f"{what}: x is on {x.device}, the weight on {w.device}")
 
 
@@ -230,9 +226,12 @@ def _meet(a, b) -> bool:
 
 
 def _check_out(what, out, x, rows, w, dtype):
-    if out.shape != (rows, w.features) or out.dtype != dtype or out.device != w.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
+    if out.shape != (rows, w.features) or out.dtype != dtype or out.device != x.device or out.stride(1) != 1 or (rows > 1 and out.stride(0) < w.features):
         raise ValueError(f"{what}: out must be {dtype} [{rows}, {w.features}] with contiguous rows that do not overlap")
-    if _meet(out, x):
+    p, q = out.data_ptr(), x.data_ptr()
+    size = 4 if dtype is torch.float32 else 2
+    # (the spans first: a call that takes 10 us has no 2 for the rest)
+    if p < q + 2 * ((x.shape[0] - 1) * x.stride(0) + w.K) and q < p + size * ((rows - 1) * out.stride(0) + w.features) and _meet(out, x):
         raise ValueError(f"{what}: out lies on x, which is read until the end")
 
 
@@ -262,7 +261,7 @@ def _status(device) -> int:
 
 def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, rows, hint, flags, cfg=None):
     """cfg: None (the rule) or (n_tile, split) of the tensor-memory kernel, (0, team) of the kernel of few rows."""
-    L, dev = _lib.lib(), w.device
+    L, dev = _lib.lib(), x.device
     xp, x_ld = x.data_ptr(), x.stride(0) if x.shape[0] > 1 else w.K
     few = _few_rows(hint, w.K, counts is not None) if cfg is None else cfg[0] == 0
     if xp % 16 or x_ld % 8:
@@ -271,7 +270,7 @@ def _launch(what, x, w: Int4Weight, out, residual, counts, offsets, src_row, row
         if not few:     # (few rows are read two bytes at a time; 1000 rows of gate / up 18944 x 3584 so took 1770 us, laid out anew 253)
             x = x.clone(memory_format=torch.contiguous_format)
             xp, x_ld = x.data_ptr(), w.K
-    args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.ptr, None if residual is None else residual.data_ptr(), out.data_ptr(),
+    args = (xp, x_ld, None if src_row is None else src_row.data_ptr(), w.data.data_ptr(), None if residual is None else residual.data_ptr(), out.data_ptr(),
             out.stride(0), None if counts is None else counts.data_ptr(), None if counts is None else offsets.data_ptr(), rows, x.shape[0], w.matrices,
             w.features, w.K, w.group, hint, flags)
     if few:
@@ -299,7 +298,7 @@ def _dense(what, x, w, out, residual, out_f32, cfg):
     T = x.shape[0]
     dtype = torch.float32 if out_f32 else torch.bfloat16
     if out is None:
-        out = torch.empty((T, w.features), dtype=dtype, device=w.device)
+        out = torch.empty((T, w.features), dtype=dtype, device=x.device)
     else:
         _check_out(what, out, x, T, w, dtype)
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
@@ -320,7 +319,7 @@ def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None
     """Per-expert linear over expert-sorted rows. counts / offsets are int32 device tensors of E (offsets may have E + 1) entries: rows of expert e are
     offsets[e] : offsets[e] + counts[e] of the result, no row belongs to two. They read the same rows of x, or with src_row (int32, one entry per row of the result) rows
     src_row[r]: the tokens themselves, without a sorted copy. Rows not covered by any expert are left untouched (uninitialised in a result that the call
-    makes). rows_hint: rows expected over all experts, of which the choice of kernel depends (default: all of the result's)."""
+    makes); out shares no memory with x. rows_hint: rows expected over all experts, on which the choice of kernel depends (default: all of the result's)."""
     what = "int4 grouped_linear"
     _check(what, x, w, bool(swiglu), 3)
     E = w.shape[0]
@@ -331,7 +330,7 @@ def grouped_linear(x, w: Int4Weight, counts, offsets, swiglu=False, src_row=None
         raise ValueError(f"{what}: src_row must be int32 [rows] on x's device")
     rows = x.shape[0] if src_row is None else src_row.shape[0]
     if out is None:
-        out = torch.empty((rows, w.features), dtype=torch.bfloat16, device=w.device)
+        out = torch.empty((rows, w.features), dtype=torch.bfloat16, device=x.device)
     else:
         _check_out(what, out, x, rows, w, torch.bfloat16)
     if rows == 0:

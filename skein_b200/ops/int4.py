@@ -172,7 +172,7 @@ def pack_weight(codes, scale, zero=None, pair=False) -> Int4Weight:
 
 def quantize_weight(w: torch.Tensor, group: int = 128, symmetric: bool = True, pair: bool = False) -> Int4Weight:
     """Nearest codes of a weight [rows, K] or [experts, rows, K]. symmetric: a group's scale maps its largest magnitude to 7 (codes 1 .. 15 around 8);
-    else scale and zero map its range, zero included, onto 0 .. 15. Scales are bf16. K must be a multiple of the group."""
+    else scale and zero map its range, zero included, onto 0 .. 15. Scales are bf16. K must be a multiple of the group, the weight finite."""
     if w.dim() not in (2, 3) or group not in GROUPS or w.shape[-1] % group:
         raise ValueError(f"int4 weight: [.., rows, K] with K a multiple of the group ({GROUPS})")
     v = w.float().unflatten(-1, (-1, group))
@@ -181,6 +181,8 @@ def quantize_weight(w: torch.Tensor, group: int = 128, symmetric: bool = True, p
     else:
         lo, hi = v.amin(-1).clamp(max=0), v.amax(-1).clamp(min=0)
         s = (hi - lo) / 15
+    if not bool(s.isfinite().all()):
+        raise ValueError("int4 weight: a group holds what is not finite, or spans more than 32-bit numbers do")
     s = torch.where(s > 0, s, torch.ones_like(s)).to(torch.bfloat16)
     if not symmetric:
         zero = (-lo / s.float()).round().clamp(0, 15).to(torch.uint8)

@@ -135,3 +135,13 @@ def test_rows_outside_are_refused():
     unset = torch.tensor([1, 2, -7, 90], dtype=torch.int32)              # rows that no expert covers
     int4.grouped_linear(x, w, torch.tensor([2, 0], dtype=torch.int32), torch.tensor([0, -5], dtype=torch.int32), src_row=unset, out=out)
     assert bool((out[2:] == 3).all()) and not bool((out[:2] == 3).any())
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_weights_that_are_not_finite_are_not_quantised(value, symmetric):
+    w = torch.randn(2, 3, 128, generator=torch.Generator().manual_seed(4))
+    int4.quantize_weight(w, 64, symmetric)
+    w[1, 2, 70] = value
+    with pytest.raises(ValueError, match="finite"):
+        int4.quantize_weight(w, 64, symmetric)

@@ -59,4 +59,7 @@ def select_balanced(logits, top, bias, groups, keep, score, group_best, renorm, 
 
 def route_balanced(logits, top, bias, groups, keep, score, group_best, renorm, scale, e_first, e_count):
     ids, w = select_balanced(logits, top, bias, groups, keep, score, group_best, renorm, scale)
-    return (ids, w) + tuple(ref.router_plan(ids, logits.shape[1], e_first, e_count))
+    counts, offsets, row_of, src = ref.router_plan(ids, logits.shape[1], e_first, e_count)
+    src_token = src.new_zeros(row_of.shape)      # (of every pair, as on the GPU: a product's result has as many rows)
+    src_token[:int(offsets[-1])] = src[:int(offsets[-1])]
+    return ids, w, counts, offsets, row_of, src_token

@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from skein_b200.ops import int4
+from skein_b200.ops import experts, int4
 
 
 def small(lead=(), rows=16, K=64, pair=False, seed=0):
@@ -145,3 +145,16 @@ def test_weights_that_are_not_finite_are_not_quantised(value, symmetric):
     w[1, 2, 70] = value
     with pytest.raises(ValueError, match="finite"):
         int4.quantize_weight(w, 64, symmetric)
+
+
+@pytest.mark.parametrize("T, first, count", [(0, 0, 4), (5, 0, 4), (5, 1, 2), (5, 4, 0)])
+def test_a_layer_of_some_or_no_tokens_and_experts(T, first, count):
+    """The layout has an entry for every pair, whatever experts are this rank's: a layer's shapes are the GPU's."""
+    x = torch.randn(T, 64, generator=torch.Generator().manual_seed(6)).bfloat16()
+    ids, p, counts, offsets, row_of, src = experts.route_balanced(torch.randn(T, 4, generator=torch.Generator().manual_seed(7)), 2, e_first=first, e_count=count)
+    assert ids.shape == p.shape == (T, 2) and counts.shape == (4,) and offsets.shape == (5,) and row_of.shape == src.shape == (2 * T,)
+    y = int4.grouped_linear(x, small((4,), 16, 64), counts, offsets, src_row=src)
+    assert y.shape == (2 * T, 16)
+    mine = (ids.reshape(-1) >= first) & (ids.reshape(-1) < first + count)
+    assert int(offsets[-1]) == int(mine.sum()) and torch.equal(row_of >= 0, mine)
+    assert torch.equal(src[row_of[mine].long()], (torch.arange(2 * T, dtype=torch.int32) // 2)[mine])

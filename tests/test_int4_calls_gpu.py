@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from skein_b200 import ops
-from skein_b200.ops import int4, reference_int4 as ri
+from skein_b200.ops import experts, int4, reference_int4 as ri
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -135,4 +135,34 @@ def test_rows_of_several_experts_are_reported(cfg):
     off = torch.tensor([0, 7, 200, 0], dtype=torch.int32, device=DEV)
     y = int4.grouped_linear(x, w, cnt, off, _cfg=cfg)
     assert float(unit(y[:200], x[:200], full[0], 128, 2.0 ** -8).max()) <= 1 and float(unit(y[200:], x[200:], full[2], 128, 2.0 ** -8).max()) <= 1
+    ops.workspace().check_status()
+
+
+@pytest.mark.parametrize("cfg", [None, (0, 0), (16, 1), (16, 4), (128, 1)])
+def test_subnormal_fp16_scales(cfg):
+    """Scales below 2^-14, where fp16 has fewer bits, are taken as they are."""
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    codes = torch.randint(0, 256, (64, 128), generator=gen, device=DEV, dtype=torch.uint8)
+    scale = (torch.randint(1, 1024, (64, 4), generator=gen, device=DEV).float() * 2.0 ** -24).half()
+    w, full = int4.pack_weight(codes, scale), ri.dequant(codes, scale, None, 64).double()
+    assert bool((scale > 0).all()) and float(scale.max()) < 2.0 ** -14
+    x = acts(11, 256)
+    assert float(unit(int4.linear(x, w, out_f32=True, _cfg=cfg), x, full, 64).max()) <= 1
+
+
+@pytest.mark.parametrize("T, first, count", [(0, 0, 4), (5, 0, 4), (5, 1, 2), (5, 4, 0), (400, 3, 1)])
+def test_a_layer_of_some_or_no_tokens_and_experts(T, first, count):
+    w, full = weight((4,), 32, 256, 128)
+    x = acts(T, 256)
+    z = torch.randn(T, 4, generator=torch.Generator().manual_seed(7))
+    ids, p, counts, offsets, row_of, src = experts.route_balanced(z.to(DEV), 2, e_first=first, e_count=count)
+    assert ids.shape == p.shape == (T, 2) and counts.shape == (4,) and offsets.shape == (5,) and row_of.shape == src.shape == (2 * T,)
+    out = torch.full((2 * T, 32), 5.0, device=DEV, dtype=torch.bfloat16)
+    int4.grouped_linear(x, w, counts, offsets, src_row=src, out=out)
+    n = int(offsets[-1])
+    assert n == int(((ids >= first) & (ids < first + count)).sum()) and bool((out[n:] == 5).all())
+    for e in range(first, first + count):
+        part = slice(int(offsets[e]), int(offsets[e + 1]))
+        if part.start < part.stop:
+            assert float(unit(out[part], x[src[part].long()], full[e], 128, 2.0 ** -8).max()) <= 1
     ops.workspace().check_status()

@@ -12,12 +12,16 @@
 //   epilogue    takes a group's accumulator out of tensor memory, multiplies it by the row's scale and adds it to its registers, fp32
 // So no rounding happens before the result, whatever the scales are. (Scaled weights rounded to bf16 would need neither the ring nor the second sum,
 // but double the error of a product, and more for a gate / up pair.)
-// What bounds it: the handing over between the roles. A step (128 rows x 128 of K) takes a CTA about 1050 cycles whatever it holds; with the
-// conversion, the drains and seven of eight MMAs left out it still took 870. The MMAs of a step are 280 cycles with up to 64 rows of x and 512 with 128, the
-// weights' share of HBM is 365 cycles per SM. So with up to 64 rows two CTAs share an SM, with 16 rows two tiles of weights a step, handovers are whole
-// steps, and tests of barriers are issued before their answers are needed. Gathered rows are bounded by the two warps that copy them. Measured: 1000 rows of
-// gate / up 37888 x 3584 243 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 467 us (1.0 PFLOP/s), 13 rows of 152064 x 3584 83 us (3.7 TB/s),
-// 128 rows over 8 experts of 28672 x 4096, gathered, 160 us (3.0 TB/s).
+// What bounds it. A step (128 weight rows x 128 of K) takes, at 1.9 GHz:
+//   128 rows of x       about 1030 cycles of the SM's one CTA, 512 of them MMAs. No unit is full: the tensor pipe is active 54 % of the time, 64 % of the issue
+//                       slots are used, and 11.2 TB/s of operands leave L2 (41 KB a step: x comes again for each 128 features), 42 % of what it can hand over.
+//                       With the conversion, the drains and seven of eight MMAs left out, but all the loads, a step still took 870.
+//   32 rows, gathered   about 1560 cycles of a CTA, two of which share the SM: 780 a step. The two warps that copy the rows bound it.
+//   16 rows, two tiles  about 2800 cycles of a CTA for two tiles, two CTAs to an SM: 700 a tile's step; the weights' share of HBM is 365 to 390.
+// So with up to 64 rows two CTAs share an SM, with 16 rows two tiles of weights a step, handovers are whole steps, and tests of barriers are issued before
+// their answers are needed. Measured: 1000 rows of gate / up 37888 x 3584 244 us (1.1 PFLOP/s), 4096 rows over 8 experts of 4096 x 14336 468 us (1.0
+// PFLOP/s); called for seconds on end, when the power cap holds the clock at 1.55 to 1.6 GHz, 290 and 556 us (0.94 and 0.86). 13 rows of 152064 x 3584 84 us
+// (3.6 TB/s), 128 rows over 8 experts of 28672 x 4096, gathered, 160 us (3.0 TB/s).
 // Pieces of a tile meet in distributed shared memory in rank order: the result does not depend on timing, and no memory outlives the call.
 #include "int4.cuh"
 #include "launch.cuh"

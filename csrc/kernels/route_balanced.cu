@@ -15,7 +15,11 @@
 // 3250 instructions per token, 35 us). The layout is a counting sort that keeps the tokens' order: for every expert a CTA has one bit per token of its
 // tile, so that a pair's place among the tile's is a count of bits, whatever order the warps came in. Up to 256 tokens the tiles are the CTAs of one
 // cluster, which add their counts up in distributed shared memory; beyond, the first kernel leaves the tiles' counts in memory and a second one
-// finishes the places. One token takes 6.7 us with 128 experts, 64 tokens 7.2 with 64, 12.6 with 256 and 19.3 with 512, 4096 tokens of 256 26.1.
+// finishes the places. One token takes 6.7 us with 128 experts, 64 tokens 7.2 with 64, 12.7 with 256 and 19.5 with 512, 4096 tokens of 256 26.1.
+// What bounds it. A token of 256 experts is about 2250 instructions of its warp (2500 in a cluster). With 64 tokens they wait for one another, 11.7 cycles each,
+// with two warps on a scheduler: the chain is the time. With 4096 the eight warps of a scheduler fill 57 % of its issue slots (64 registers a thread allow
+// no more of them), which is 10 to 15 us; the second kernel, whose CTAs read all tiles' counts, waits for memory for most of the rest (31 of 39 cycles per
+// instruction), in part behind the first.
 #include "launch.cuh"
 #include "ptx.cuh"
 #include <cooperative_groups.h>

@@ -25,7 +25,8 @@ def route_balanced(logits, top, bias=None, groups=1, keep=1, score="sigmoid", gr
 
     Returns (ids int32 [T, top], weights fp32 [T, top], counts [E], offsets [E + 1], row_of [T * top], src_token [T * top]) as `ops.route` does: pair
     (t, j) sits at row_of[t * top + j] of the expert-sorted rows (-1: an expert outside e_first .. + e_count), src_token is its inverse; rows of
-    src_token from offsets[E] on are unset."""
+    src_token from offsets[E] on are unset. On a GPU the six lie in one allocation, which lives as long as any of them, and a call takes at most
+    227,328 tokens (148 tiles of 1536)."""
     dtype = logits.dtype
     if logits.dim() != 2 or dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("route_balanced: logits must be [tokens, experts] fp32 or bf16 with contiguous rows")

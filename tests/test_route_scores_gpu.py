@@ -80,3 +80,13 @@ def test_subnormal_numbers_count(T):
     z = (torch.arange(24) % 5).float().repeat(T, 1) * 2.0 ** -140       # (sigmoids of 1/2, softmaxes of 1/24, whatever the logits)
     for score in experts.SCORES:
         assert experts.route_balanced(z.to(DEV), 9, score=score)[0].cpu().tolist() == [list(range(9))] * T
+
+
+def test_as_many_tokens_as_a_call_takes():
+    T = 148 * 1536
+    z = torch.randn(T + 1, 3, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    ids, _, counts, offsets, row_of, src = experts.route_balanced(z[:T], 1)
+    assert torch.equal(ids[:, 0].long(), z[:T].double().sigmoid().argmax(1)) and int(offsets[-1]) == T
+    assert torch.equal(counts.long(), torch.bincount(ids[:, 0], minlength=3)) and torch.equal(src[row_of.long()], torch.arange(T, device=DEV, dtype=torch.int32))
+    with pytest.raises(ValueError, match="more than one call takes"):
+        experts.route_balanced(z, 1)

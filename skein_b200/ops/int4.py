@@ -299,14 +299,15 @@ def swiglu_linear(x, w: Int4Weight, out=None, _cfg=None):
 def _dense(what, x, w, out, residual, out_f32, cfg):
     T = x.shape[0]
     dtype = torch.float32 if out_f32 else torch.bfloat16
-    if out is None:
-        out = torch.empty((T, w.features), dtype=dtype, device=x.device)
-    else:
+    given = out is not None
+    if given:
         _check_out(what, out, x, T, w, dtype)
+    else:
+        out = torch.empty((T, w.features), dtype=dtype, device=x.device)
     if residual is not None and (residual.shape != out.shape or residual.dtype != out.dtype or residual.device != out.device
                                  or residual.stride(1) != 1 or (T > 1 and residual.stride(0) != out.stride(0))):
         raise ValueError(f"{what}: the residual must have the result's shape, type and strides")
-    if residual is not None and residual.data_ptr() != out.data_ptr() and _meet(residual, out):
+    if given and residual is not None and residual.data_ptr() != out.data_ptr() and _meet(residual, out):
         raise ValueError(f"{what}: the residual is out itself or lies beside it")
     if T == 0:
         return out
